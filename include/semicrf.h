@@ -28,7 +28,8 @@
  *
  * Conventions
  *  - All tensors are device pointers to contiguous row-major float32 (int64
- *    for lengths/labels) on the current CUDA device.
+ *    for lengths/labels) on the current CUDA device; the encoder operators
+ *    at the end of this file state their own types and strides.
  *  - The caller owns every buffer.  The library never allocates or frees
  *    device memory: scratch space is passed in, sized by the matching
  *    *_workspace_size query.
@@ -204,6 +205,118 @@ int semicrf_edge_scan_backward(int64_t B, int64_t N, int64_t K, int64_t C, const
  *    the library's device code into it; make that call before capturing any
  *    stream in that context. */
 int semicrf_forward_noalloc(const semicrf_problem* p, float* partition, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Encoder operators: what a gated recurrent encoder in front of the CRF head
+ * is made of.  They have no counterpart in the reference.
+ *
+ * Activations are (batch, time, channel) tensors of one type
+ * (semicrf_dtype), channels contiguous, the other two strides free (so a
+ * slice of a wider projection needs no copy).  All sums, states and
+ * statistics are float32; an output is rounded to its type once.  `lengths`
+ * (B,) may be NULL (every position is valid); positions at or past a
+ * sequence's length are never read into a result, give zeros and get zero
+ * gradients, whatever they hold.
+ * ------------------------------------------------------------------------- */
+enum semicrf_dtype { SEMICRF_F32 = 0, SEMICRF_BF16 = 1, SEMICRF_F16 = 2 };
+
+typedef struct semicrf_sequence {
+    void* data;              /* NULL where the tensor is absent */
+    int64_t batch_stride;    /* in elements */
+    int64_t time_stride;
+} semicrf_sequence;
+
+/* Gated linear recurrence: f = sigmoid(gate),
+ *   state_t = f_t * state_{t-1} + (1 - f_t) * x_t,   h_t = state_t,
+ * from initial_state (zeros if NULL) over the valid positions, ascending, or
+ * descending with reverse != 0. */
+typedef struct semicrf_recurrence {
+    int64_t batch, T, D;
+    int32_t dtype;               /* enum semicrf_dtype, of x, gate, h and their gradients */
+    int32_t reverse;
+    semicrf_sequence x, gate;    /* (B, T, D) */
+    const int64_t* lengths;      /* (B,) or NULL */
+    const float* initial_state;  /* (B, D) or NULL */
+} semicrf_recurrence;
+
+/* Bytes the forward keeps for the backward (the state at the start of each
+ * run of positions), and scratch bytes of either call. */
+size_t semicrf_recurrence_saved_size(const semicrf_recurrence* p);
+size_t semicrf_recurrence_workspace_size(const semicrf_recurrence* p);
+/* h (B, T, D) and final_state (B, D).  saved may be NULL when no backward follows. */
+int semicrf_recurrence_forward(const semicrf_recurrence* p, const semicrf_sequence* h,
+                               float* final_state, void* saved, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* Gradients of sum(grad_h * h) + sum(grad_state * final_state); grad_h.data
+ * or grad_state may be NULL (zeros).  grad_initial (B, D) may be NULL. */
+int semicrf_recurrence_backward(const semicrf_recurrence* p, const void* saved,
+                                const semicrf_sequence* grad_h, const float* grad_state,
+                                const semicrf_sequence* grad_x,
+                                const semicrf_sequence* grad_gate, float* grad_initial,
+                                void* workspace, size_t workspace_bytes, void* stream);
+/* One position of B independent streams: x, gate (B, D) with row strides,
+ * state and state_out (B, D) float32 (state_out may be state), h (B, D).
+ * active (B,) may be NULL; where it is 0 the state is kept and h is 0. */
+int semicrf_recurrence_step(int64_t B, int64_t D, int dtype, const void* x, int64_t x_stride,
+                            const void* gate, int64_t gate_stride, const uint8_t* active,
+                            const float* state, float* state_out, void* h, void* stream);
+
+/* Gated residual norm, per position over its D channels:
+ *   b = branch / rms(branch) * branch_weight
+ *   r = residual + residual_scale * silu(gate) * b
+ *   n = r / rms(r) * next_weight,        rms(v) = sqrt(mean(v^2) + eps).
+ * With branch.data NULL (gate.data, branch_weight and residual_scale then
+ * too) r is residual itself and only n is computed. */
+typedef struct semicrf_block_norm {
+    int64_t batch, T, D;
+    int32_t dtype;
+    float eps;
+    semicrf_sequence residual, branch, gate; /* (B, T, D) */
+    const float* branch_weight;              /* (D,) */
+    const float* residual_scale;             /* (D,) */
+    const float* next_weight;                /* (D,) */
+    const int64_t* lengths;                  /* (B,) or NULL */
+} semicrf_block_norm;
+
+/* residual_out r (not written without a branch) and normed n, (B, T, D).
+ * statistics (B, T, 2) float32 holds 1 / rms of branch and of r for the
+ * backward (may be NULL).  codes / scales: the 8-bit checkpoint of n
+ * (semicrf_pack's layout), or both NULL. */
+int semicrf_block_norm_forward(const semicrf_block_norm* p, const semicrf_sequence* residual_out,
+                               const semicrf_sequence* normed, float* statistics, int8_t* codes,
+                               uint8_t* scales, void* stream);
+size_t semicrf_block_norm_workspace_size(const semicrf_block_norm* p);
+/* grad_weights (3, D) float32: branch_weight, residual_scale, next_weight
+ * (only the last row is written without a branch).  grad_residual_out.data
+ * or grad_normed.data may be NULL (zeros). */
+int semicrf_block_norm_backward(const semicrf_block_norm* p, const float* statistics,
+                                const semicrf_sequence* grad_residual_out,
+                                const semicrf_sequence* grad_normed,
+                                const semicrf_sequence* grad_residual,
+                                const semicrf_sequence* grad_branch,
+                                const semicrf_sequence* grad_gate, float* grad_weights,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* 8-bit activation checkpoints.  Each position's channels are taken in groups
+ * of 32; a group stores the smallest e >= -126 with max |x| <= 127 * 2^e as
+ * the byte e + 127 and its values as int8 codes rint(x / 2^e), no code past
+ * the type's largest finite value.  A group of zeros has byte 0; one with a
+ * value that is not finite has byte 255 and reads back as NaN.
+ * codes (B*T, 32 * ceil(D/32)), zero beyond D; scales (B*T, ceil(D/32)). */
+int semicrf_pack(int64_t B, int64_t T, int64_t D, int dtype, const semicrf_sequence* x,
+                 const int64_t* lengths, int8_t* codes, uint8_t* scales, void* stream);
+/* out (rows, D), contiguous, of type dtype. */
+int semicrf_unpack(int64_t rows, int64_t D, int dtype, const int8_t* codes,
+                   const uint8_t* scales, void* out, void* stream);
+/* Gradient of a linear layer's weight from its input's checkpoint:
+ * out (M, D) = sum over valid positions of grad_output^T x, grad_output
+ * (B, T, M) of type dtype, out of type out_dtype. */
+size_t semicrf_packed_weight_grad_workspace_size(int64_t B, int64_t T, int64_t D, int64_t M,
+                                                 int dtype);
+int semicrf_packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
+                               const semicrf_sequence* grad_output, const int8_t* codes,
+                               const uint8_t* scales, const int64_t* lengths, int out_dtype,
+                               void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 const char* semicrf_strerror(int status);
 int semicrf_abi_version(void);

@@ -6,8 +6,14 @@ A drop-in for the reference's streaming hot path
 backed by hand-written sm_100a CUDA kernels in libsemicrf.so (C ABI:
 include/semicrf.h).  There is no Triton, no backend dispatch and no CPU
 fallback.
+
+Beside the head, the operators of a gated recurrent encoder in front of it:
+``gated_linear_recurrence`` (and its one-position ``_step``),
+``gated_residual_norm`` / ``rms_norm``, and 8-bit activation checkpoints
+(``pack_activation``, ``packed_linear``, ``packed_weight_grad``).
 """
 
+from .block_norm import gated_residual_norm, rms_norm
 from .duration import (
     CallableDuration,
     DurationDistribution,
@@ -20,6 +26,8 @@ from .duration import (
 )
 from .helpers import Segment, ViterbiResult, score_gold_vectorized
 from .nn import SemiMarkovCRFHead
+from .packed import PackedActivation, pack_activation, packed_linear, packed_weight_grad
+from .recurrence import gated_linear_recurrence, gated_linear_recurrence_step
 from .streaming import (
     NEG_INF,
     SemiCRFStreaming,
@@ -55,4 +63,12 @@ __all__ = [
     "NEG_INF",
     "UncertaintyMixin",
     "UncertaintySemiMarkovCRFHead",
+    "gated_linear_recurrence",
+    "gated_linear_recurrence_step",
+    "gated_residual_norm",
+    "rms_norm",
+    "PackedActivation",
+    "pack_activation",
+    "packed_linear",
+    "packed_weight_grad",
 ]

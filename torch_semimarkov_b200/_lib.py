@@ -98,7 +98,23 @@ EXPORTED_SYMBOLS = (
     "semicrf_edge_scan_forward",
     "semicrf_edge_scan_backward_workspace_size",
     "semicrf_edge_scan_backward",
+    "semicrf_recurrence_saved_size",
+    "semicrf_recurrence_workspace_size",
+    "semicrf_recurrence_forward",
+    "semicrf_recurrence_backward",
+    "semicrf_recurrence_step",
+    "semicrf_block_norm_forward",
+    "semicrf_block_norm_workspace_size",
+    "semicrf_block_norm_backward",
+    "semicrf_pack",
+    "semicrf_unpack",
+    "semicrf_packed_weight_grad_workspace_size",
+    "semicrf_packed_weight_grad",
 )
+
+# enum semicrf_dtype: the activation types of the encoder operators
+ACTIVATION_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+PACK_GROUP = 32  # channels that share a scale in an 8-bit checkpoint
 
 
 class SemicrfProblem(ctypes.Structure):
@@ -120,6 +136,51 @@ class SemicrfProblem(ctypes.Structure):
         ("checkpoint_interval", ctypes.c_int64),
         ("backward_mode", ctypes.c_int32),
         ("chunk_warmup", ctypes.c_int32),
+    ]
+
+
+class SemicrfSequence(ctypes.Structure):
+    """Mirror of ``struct semicrf_sequence``: a (batch, time, channel) tensor."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_int64),
+        ("time_stride", ctypes.c_int64),
+    ]
+
+
+class SemicrfRecurrence(ctypes.Structure):
+    """Mirror of ``struct semicrf_recurrence``."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("T", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reverse", ctypes.c_int32),
+        ("x", SemicrfSequence),
+        ("gate", SemicrfSequence),
+        ("lengths", ctypes.c_void_p),
+        ("initial_state", ctypes.c_void_p),
+    ]
+
+
+class SemicrfBlockNorm(ctypes.Structure):
+    """Mirror of ``struct semicrf_block_norm``."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("T", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("residual", SemicrfSequence),
+        ("branch", SemicrfSequence),
+        ("gate", SemicrfSequence),
+        ("branch_weight", ctypes.c_void_p),
+        ("residual_scale", ctypes.c_void_p),
+        ("next_weight", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
     ]
 
 
@@ -171,6 +232,32 @@ def load():
     lib.semicrf_edge_scan_forward.argtypes = [i64, i64, i64, i64, vp, vp, ci, vp, vp, vp]
     lib.semicrf_edge_scan_backward.restype = ci
     lib.semicrf_edge_scan_backward.argtypes = [i64, i64, i64, i64, vp, vp, ci, vp, vp, vp, vp,
+                                               sz, vp]
+    R, N, Q = (ctypes.POINTER(c) for c in (SemicrfRecurrence, SemicrfBlockNorm, SemicrfSequence))
+    for name, arg in (("semicrf_recurrence_saved_size", R),
+                      ("semicrf_recurrence_workspace_size", R),
+                      ("semicrf_block_norm_workspace_size", N)):
+        f = getattr(lib, name)
+        f.restype = sz
+        f.argtypes = [arg]
+    lib.semicrf_recurrence_forward.restype = ci
+    lib.semicrf_recurrence_forward.argtypes = [R, Q, vp, vp, vp, sz, vp]
+    lib.semicrf_recurrence_backward.restype = ci
+    lib.semicrf_recurrence_backward.argtypes = [R, vp, Q, vp, Q, Q, vp, vp, sz, vp]
+    lib.semicrf_recurrence_step.restype = ci
+    lib.semicrf_recurrence_step.argtypes = [i64, i64, ci, vp, i64, vp, i64, vp, vp, vp, vp, vp]
+    lib.semicrf_block_norm_forward.restype = ci
+    lib.semicrf_block_norm_forward.argtypes = [N, Q, Q, vp, vp, vp, vp]
+    lib.semicrf_block_norm_backward.restype = ci
+    lib.semicrf_block_norm_backward.argtypes = [N, vp, Q, Q, Q, Q, Q, vp, vp, sz, vp]
+    lib.semicrf_pack.restype = ci
+    lib.semicrf_pack.argtypes = [i64, i64, i64, ci, Q, vp, vp, vp, vp]
+    lib.semicrf_unpack.restype = ci
+    lib.semicrf_unpack.argtypes = [i64, i64, ci, vp, vp, vp, vp]
+    lib.semicrf_packed_weight_grad_workspace_size.restype = sz
+    lib.semicrf_packed_weight_grad_workspace_size.argtypes = [i64, i64, i64, i64, ci]
+    lib.semicrf_packed_weight_grad.restype = ci
+    lib.semicrf_packed_weight_grad.argtypes = [i64, i64, i64, i64, ci, Q, vp, vp, vp, ci, vp, vp,
                                                sz, vp]
     _lib = lib
     return lib
@@ -442,3 +529,249 @@ def edge_scan_backward(edge, lengths, semiring, saved, grad_output):
                                             _ptr(g), _ptr(ge), _ptr(ws), ws.numel(), _stream(dev))
         check(st, "semicrf_edge_scan_backward")
     return ge
+
+
+# ---------------------------------------------------------------------------
+# encoder operators
+# ---------------------------------------------------------------------------
+def activation(t, name: str, shape=None, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A checked (batch, time, channel) activation whose channels are contiguous
+    (copied where they are not; the other strides stay as they are)."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        raise ValueError(f"{name} must be a (batch, time, channel) tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"torch_semimarkov_b200 runs on CUDA devices only ({name} is on the "
+                           "CPU; there is no CPU fallback)")
+    if t.dtype not in ACTIVATION_DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if like is not None:
+        if t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+        if t.dtype != like.dtype:
+            raise ValueError(f"{name} is {t.dtype}, expected {like.dtype}")
+        if shape is None:
+            shape = like.shape
+    if shape is not None and t.shape != torch.Size(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.shape[2] < 1:
+        raise ValueError(f"{name} has no channels")
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def float_vector(t, name: str, shape, device) -> torch.Tensor:
+    """A checked float32 copy (or the tensor itself) of a parameter or state."""
+    if not isinstance(t, torch.Tensor) or not t.is_floating_point():
+        raise ValueError(f"{name} must be a floating-point tensor")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.shape != torch.Size(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t.to(torch.float32).contiguous()
+
+
+def valid_lengths(lengths, B: int, T: int, device) -> Optional[torch.Tensor]:
+    """lengths (B,) as int64 on the device, or None.  Values on the CPU are
+    checked to lie in [0, T]; the kernels clamp those already on the device."""
+    if lengths is None:
+        return None
+    if not isinstance(lengths, torch.Tensor):
+        lengths = torch.as_tensor(lengths)
+    if lengths.shape != (B,) or lengths.is_floating_point():
+        raise ValueError(f"lengths must be a ({B},) integer tensor")
+    if lengths.device.type == "cpu" and B > 0:
+        lo, hi = int(lengths.min()), int(lengths.max())
+        if lo < 0 or hi > T:
+            raise ValueError(f"lengths must lie in [0, {T}], got [{lo}, {hi}]")
+    return lengths.to(device=device, dtype=torch.int64).contiguous()
+
+
+def _sequence(t: Optional[torch.Tensor]) -> SemicrfSequence:
+    if t is None:
+        return SemicrfSequence(None, 0, 0)
+    return SemicrfSequence(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+class _SameDevice:
+    """The context of a call on the device that is current already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def _on(device):
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
+def _recurrence(x, gate, initial_state, lengths, reverse) -> SemicrfRecurrence:
+    B, T, D = x.shape
+    return SemicrfRecurrence(B, T, D, ACTIVATION_DTYPES[x.dtype], int(bool(reverse)),
+                             _sequence(x), _sequence(gate), _addr(lengths), _addr(initial_state))
+
+
+def recurrence_forward(x, gate, initial_state, lengths, reverse, want_saved):
+    """semicrf_recurrence_forward.  Returns (h, final_state, saved or None)."""
+    lib = load()
+    B, T, D = x.shape
+    dev = x.device
+    p = _recurrence(x, gate, initial_state, lengths, reverse)
+    with _on(dev):
+        h = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        state = torch.empty((B, D), dtype=torch.float32, device=dev)
+        saved = _scratch(lib.semicrf_recurrence_saved_size(p), dev) if want_saved else None
+        ws = _scratch(lib.semicrf_recurrence_workspace_size(p), dev)
+        st = lib.semicrf_recurrence_forward(p, _sequence(h), state.data_ptr(), _addr(saved),
+                                            ws.data_ptr(), ws.numel(), _stream(dev))
+        check(st, "semicrf_recurrence_forward")
+    return h, state, saved
+
+
+def recurrence_backward(x, gate, lengths, reverse, saved, grad_h, grad_state, want_initial):
+    """semicrf_recurrence_backward.  Returns (grad_x, grad_gate, grad_initial or None)."""
+    lib = load()
+    B, T, D = x.shape
+    dev = x.device
+    p = _recurrence(x, gate, None, lengths, reverse)
+    with _on(dev):
+        gx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        gg = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        gi = torch.empty((B, D), dtype=torch.float32, device=dev) if want_initial else None
+        ws = _scratch(lib.semicrf_recurrence_workspace_size(p), dev)
+        st = lib.semicrf_recurrence_backward(p, saved.data_ptr(), _sequence(grad_h),
+                                             _addr(grad_state), _sequence(gx), _sequence(gg),
+                                             _addr(gi), ws.data_ptr(), ws.numel(), _stream(dev))
+        check(st, "semicrf_recurrence_backward")
+    return gx, gg, gi
+
+
+def recurrence_step(x, gate, state, active, state_out):
+    """semicrf_recurrence_step.  Returns (h, state_out)."""
+    lib = load()
+    B, D = x.shape
+    dev = x.device
+    with _on(dev):
+        h = torch.empty((B, D), dtype=x.dtype, device=dev)
+        if state_out is None:
+            state_out = torch.empty((B, D), dtype=torch.float32, device=dev)
+        st = lib.semicrf_recurrence_step(B, D, ACTIVATION_DTYPES[x.dtype], x.data_ptr(),
+                                         x.stride(0), gate.data_ptr(), gate.stride(0),
+                                         _addr(active), state.data_ptr(), state_out.data_ptr(),
+                                         h.data_ptr(), _stream(dev))
+        check(st, "semicrf_recurrence_step")
+    return h, state_out
+
+
+def _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
+                eps) -> SemicrfBlockNorm:
+    B, T, D = residual.shape
+    return SemicrfBlockNorm(B, T, D, ACTIVATION_DTYPES[residual.dtype], float(eps),
+                            _sequence(residual), _sequence(branch), _sequence(gate),
+                            _addr(branch_weight), _addr(residual_scale), _addr(next_weight),
+                            _addr(lengths))
+
+
+def packed_buffers(B: int, T: int, D: int, device):
+    """Codes (B, T, 32 * ceil(D/32)) int8 and scales (B, T, ceil(D/32)) uint8."""
+    G = -(-D // PACK_GROUP)
+    return (torch.empty((B, T, G * PACK_GROUP), dtype=torch.int8, device=device),
+            torch.empty((B, T, G), dtype=torch.uint8, device=device))
+
+
+def block_norm_forward(residual, branch, gate, branch_weight, residual_scale, next_weight,
+                       lengths, eps, want_statistics, pack):
+    """semicrf_block_norm_forward.  Returns (residual_out or None without a
+    branch, normed, statistics or None, codes or None, scales or None)."""
+    lib = load()
+    B, T, D = residual.shape
+    dev = residual.device
+    p = _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
+                    eps)
+    with _on(dev):
+        out = None if branch is None else torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+        normed = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+        stats = (torch.empty((B, T, 2), dtype=torch.float32, device=dev) if want_statistics
+                 else None)
+        codes, scales = packed_buffers(B, T, D, dev) if pack else (None, None)
+        st = lib.semicrf_block_norm_forward(p, _sequence(out), _sequence(normed), _addr(stats),
+                                            _addr(codes), _addr(scales), _stream(dev))
+        check(st, "semicrf_block_norm_forward")
+    return out, normed, stats, codes, scales
+
+
+def block_norm_backward(residual, branch, gate, branch_weight, residual_scale, next_weight,
+                        lengths, eps, stats, grad_out, grad_normed):
+    """semicrf_block_norm_backward.  Returns (grad_residual, grad_branch or
+    None, grad_gate or None, grad_weights (3, D) float32)."""
+    lib = load()
+    B, T, D = residual.shape
+    dev = residual.device
+    p = _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
+                    eps)
+    with _on(dev):
+        gr = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+        gb = gg = None
+        if branch is not None:
+            gb = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+            gg = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+        gw = torch.empty((3, D), dtype=torch.float32, device=dev)
+        ws = _scratch(lib.semicrf_block_norm_workspace_size(p), dev)
+        st = lib.semicrf_block_norm_backward(p, stats.data_ptr(), _sequence(grad_out),
+                                             _sequence(grad_normed), _sequence(gr), _sequence(gb),
+                                             _sequence(gg), gw.data_ptr(), ws.data_ptr(),
+                                             ws.numel(), _stream(dev))
+        check(st, "semicrf_block_norm_backward")
+    return gr, gb, gg, gw
+
+
+def pack(x, lengths):
+    """semicrf_pack.  Returns (codes, scales)."""
+    lib = load()
+    B, T, D = x.shape
+    dev = x.device
+    with _on(dev):
+        codes, scales = packed_buffers(B, T, D, dev)
+        st = lib.semicrf_pack(B, T, D, ACTIVATION_DTYPES[x.dtype], _sequence(x), _addr(lengths),
+                              codes.data_ptr(), scales.data_ptr(), _stream(dev))
+        check(st, "semicrf_pack")
+    return codes, scales
+
+
+def unpack(codes, scales, D: int, dtype):
+    """semicrf_unpack.  Returns the (B, T, D) values."""
+    lib = load()
+    B, T = codes.shape[:2]
+    dev = codes.device
+    with _on(dev):
+        out = torch.empty((B, T, D), dtype=dtype, device=dev)
+        st = lib.semicrf_unpack(B * T, D, ACTIVATION_DTYPES[dtype], codes.data_ptr(),
+                                scales.data_ptr(), out.data_ptr(), _stream(dev))
+        check(st, "semicrf_unpack")
+    return out
+
+
+def packed_weight_grad(grad_output, codes, scales, D: int, lengths, out_dtype):
+    """semicrf_packed_weight_grad.  Returns the (M, D) gradient."""
+    lib = load()
+    B, T, M = grad_output.shape
+    dev = grad_output.device
+    dt = ACTIVATION_DTYPES[grad_output.dtype]
+    with _on(dev):
+        out = torch.empty((M, D), dtype=out_dtype, device=dev)
+        ws = _scratch(lib.semicrf_packed_weight_grad_workspace_size(B, T, D, M, dt), dev)
+        st = lib.semicrf_packed_weight_grad(B, T, D, M, dt, _sequence(grad_output),
+                                            codes.data_ptr(), scales.data_ptr(), _addr(lengths),
+                                            ACTIVATION_DTYPES[out_dtype], out.data_ptr(),
+                                            ws.data_ptr(), ws.numel(), _stream(dev))
+        check(st, "semicrf_packed_weight_grad")
+    return out

@@ -19,7 +19,7 @@ LIB = os.path.join(HERE, "libsemicrf.so")
 PROBE_LIB = os.path.join(HERE, "libsemicrf_probe.so")
 PROBE_SOURCES = ["probe.cu"]
 SOURCES = ["api.cu", "chain.cu", "lchain.cu", "lchain_ws.cu", "lchain_fix.cu", "lchain_cl.cu", "lchunk.cu", "lmarg.cu", "marginals.cu", "viterbi.cu", "vchain.cu", "kcc.cu", "kblk.cu", "escan.cu", "gold.cu",
-           "noalloc.cu"]
+           "noalloc.cu", "encoder_api.cu", "recurrence.cu", "blocknorm.cu", "packed.cu", "packgrad.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",

@@ -1,0 +1,174 @@
+// Internal declarations of the encoder operators: the gated linear recurrence
+// (recurrence.cu), the gated residual norm (blocknorm.cu) and the 8-bit
+// activation checkpoints (packed.cu, packgrad.cu).
+//
+// Activations are float32, bfloat16 or float16 (semicrf_dtype); every sum,
+// state and statistic is float32, and a value is rounded to its type once,
+// when it is stored.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/semicrf.h"
+
+namespace semicrf {
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// N values of T that are loaded and stored together
+template <class T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+// A (batch, time, channel) tensor: contiguous channels, strides in elements.
+template <class T>
+struct Seq {
+  T* p;
+  int64_t sb, st;
+  __device__ __forceinline__ T* row(int64_t b, int64_t t) const { return p + b * sb + t * st; }
+};
+template <class T>
+Seq<T> as_seq(const semicrf_sequence& s) {
+  return Seq<T>{static_cast<T*>(s.data), s.batch_stride, s.time_stride};
+}
+
+// True when every row of s can be read in vectors of n elements.
+inline bool seq_aligned(const semicrf_sequence& s, int64_t B, int64_t T, int elem, int n) {
+  if (!s.data) return true;
+  return reinterpret_cast<uintptr_t>(s.data) % ((uintptr_t)elem * n) == 0 &&
+         (B <= 1 || s.batch_stride % n == 0) && (T <= 1 || s.time_stride % n == 0);
+}
+
+// Number of valid positions of sequence b (all T without lengths).
+__device__ __forceinline__ int64_t valid_length(const int64_t* lengths, int64_t b, int64_t T) {
+  if (!lengths) return T;
+  const int64_t n = lengths[b];
+  return n < 0 ? 0 : (n > T ? T : n);
+}
+
+// sigmoid(g) and sigmoid(-g), each to a few units of its own last place: with
+// e = exp(-|g|) both are quotients over 1 + e, so neither cancels.
+__device__ __forceinline__ void sigmoid_pair(float g, float& pos, float& neg) {
+  const float e = __expf(-fabsf(g));
+  const float hi = __fdividef(1.f, 1.f + e);
+  const float lo = e * hi;
+  pos = g < 0.f ? lo : hi;
+  neg = g < 0.f ? hi : lo;
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit checkpoints: 32 channels of a position share the scale 2^e, e + 127 in
+// a byte.  A power of two costs up to one bit against a free scale, and makes
+// both directions exact operations: the codes do not depend on how a division
+// rounds, and a decoded value has 7 bits, so it is exact in bfloat16.
+// ---------------------------------------------------------------------------
+constexpr int kPackGroup = 32;
+__host__ __device__ inline int64_t pack_groups(int64_t D) {
+  return (D + kPackGroup - 1) / kPackGroup;
+}
+
+template <class T>
+__device__ __forceinline__ float largest_finite();
+template <>
+__device__ __forceinline__ float largest_finite<float>() { return 3.402823466e38f; }
+template <>
+__device__ __forceinline__ float largest_finite<__nv_bfloat16>() { return 3.389531390e38f; }
+template <>
+__device__ __forceinline__ float largest_finite<__half>() { return 65504.f; }
+
+__device__ __forceinline__ float pack_scale(uint8_t byte) {  // 255 (inf) times code 0 is NaN
+  return __int_as_float((int)byte << 23);
+}
+
+// Codes of a group whose values lie V to a lane in 32 / V neighbouring lanes
+// (all lanes of the warp call this); returns the scale byte.
+template <class T, int V>
+__device__ __forceinline__ uint8_t pack_encode(const float (&v)[V], int8_t (&q)[V]) {
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 1; o < kPackGroup / V; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+  // top = m 2^p, 1/2 <= m < 1, exponent field p + 126: e is p - 7 where m <= 127/128, else p - 6
+  const int field = (int)(top >> 23);
+  int byte = field - 6 + ((top & 0x7fffffu) > 0x7e0000u);
+  byte = byte < 1 ? 1 : byte;
+  if (top == 0) byte = 0;
+  const bool finite = field < 255;
+  if (!finite) byte = 255;
+  const float inv = __int_as_float((254 - (finite ? byte : 254)) << 23);
+  const float most = fminf(127.f, floorf(largest_finite<T>() * inv));
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float r = fminf(fmaxf(rintf(v[j] * inv), -most), most);
+    q[j] = finite ? (int8_t)(int)r : (int8_t)0;
+  }
+  return (uint8_t)byte;
+}
+
+inline int launch_status() {
+  return cudaGetLastError() == cudaSuccess ? SEMICRF_OK : SEMICRF_ERR_CUDA;
+}
+
+// recurrence.cu
+size_t recurrence_saved_bytes(const semicrf_recurrence* p);
+size_t recurrence_workspace_bytes(const semicrf_recurrence* p);
+int recurrence_forward(const semicrf_recurrence* p, const semicrf_sequence& h, float* final_state,
+                       void* saved, void* workspace, cudaStream_t stream);
+int recurrence_backward(const semicrf_recurrence* p, const void* saved,
+                        const semicrf_sequence& grad_h, const float* grad_state,
+                        const semicrf_sequence& grad_x, const semicrf_sequence& grad_gate,
+                        float* grad_initial, void* workspace, cudaStream_t stream);
+int recurrence_step(int64_t B, int64_t D, int dtype, const void* x, int64_t x_stride,
+                    const void* gate, int64_t gate_stride, const uint8_t* active,
+                    const float* state, float* state_out, void* h, cudaStream_t stream);
+
+// blocknorm.cu
+size_t block_norm_workspace_bytes(const semicrf_block_norm* p);
+int block_norm_forward(const semicrf_block_norm* p, const semicrf_sequence& residual_out,
+                       const semicrf_sequence& normed, float* statistics, int8_t* codes,
+                       uint8_t* scales, cudaStream_t stream);
+int block_norm_backward(const semicrf_block_norm* p, const float* statistics,
+                        const semicrf_sequence& grad_residual_out,
+                        const semicrf_sequence& grad_normed, const semicrf_sequence& grad_residual,
+                        const semicrf_sequence& grad_branch, const semicrf_sequence& grad_gate,
+                        float* grad_weights, void* workspace, cudaStream_t stream);
+
+// packed.cu
+int pack_rows(int64_t B, int64_t T, int64_t D, int dtype, const semicrf_sequence& x,
+              const int64_t* lengths, int8_t* codes, uint8_t* scales, cudaStream_t stream);
+int unpack_rows(int64_t rows, int64_t D, int dtype, const int8_t* codes, const uint8_t* scales,
+                void* out, cudaStream_t stream);
+
+// packgrad.cu
+size_t packed_weight_grad_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t M, int dtype);
+int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
+                       const semicrf_sequence& grad_output, const int8_t* codes,
+                       const uint8_t* scales, const int64_t* lengths, int out_dtype, void* out,
+                       void* workspace, cudaStream_t stream);
+
+}  // namespace semicrf
