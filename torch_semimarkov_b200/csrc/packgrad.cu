@@ -1,8 +1,30 @@
 // packgrad.cu -- the gradient of a linear layer's weight from the 8-bit
-// checkpoint of its input: out (M, D) = sum_n dy[n, :]^T x[n, :].
+// checkpoint of its input: out (M, D) = sum over positions n of dy[n, :]^T x[n, :].
 //
-// A CTA of 256 threads owns 64 x 64 outputs and a run of positions, 4 x 4
-// outputs to a thread; runs are summed by a second kernel in order.
+// A matrix product over positions, on the tensor cores (tcgen05.mma,
+// kind::f16, bfloat16 operands, float32 accumulators in tensor memory).  Both
+// operands lie in memory with their channels contiguous, so both are
+// MN-major; a position is one row of the shared-memory tile.
+//
+// x: a code times a power of two has 7 bits, so its bfloat16 value is exact.
+// dy: bfloat16 as it is; float16 and float32 are cut into 2 and 3 bfloat16
+// pieces of 8 bits each (exact: 11 and 24 bits), one product each.  So every
+// product is exact and only the float32 sums round.
+//
+// Tiles: 256 x 256 outputs to a pair of CTAs (cta_group::2: a CTA brings 128
+// channels of either operand, so each code is decoded for 256 outputs), or
+// 128 x 128 to one CTA where M or D is at most 128 and for float32.  Each
+// tile takes a run of positions; the runs' partial results are summed in
+// order by a second kernel.
+//
+// Roles: producer warps fill a ring of stages of 64 positions, dy by 16-byte
+// asynchronous copies straight into the swizzled tile (bfloat16 rows on
+// 16-byte boundaries) or through registers, codes through registers; both
+// are requested kLook stages before they are needed.  One thread issues the
+// products.  The tensor cores truncate their float32 sums (measured: 1.8e-8
+// of the result for each 16 positions), which is nothing beside 16-bit dy.
+// For float32 the leading piece is summed apart from the others and, every
+// 512 positions, moved from tensor memory to registers that round to nearest.
 
 #include <algorithm>
 
@@ -13,116 +35,583 @@ int device_sm_count();  // api.cu
 
 namespace {
 
-constexpr int kTileOut = 64, kStep = 16;
+constexpr int kTile = 128;      // channels of dy, and of x, that a CTA brings
+constexpr int kStep = 64;       // positions of a stage
+constexpr int kAtom = kStep * 128;  // bytes of 64 channels of a stage: 64 rows of 128
+constexpr int kOperand = 2 * kAtom; // bytes of an operand of a stage
+constexpr int kWarps = 16;      // producers and readers of tensor memory; one more issues
+constexpr int kSegment = 8;     // float32: stages that tensor memory sums
+constexpr unsigned kWaitLimit = 1u << 22;
 
 template <class T>
-__global__ void __launch_bounds__(256) weight_grad_kernel(int64_t N, int64_t T_, int64_t D, int64_t M,
-                                                          int64_t run, Seq<const T> dy,
-                                                          const int8_t* __restrict__ codes,
-                                                          const uint8_t* __restrict__ scales,
-                                                          const int64_t* __restrict__ lengths,
-                                                          float* __restrict__ partial) {
-  __shared__ float a[kStep][kTileOut], x[kStep][kTileOut];
-  const int64_t m0 = (int64_t)blockIdx.x * kTileOut, d0 = (int64_t)blockIdx.y * kTileOut;
-  const int64_t G = pack_groups(D);
-  const int64_t first = blockIdx.z * run, last = first + run < N ? first + run : N;
-  const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-  const int tm = (threadIdx.x >> 4) * 4, td = (threadIdx.x & 15) * 4;
-  float acc[4][4] = {};
-  for (int64_t n0 = first; n0 < last; n0 += kStep) {
+struct Form;  // pieces of a value; producer warps; warps that read tensor memory
+template <>
+struct Form<__nv_bfloat16> { static constexpr int pieces = 1, producers = 16, readers = 16; };
+template <>
+struct Form<__half> { static constexpr int pieces = 2, producers = 16, readers = 16; };
+template <>
+struct Form<float> { static constexpr int pieces = 3, producers = 8, readers = 8; };
+
+template <class T>
+struct Shape {
+  static constexpr int kStage = (Form<T>::pieces + 1) * kOperand;
+  static constexpr int kStages = 200 * 1024 / kStage < 6 ? 200 * 1024 / kStage : 6;
+  static constexpr int kBytes = kStages * kStage + 1024;  // and room to align
+};
+
+// Division by a fixed T for values below 2^31: multiply by a rounded-up
+// reciprocal and shift (Granlund and Montgomery).
+struct Divider {
+  unsigned d, mul, shift;
+};
+Divider make_divider(unsigned d) {
+  unsigned s = 0;
+  while ((1ull << s) < d) ++s;
+  return Divider{d, (unsigned)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+__device__ __forceinline__ unsigned quotient(unsigned n, const Divider& v) {
+  return (__umulhi(n, v.mul) + n) >> v.shift;
+}
+
+struct GradArgs {
+  int64_t N, M, Dp, G;  // positions, width of dy, code row bytes, scale row bytes
+  int64_t run;          // positions of a tile, a multiple of kStep
+  const void* dy;
+  int64_t sb, st;
+  bool vec;             // rows of dy start on 16-byte boundaries
+  const int8_t* codes;
+  const uint8_t* scales;
+  const int64_t* lengths;
+  unsigned T_;
+  Divider by_t;
+  int tiles_m, tiles_d;  // of 128 rows; of 128 CG columns
+  float* partial;  // (runs, tiles_m, tiles_d, 128 CG, 128): a tile's columns one after another
+};
+
+__device__ __forceinline__ unsigned smem_addr(const void* p) {
+  return (unsigned)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void barrier_init(uint64_t* b, unsigned n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ unsigned peer_addr(unsigned addr, unsigned rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// Arrives on the barrier of the pair's first CTA (its own without a pair).
+template <int CG>
+__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
+  if (CG == 1)
+    asm volatile("{.reg .b64 t; mbarrier.arrive.shared::cta.b64 t, [%0];}" ::"r"(smem_addr(b))
+                 : "memory");
+  else
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                     peer_addr(smem_addr(b), 0))
+                 : "memory");
+}
+// False when the phase does not complete within the limit.
+__device__ __forceinline__ bool barrier_wait(uint64_t* b, unsigned parity) {
+  for (unsigned k = 0; k < kWaitLimit; ++k) {
+    unsigned done;
+    asm volatile(
+        "{.reg .pred p;"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;"
+        "selp.u32 %0, 1, 0, p;}"
+        : "=r"(done)
+        : "r"(smem_addr(b)), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// The barrier (of both CTAs of a pair) completes when the products issued so far have.
+template <int CG>
+__device__ __forceinline__ void commit_to(uint64_t* b) {
+  if (CG == 1)
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+            smem_addr(b))
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_addr(b)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void product(unsigned d, uint64_t a, uint64_t b, bool add) {
+  // float32 accumulator, bfloat16 operands, both MN-major, 128 CG x 128 CG
+  constexpr unsigned kind = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
+                            ((unsigned)(kTile * CG >> 3) << 17) |
+                            ((unsigned)(kTile * CG >> 4) << 24);
+  if (CG == 1)
+    asm volatile(
+        "{.reg .pred p; setp.ne.u32 p, %4, 0;"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d),
+        "l"(a), "l"(b), "r"(kind), "r"((unsigned)add)
+        : "memory");
+  else
+    asm volatile(
+        "{.reg .pred p; setp.ne.u32 p, %4, 0;"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d),
+        "l"(a), "l"(b), "r"(kind), "r"((unsigned)add)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void sync_all() {  // the CTA, or the pair
+  if (CG == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+// 16 columns of this warp's 32 rows of tensor memory, one row a lane
+__device__ __forceinline__ void read_columns(unsigned at, float (&f)[16]) {
+  unsigned v[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int k = 0; k < kStep; k += 4) {
-      const int64_t n = n0 + k + r;
-      float va = 0.f, vx = 0.f;
-      if (n < last) {
-        const int64_t b = n / T_, t = n - b * T_;
-        if (t < valid_length(lengths, b, T_)) {
-          if (m0 + c < M) va = to_f32(dy.row(b, t)[m0 + c]);
-          if (d0 + c < D)
-            vx = (float)codes[n * G * kPackGroup + d0 + c] *
-                 pack_scale(scales[n * G + (d0 + c) / kPackGroup]);
+  for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(v[k]);
+}
+// Shared-memory operand, MN-major, 128-byte swizzle: 64 channels are one row
+// of 128 bytes, 8 positions 1024 bytes, the next 64 channels kAtom further.
+__device__ __forceinline__ uint64_t operand(unsigned addr) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(kAtom >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// 8 codes to 8 bfloat16 values: code byte q = (q & 127) - (q & 128); either
+// part OR 0x4300 is a bfloat16 of 128 more, so their difference is q, exactly.
+__device__ __forceinline__ uint4 decode(uint2 q, uint8_t byte) {
+  const __nv_bfloat162 unit = __bfloat162bfloat162(__float2bfloat16_rn(pack_scale(byte)));
+  unsigned o[4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned w = k ? q.y : q.x;
+    const unsigned lo = w & 0x7f7f7f7fu, hi = w & 0x80808080u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned pick = h ? 0x4342u : 0x4140u;  // two bytes, each below a 0x43
+      const unsigned a = __byte_perm(lo, 0x43434343u, pick), c = __byte_perm(hi, 0x43434343u, pick);
+      const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                               *reinterpret_cast<const __nv_bfloat162*>(&c)),
+                                       unit);
+      o[2 * k + h] = *reinterpret_cast<const unsigned*>(&v);
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// One value's pieces: each the leading 8 bits of what is left, by truncation,
+// so no piece overflows and the last leaves nothing.
+template <int NP>
+__device__ __forceinline__ void cut(float v, unsigned short (&piece)[NP]) {
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const unsigned bits = __float_as_uint(v) & 0xffff0000u;
+    piece[k] = (unsigned short)(bits >> 16);
+    v = isinf(v) ? 0.f : v - __uint_as_float(bits);
+  }
+}
+
+template <class T, int CG, bool ASYNC>
+__global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const GradArgs a) {
+  using F = Form<T>;
+  using S = Shape<T>;
+  constexpr int NP = F::pieces, NS = S::kStages;
+  constexpr int kRowsPass = 2 * F::producers, kPasses = kStep / kRowsPass;
+  constexpr int kLook = ASYNC ? 3 : 1;  // stages requested ahead
+  constexpr bool kApart = NP == 3;      // float32: segments, lower pieces apart
+  constexpr int kCols = kTile * CG;     // columns of the accumulator
+  constexpr int kTmem = kApart ? 512 : kCols;
+  static_assert(!kApart || CG == 1, "tensor memory holds two segments and the lower pieces");
+  static_assert(kLook < NS, "a requested stage must not wait for an unpublished one");
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t full[NS], empty[NS], ready[2], taken[2];
+  __shared__ unsigned tmem_at;
+  unsigned char* ring = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = CG == 1 ? 0 : (int)(blockIdx.x % CG);
+  const int pairs_m = a.tiles_m / CG, tile = (int)blockIdx.x / CG;
+  const int tm = tile % pairs_m * CG + rank, td = tile / pairs_m;
+  const int64_t first = blockIdx.y * a.run;
+  const int64_t left = a.N - first;
+  const int count = (int)(left < a.run ? (left < 0 ? 0 : left) : a.run);
+  const int steps = (count + kStep - 1) / kStep;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      barrier_init(&full[s], F::producers * CG);
+      barrier_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      barrier_init(&ready[s], 1);
+      barrier_init(&taken[s], F::readers);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kWarps) {
+    if (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_addr(&tmem_at)),
+                   "n"(kTmem)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_addr(&tmem_at)),
+                   "n"(kTmem)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (CG > 1) sync_all<CG>();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem = tmem_at;
+
+  bool ok = true;
+  if (warp < F::producers) {
+    // this thread's 8 channels of dy and of x, and its first row of a stage
+    const int col = tid & 15, row0 = tid >> 4;
+    const int64_t m = (int64_t)tm * kTile + col * 8;
+    const int64_t d = ((int64_t)td * CG + rank) * kTile + col * 8;
+    const bool has_m = m < a.M, has_d = d < a.Dp;
+    const unsigned width = !has_m ? 0u : (unsigned)(a.M - m < 8 ? a.M - m : 8);
+    // where its 16-byte piece of a row lies; later passes are a multiple of 8 rows on
+    const unsigned dst = (unsigned)(col >> 3) * kAtom + (unsigned)((col & 7) ^ (row0 & 7)) * 16 +
+                         (unsigned)row0 * 128;
+    const T* dy = static_cast<const T*>(a.dy) + (has_m ? m : 0);
+    const int8_t* codes = a.codes + (first + row0) * a.Dp + (has_d ? d : 0);
+    const uint8_t* scales = a.scales + (first + row0) * a.G + (has_d ? d / kPackGroup : 0);
+    // the sequence and position of row0 of the stage that is requested next
+    int64_t b = (first + row0) / a.T_;
+    unsigned t = (unsigned)(first + row0 - b * a.T_);
+
+    struct Held {
+      uint2 q[kPasses];
+      uint8_t byte[kPasses];
+      Pack<T, 8> v[ASYNC ? 1 : kPasses];
+    } held[kLook];
+
+    const auto request = [&](int j, Held& h) {
+      if (j < steps) {
+        const int slot = j % NS;
+        if (j >= NS) {
+          ok = __all_sync(~0u, barrier_wait(&empty[slot], (unsigned)(j / NS - 1) & 1));
+          if (!ok) return;
+        }
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          unsigned tt = t + p * kRowsPass;
+          int64_t bb = b;
+          if (tt >= a.T_) {
+            const unsigned q = quotient(tt, a.by_t);
+            bb += q;
+            tt -= q * a.T_;
+          }
+          const bool live = j * kStep + row0 + p * kRowsPass < count &&
+                            (!a.lengths || (int64_t)tt < a.lengths[bb]);
+          const T* src = dy + bb * a.sb + (int64_t)tt * a.st;
+          if (ASYNC) {
+            const unsigned bytes = live ? 2 * width : 0u;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             smem_addr(ring + slot * S::kStage + dst + p * kRowsPass * 128)),
+                         "l"(bytes ? src : static_cast<const T*>(a.dy)), "r"(bytes)
+                         : "memory");
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) h.v[p].v[k] = from_f32<T>(0.f);
+            if (live && a.vec && width == 8) {
+              constexpr int V = 16 / sizeof(T);
+#pragma unroll
+              for (int k = 0; k < 8; k += V)
+                *reinterpret_cast<Pack<T, V>*>(&h.v[p].v[k]) =
+                    *reinterpret_cast<const Pack<T, V>*>(src + k);
+            } else if (live) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (k < width) h.v[p].v[k] = src[k];
+            }
+          }
+          h.q[p] = make_uint2(0, 0);
+          h.byte[p] = 0;
+          if (live && has_d) {
+            h.q[p] = *reinterpret_cast<const uint2*>(codes + p * kRowsPass * a.Dp);
+            h.byte[p] = scales[p * kRowsPass * a.G];
+          }
+        }
+        codes += kStep * a.Dp;
+        scales += kStep * a.G;
+        t += kStep;
+        if (t >= a.T_) {
+          const unsigned q = quotient(t, a.by_t);
+          b += q;
+          t -= q * a.T_;
         }
       }
-      a[k + r][c] = va;
-      x[k + r][c] = vx;
+      if (ASYNC) asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const auto publish = [&](int it, Held& h) {
+      unsigned char* base = ring + it % NS * S::kStage + dst;
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        unsigned char* at = base + p * kRowsPass * 128;
+        if (!ASYNC) {
+          unsigned short piece[8][NP];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) cut<NP>(to_f32(h.v[p].v[k]), piece[k]);
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            unsigned w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = (unsigned)piece[2 * k][j] | ((unsigned)piece[2 * k + 1][j] << 16);
+            *reinterpret_cast<uint4*>(at + j * kOperand) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        *reinterpret_cast<uint4*>(at + NP * kOperand) = decode(h.q[p], h.byte[p]);
+      }
+      if (ASYNC) asm volatile("cp.async.wait_group %0;" ::"n"(kLook - 1) : "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) barrier_arrive<CG>(&full[it % NS]);
+    };
+
+#pragma unroll
+    for (int u = 0; u < kLook; ++u) request(u, held[u]);
+    for (int it = 0; it < steps && ok; it += kLook)
+#pragma unroll
+      for (int u = 0; u < kLook; ++u)
+        if (it + u < steps && ok) {
+          publish(it + u, held[u]);
+          request(it + u + kLook, held[u]);
+        }
+    if (ASYNC) asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kWarps && lane == 0 && rank == 0) {
+    for (int it = 0; it < steps && ok; ++it) {
+      const int slot = it % NS, segment = it / kSegment, buffer = kApart ? segment & 1 : 0;
+      const bool opens = kApart ? it % kSegment == 0 : it == 0;
+      if (kApart && opens && segment >= 2)
+        ok = barrier_wait(&taken[buffer], (unsigned)(segment / 2 - 1) & 1);
+      ok = ok && barrier_wait(&full[slot], (unsigned)(it / NS) & 1);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const unsigned at = smem_addr(ring + slot * S::kStage);
+#pragma unroll
+      for (int k = 0; k < kStep / 16; ++k) {
+        const uint64_t bd = operand(at + NP * kOperand + k * 2048);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const uint64_t ad = operand(at + j * kOperand + k * 2048);
+          if (kApart)
+            product<CG>(tmem + (j ? 2 * kCols : buffer * kCols), ad, bd,
+                        j ? it > 0 || k > 0 || j > 1 : !opens || k > 0);
+          else
+            product<CG>(tmem, ad, bd, it > 0 || k > 0 || j > 0);
+        }
+      }
+      commit_to<CG>(&empty[slot]);
+      if (it == steps - 1 || (kApart && it % kSegment == kSegment - 1))
+        commit_to<CG>(&ready[buffer]);
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kStep; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[k][tm + i], x[k][td + j], acc[i][j]);
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (m0 + tm + i < M && d0 + td + j < D)
-        partial[(blockIdx.z * M + m0 + tm + i) * D + d0 + td + j] = acc[i][j];
+  __syncwarp();
+
+  // Tensor memory to the partial result: a warp reads its 32 lanes (rows of
+  // the tile) and a share of the columns; a column's rows are contiguous.
+  if (warp >= kWarps - F::readers && warp < kWarps) {
+    constexpr int kShare = kCols / (F::readers / 4);
+    static_assert(kShare % 16 == 0, "a warp reads 16 columns at once");
+    const int quarter = warp & 3, c0 = (warp - (kWarps - F::readers)) / 4 * kShare;
+    const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
+    float sum[kShare];
+#pragma unroll
+    for (int k = 0; k < kShare; ++k) sum[k] = 0.f;
+    const int segments = !steps ? 0 : kApart ? (steps + kSegment - 1) / kSegment : 1;
+    bool good = true;
+    for (int g = 0; g < segments && good; ++g) {
+      const int buffer = g & 1;
+      good = __all_sync(~0u, barrier_wait(&ready[buffer], (unsigned)(g / 2) & 1));
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (!good) break;
+#pragma unroll
+      for (int c = 0; c < kShare; c += 16) {
+        float v[16];
+        read_columns(at + buffer * kCols + c, v);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum[c + k] += v[k];
+        if (kApart && g == segments - 1) {
+          read_columns(at + 2 * kCols + c, v);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) sum[c + k] += v[k];
+        }
+      }
+      if (kApart) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) barrier_arrive<1>(&taken[buffer]);
+      }
+    }
+    float* out = a.partial +
+                 ((((int64_t)blockIdx.y * a.tiles_m + tm) * a.tiles_d + td) * kCols + c0) * kTile +
+                 quarter * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < kShare; ++k)  // a wait that ran out shows as NaN
+      out[(int64_t)k * kTile] = good ? sum[k] : __uint_as_float(0x7fc00000u);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (CG > 1) sync_all<CG>();
+  if (warp == kWarps) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem));
+  }
 }
 
+// Sums the runs in order.  A block takes 32 x 32 outputs of a tile: reads
+// along the tile's rows, writes along the output's.
 template <class O>
-__global__ void sum_runs_kernel(int64_t n, int runs, const float* __restrict__ partial,
-                                O* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  float s = 0.f;
-  for (int k = 0; k < runs; ++k) s += partial[k * n + i];
-  out[i] = from_f32<O>(s);
-}
-
-int runs_of(int64_t N, int64_t D, int64_t M) {
-  const int64_t tiles = ((M + kTileOut - 1) / kTileOut) * ((D + kTileOut - 1) / kTileOut);
-  const int64_t want = std::max<int64_t>(1, 4 * device_sm_count() / tiles);
-  return (int)std::min<int64_t>(want, std::max<int64_t>(1, N / 256));
-}
-
-template <class T>
-int run(int64_t B, int64_t T_, int64_t D, int64_t M, const semicrf_sequence& dy,
-        const int8_t* codes, const uint8_t* scales, const int64_t* lengths, int out_dtype,
-        void* out, void* workspace, cudaStream_t stream) {
-  const int64_t N = B * T_;
-  const int runs = runs_of(N, D, M);
-  const int64_t run_len = N ? (N + runs - 1) / runs : 0;
-  float* partial = static_cast<float*>(workspace);
-  const dim3 grid((unsigned)((M + kTileOut - 1) / kTileOut),
-                  (unsigned)((D + kTileOut - 1) / kTileOut), (unsigned)runs);
-  weight_grad_kernel<T><<<grid, 256, 0, stream>>>(N, T_, D, M, run_len, as_seq<const T>(dy), codes,
-                                                  scales, lengths, partial);
-  const unsigned sg = (unsigned)((M * D + 255) / 256);
-  switch (out_dtype) {
-    case SEMICRF_F32:
-      sum_runs_kernel<<<sg, 256, 0, stream>>>(M * D, runs, partial, static_cast<float*>(out));
-      break;
-    case SEMICRF_BF16:
-      sum_runs_kernel<<<sg, 256, 0, stream>>>(M * D, runs, partial,
-                                              static_cast<__nv_bfloat16*>(out));
-      break;
-    default:
-      sum_runs_kernel<<<sg, 256, 0, stream>>>(M * D, runs, partial, static_cast<__half*>(out));
+__global__ void __launch_bounds__(256) sum_runs_kernel(int64_t D, int64_t M, int tiles_m, int64_t cols,
+                                                       int runs, const float* __restrict__ partial,
+                                                       O* __restrict__ out) {
+  __shared__ float tile[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t m0 = (int64_t)blockIdx.x * 32, d0 = (int64_t)blockIdx.y * 32;
+  const int64_t size = (int64_t)tiles_m * cols * kTile;
+  const float* src = partial + (m0 / kTile * cols + d0) * kTile + m0 % kTile + x;
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    float s = 0.f;
+    for (int r = 0; r < runs; ++r) s += src[r * size + (int64_t)(y + k) * kTile];
+    tile[y + k][x] = s;
   }
-  return launch_status();
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 32; k += 8)
+    if (m0 + y + k < M && d0 + x < D) out[(m0 + y + k) * D + d0 + x] = from_f32<O>(tile[x][y + k]);
+}
+
+struct Plan {
+  int group, tiles_m, tiles_d, runs;  // CTAs of a tile; its tiles of 128 rows, 128 group columns
+  int64_t run;
+};
+
+// Runs: as many as fill the SMs once, of four stages at least.
+Plan plan(int64_t N, int64_t D, int64_t M, int dtype) {
+  Plan p;
+  p.group = dtype != SEMICRF_F32 && M > kTile && D > kTile ? 2 : 1;
+  const int64_t edge = (int64_t)kTile * p.group;
+  p.tiles_m = (int)((M + edge - 1) / edge) * p.group;
+  p.tiles_d = (int)((D + edge - 1) / edge);
+  const int64_t steps = (N + kStep - 1) / kStep;
+  const int64_t ctas = (int64_t)p.tiles_m * p.tiles_d;
+  int64_t runs = std::max<int64_t>(1, device_sm_count() / ctas);
+  runs = std::max<int64_t>(1, std::min(runs, steps / 4));
+  const int64_t per = std::max<int64_t>(1, (steps + runs - 1) / runs);
+  p.run = per * kStep;
+  p.runs = (int)std::max<int64_t>(1, (steps + per - 1) / per);
+  return p;
+}
+
+template <class T, int CG, bool ASYNC>
+int launch(const GradArgs& a, int runs, cudaStream_t stream) {
+  const auto kernel = weight_grad_kernel<T, CG, ASYNC>;
+  constexpr int bytes = Shape<T>::kBytes;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      cudaSuccess)
+    return SEMICRF_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(a.tiles_m * a.tiles_d), (unsigned)runs);
+  cfg.blockDim = dim3(32 * kWarps + 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? SEMICRF_OK : SEMICRF_ERR_CUDA;
+}
+
+template <class T, bool ASYNC>
+int launch_group(const GradArgs& a, const Plan& p, cudaStream_t stream) {
+  return p.group == 2 ? launch<T, 2, ASYNC>(a, p.runs, stream)
+                      : launch<T, 1, ASYNC>(a, p.runs, stream);
 }
 
 }  // namespace
 
-size_t packed_weight_grad_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t M, int) {
-  return sizeof(float) * M * D * runs_of(B * T, D, M);
+size_t packed_weight_grad_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t M,
+                                          int dtype) {
+  const Plan p = plan(B * T, D, M, dtype);
+  return sizeof(float) * p.runs * p.tiles_m * kTile * p.tiles_d * p.group * kTile;
 }
 
 int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
                        const semicrf_sequence& dy, const int8_t* codes, const uint8_t* scales,
                        const int64_t* lengths, int out_dtype, void* out, void* workspace,
                        cudaStream_t stream) {
+  const Plan p = plan(B * T, D, M, dtype);
+  if (T >= (1 << 30) || p.run >= (1 << 30)) return SEMICRF_ERR_UNSUPPORTED;  // Divider's range
+  GradArgs a{};
+  a.N = B * T;
+  a.M = M;
+  a.G = pack_groups(D);
+  a.Dp = a.G * kPackGroup;
+  a.run = p.run;
+  a.dy = dy.data;
+  a.sb = dy.batch_stride;
+  a.st = dy.time_stride;
+  a.codes = codes;
+  a.scales = scales;
+  a.vec = seq_aligned(dy, B, T, dtype == SEMICRF_F32 ? 4 : 2, dtype == SEMICRF_F32 ? 4 : 8);
+  a.lengths = lengths;
+  a.T_ = (unsigned)std::max<int64_t>(T, 1);
+  a.by_t = make_divider(a.T_);
+  a.tiles_m = p.tiles_m;
+  a.tiles_d = p.tiles_d;
+  a.partial = static_cast<float*>(workspace);
+  int st;
   switch (dtype) {
-    case SEMICRF_F32:
-      return run<float>(B, T, D, M, dy, codes, scales, lengths, out_dtype, out, workspace, stream);
+    case SEMICRF_F32: st = launch<float, 1, false>(a, p.runs, stream); break;
     case SEMICRF_BF16:
-      return run<__nv_bfloat16>(B, T, D, M, dy, codes, scales, lengths, out_dtype, out, workspace,
-                                stream);
-    default:
-      return run<__half>(B, T, D, M, dy, codes, scales, lengths, out_dtype, out, workspace, stream);
+      st = a.vec ? launch_group<__nv_bfloat16, true>(a, p, stream)
+                 : launch_group<__nv_bfloat16, false>(a, p, stream);
+      break;
+    default: st = launch_group<__half, false>(a, p, stream);
   }
+  if (st != SEMICRF_OK) return st;
+  const dim3 grid((unsigned)((M + 31) / 32), (unsigned)((D + 31) / 32));
+  const int64_t cols = (int64_t)p.tiles_d * p.group * kTile;
+  switch (out_dtype) {
+    case SEMICRF_F32:
+      sum_runs_kernel<<<grid, 256, 0, stream>>>(D, M, p.tiles_m, cols, p.runs, a.partial,
+                                                static_cast<float*>(out));
+      break;
+    case SEMICRF_BF16:
+      sum_runs_kernel<<<grid, 256, 0, stream>>>(D, M, p.tiles_m, cols, p.runs, a.partial,
+                                                static_cast<__nv_bfloat16*>(out));
+      break;
+    default:
+      sum_runs_kernel<<<grid, 256, 0, stream>>>(D, M, p.tiles_m, cols, p.runs, a.partial,
+                                                static_cast<__half*>(out));
+  }
+  return launch_status();
 }
 
 }  // namespace semicrf
