@@ -26,6 +26,8 @@
 // For float32 the leading piece is summed apart from the others and, every
 // 512 positions, moved from tensor memory to registers that round to nearest.
 
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "encoder_internal.cuh"
@@ -41,7 +43,7 @@ constexpr int kAtom = kStep * 128;  // bytes of 64 channels of a stage: 64 rows 
 constexpr int kOperand = 2 * kAtom; // bytes of an operand of a stage
 constexpr int kWarps = 16;      // producers and readers of tensor memory; one more issues
 constexpr int kSegment = 8;     // float32: stages that tensor memory sums
-constexpr unsigned kWaitLimit = 1u << 22;
+constexpr unsigned kWaitLimit = 1u << 20;
 
 template <class T>
 struct Form;  // pieces of a value; producer warps; warps that read tensor memory
@@ -482,6 +484,236 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
   }
 }
 
+// ---------------------------------------------------------------------------
+// bfloat16 dy whose positions are evenly spaced: the bulk-copy form.  A warp's
+// thread fetches dy (into the operand tile, swizzled) and codes (as they are)
+// by TMA, another warp brings the scales and finds masked rows; the sixteen
+// decoding warps touch only shared memory, so their fence before a stage is
+// published never waits for a load from global memory.
+// ---------------------------------------------------------------------------
+constexpr int kCodes = kStep * kTile;        // bytes of a stage's codes
+constexpr int kBulkStage = 2 * kOperand + kCodes;
+constexpr int kBulkStages = 5;
+constexpr int kBulkBytes = kBulkStages * kBulkStage + 1024;
+constexpr int kBulkThreads = 32 * (kWarps + 3);
+constexpr int kScaleLook = 4;                // stages whose scales are in flight
+constexpr int kGroups = 4;                   // decoding groups: each takes every fourth stage
+
+__device__ __forceinline__ void expect_bytes(uint64_t* b, unsigned n) {
+  asm volatile("{.reg .b64 t; mbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;}" ::"r"(
+                   smem_addr(b)),
+               "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void fetch_tile(unsigned dst, const CUtensorMap* map, int x, int y,
+                                           uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(smem_addr(b))
+      : "memory");
+}
+
+template <int CG>
+__global__ void __launch_bounds__(kBulkThreads, 1)
+    weight_grad_bulk_kernel(const GradArgs a, const __grid_constant__ CUtensorMap dy_map,
+                            const __grid_constant__ CUtensorMap code_map) {
+  constexpr int NS = kBulkStages, kCols = kTile * CG;
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t landed[NS], full[NS], empty[NS], ready;
+  __shared__ unsigned scale[NS][kStep];  // a row's four scale bytes
+  __shared__ unsigned masked[NS][2];     // rows to be cleared
+  __shared__ unsigned tmem_at;
+  unsigned char* ring = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = CG == 1 ? 0 : (int)(blockIdx.x % CG);
+  const int pairs_m = a.tiles_m / CG, tile = (int)blockIdx.x / CG;
+  const int tm = tile % pairs_m * CG + rank, td = tile / pairs_m;
+  const int64_t first = blockIdx.y * a.run;
+  const int64_t left = a.N - first;
+  const int count = (int)(left < a.run ? (left < 0 ? 0 : left) : a.run);
+  const int steps = (count + kStep - 1) / kStep;
+
+  if (tid == 0) {
+    for (int s = 0; s < NS; ++s) {
+      barrier_init(&landed[s], 2);  // the copies, and the scales
+      barrier_init(&full[s], kWarps / kGroups * CG);
+      barrier_init(&empty[s], 1);
+    }
+    barrier_init(&ready, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kWarps) {
+    if (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_addr(&tmem_at)),
+                   "n"(kCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       smem_addr(&tmem_at)),
+                   "n"(kCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (CG > 1) sync_all<CG>();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned tmem = tmem_at;
+
+  bool ok = true;
+  if (warp < kWarps) {
+    constexpr int kPart = 32 * kWarps / kGroups, kRows = kPart / 16;
+    const int part = tid % kPart, col = part & 15, row0 = part >> 4;  // rows row0, + kRows, ...
+    const unsigned dst = (unsigned)(col >> 3) * kAtom + (unsigned)((col & 7) ^ (row0 & 7)) * 16 +
+                         (unsigned)row0 * 128;
+    for (int it = tid / kPart; it < steps; it += kGroups) {
+      const int slot = it % NS;
+      ok = __all_sync(~0u, barrier_wait(&landed[slot], (unsigned)(it / NS) & 1));
+      if (!ok) break;
+      unsigned char* base = ring + slot * kBulkStage;
+      const unsigned char* codes = base + 2 * kOperand + row0 * kTile + col * 8;
+      const unsigned off0 = masked[slot][0], off1 = masked[slot][1];
+#pragma unroll
+      for (int p = 0; p < kStep / kRows; ++p) {
+        const uint2 q = *reinterpret_cast<const uint2*>(codes + p * kRows * kTile);
+        const uint8_t byte = (uint8_t)(scale[slot][row0 + kRows * p] >> (col >> 2) * 8);
+        *reinterpret_cast<uint4*>(base + kOperand + dst + p * kRows * 128) = decode(q, byte);
+      }
+      if (off0 | off1)
+#pragma unroll 1
+        for (int row = row0; row < kStep; row += kRows)
+          if ((row < 32 ? off0 : off1) >> (row & 31) & 1)
+            *reinterpret_cast<uint4*>(base + dst + (row - row0) * 128) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) barrier_arrive<CG>(&full[slot]);
+    }
+  } else if (warp == kWarps && lane == 0 && rank == 0) {
+    for (int it = 0; it < steps; ++it) {
+      const int slot = it % NS;
+      ok = barrier_wait(&full[slot], (unsigned)(it / NS) & 1);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const unsigned at = smem_addr(ring + slot * kBulkStage);
+#pragma unroll
+      for (int k = 0; k < kStep / 16; ++k)
+        product<CG>(tmem, operand(at + k * 2048), operand(at + kOperand + k * 2048),
+                    it > 0 || k > 0);
+      commit_to<CG>(&empty[slot]);
+    }
+    if (ok && steps) commit_to<CG>(&ready);
+  } else if (warp == kWarps + 1 && lane == 0) {
+    const int m0 = tm * kTile, d0 = (td * CG + rank) * kTile;
+    for (int it = 0; it < steps; ++it) {
+      const int slot = it % NS;
+      if (it >= NS) {
+        ok = barrier_wait(&empty[slot], (unsigned)(it / NS - 1) & 1);
+        if (!ok) break;
+      }
+      const unsigned at = smem_addr(ring + slot * kBulkStage);
+      const int n0 = (int)first + it * kStep;
+      expect_bytes(&landed[slot], kOperand + kCodes);
+      fetch_tile(at, &dy_map, m0, n0, &landed[slot]);
+      fetch_tile(at + kAtom, &dy_map, m0 + 64, n0, &landed[slot]);
+      fetch_tile(at + 2 * kOperand, &code_map, d0, n0, &landed[slot]);
+    }
+  } else if (warp == kWarps + 2) {
+    // rows lane and lane + 32 of a stage
+    const int g0 = (td * CG + rank) * (kTile / kPackGroup);
+    const bool whole = a.G % 4 == 0 && g0 + 4 <= a.G && reinterpret_cast<uintptr_t>(a.scales) % 4 == 0;
+    const int64_t b0 = first / a.T_;
+    const unsigned t0 = (unsigned)(first - b0 * a.T_);
+    struct Held {
+      unsigned v[2];
+      bool live[2];
+    } held[kScaleLook];
+    const auto request = [&](int it, Held& h) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int n = it * kStep + lane + 32 * p;
+        h.v[p] = 0;
+        h.live[p] = n < count;
+        if (h.live[p] && a.lengths) {
+          const unsigned k = t0 + (unsigned)n, q = quotient(k, a.by_t);
+          h.live[p] = (int64_t)(k - q * a.T_) < a.lengths[b0 + q];
+        }
+        if (!h.live[p]) continue;
+        const uint8_t* src = a.scales + (first + n) * a.G + g0;
+        if (whole) {
+          h.v[p] = *reinterpret_cast<const unsigned*>(src);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (g0 + k < a.G) h.v[p] |= (unsigned)src[k] << 8 * k;
+        }
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < kScaleLook; ++u) request(u, held[u]);
+    for (int base = 0; base < steps && ok; base += kScaleLook)
+#pragma unroll
+      for (int u = 0; u < kScaleLook; ++u) {
+        const int it = base + u, slot = it % NS;
+        if (it >= steps || !ok) continue;
+        if (it >= NS)
+          ok = __all_sync(~0u, barrier_wait(&empty[slot], (unsigned)(it / NS - 1) & 1));
+        if (!ok) continue;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          scale[slot][lane + 32 * p] = held[u].v[p];
+          const unsigned off = __ballot_sync(~0u, !held[u].live[p]);
+          if (lane == 0) masked[slot][p] = off;
+        }
+        __syncwarp();
+        if (lane == 0) barrier_arrive<1>(&landed[slot]);
+        request(it + kScaleLook, held[u]);
+      }
+  }
+  __syncwarp();
+
+  if (warp < kWarps) {
+    constexpr int kShare = kCols / 4;
+    const int quarter = warp & 3, c0 = (warp >> 2) * kShare;
+    const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
+    const bool good = !steps || __all_sync(~0u, barrier_wait(&ready, 0));
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    float* out = a.partial +
+                 ((((int64_t)blockIdx.y * a.tiles_m + tm) * a.tiles_d + td) * kCols + c0) * kTile +
+                 quarter * 32 + lane;
+#pragma unroll
+    for (int c = 0; c < kShare; c += 16) {
+      float v[16];
+      if (steps && good) {
+        read_columns(at + c, v);
+      } else {  // no positions: zeros; a wait that ran out shows as NaN
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = good ? 0.f : __uint_as_float(0x7fc00000u);
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) out[(int64_t)(c + k) * kTile] = v[k];
+    }
+  } else if (!ok && warp == kWarps + 1) {
+    // copies in flight must land before the CTA's memory is given up
+    for (int s = 0; s < NS; ++s)
+      for (unsigned ph = 0; ph < 2; ++ph) barrier_wait(&landed[s], ph);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (CG > 1) sync_all<CG>();
+  if (warp == kWarps) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols));
+  }
+}
+
 // Sums the runs in order.  A block takes 32 x 32 outputs of a tile: reads
 // along the tile's rows, writes along the output's.
 template <class O>
@@ -548,6 +780,62 @@ int launch(const GradArgs& a, int runs, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? SEMICRF_OK : SEMICRF_ERR_CUDA;
 }
 
+// cuTensorMapEncodeTiled, looked up once: the library does not link libcuda.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) !=
+            cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t width,
+              int64_t rows, int64_t row_bytes, int box, CUtensorMapSwizzle swizzle) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+  const cuuint32_t boxes[2] = {(cuuint32_t)box, (cuuint32_t)kStep}, ones[2] = {1, 1};
+  return encode(map, type, 2, const_cast<void*>(base), dims, strides, boxes, ones,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int CG>
+int launch_bulk(const GradArgs& a, int runs, cudaStream_t stream) {
+  const auto kernel = weight_grad_bulk_kernel<CG>;
+  CUtensorMap dy, codes;
+  if (!make_map(&dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.dy, a.M, a.N, a.st * 2, 64,
+                CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_map(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.Dp, a.N, a.Dp, kTile,
+                CU_TENSOR_MAP_SWIZZLE_NONE) ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkBytes) !=
+          cudaSuccess)
+    return SEMICRF_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(a.tiles_m * a.tiles_d), (unsigned)runs);
+  cfg.blockDim = dim3(kBulkThreads);
+  cfg.dynamicSmemBytes = kBulkBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a, dy, codes) == cudaSuccess ? SEMICRF_OK
+                                                                       : SEMICRF_ERR_CUDA;
+}
+
 template <class T, bool ASYNC>
 int launch_group(const GradArgs& a, const Plan& p, cudaStream_t stream) {
   return p.group == 2 ? launch<T, 2, ASYNC>(a, p.runs, stream)
@@ -586,12 +874,21 @@ int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
   a.tiles_m = p.tiles_m;
   a.tiles_d = p.tiles_d;
   a.partial = static_cast<float*>(workspace);
+  // the distance between positions where it is one and the same
+  const int64_t row = T > 1 ? a.st : B > 1 ? a.sb : (M + 7) / 8 * 8;
   int st;
   switch (dtype) {
     case SEMICRF_F32: st = launch<float, 1, false>(a, p.runs, stream); break;
     case SEMICRF_BF16:
-      st = a.vec ? launch_group<__nv_bfloat16, true>(a, p, stream)
-                 : launch_group<__nv_bfloat16, false>(a, p, stream);
+      // bulk copies want aligned rows at one distance, and a row index in 31 bits
+      if (a.vec && a.N && a.N < (1ll << 31) - kStep && reinterpret_cast<uintptr_t>(codes) % 16 == 0 &&
+          (B == 1 || T == 1 || a.sb == T * a.st) && row >= M && row < (1ll << 36)) {
+        a.st = row;
+        st = p.group == 2 ? launch_bulk<2>(a, p.runs, stream) : launch_bulk<1>(a, p.runs, stream);
+      } else {
+        st = a.vec ? launch_group<__nv_bfloat16, true>(a, p, stream)
+                   : launch_group<__nv_bfloat16, false>(a, p, stream);
+      }
       break;
     default: st = launch_group<__half, false>(a, p, stream);
   }
