@@ -108,7 +108,7 @@ __device__ __forceinline__ void barrier_arrive(uint64_t* b) {
     asm volatile("{.reg .b64 t; mbarrier.arrive.shared::cta.b64 t, [%0];}" ::"r"(smem_addr(b))
                  : "memory");
   else
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
                      peer_addr(smem_addr(b), 0))
                  : "memory");
 }
@@ -485,19 +485,26 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
 }
 
 // ---------------------------------------------------------------------------
-// bfloat16 dy whose positions are evenly spaced: the bulk-copy form.  A warp's
-// thread fetches dy (into the operand tile, swizzled) and codes (as they are)
-// by TMA, another warp brings the scales and finds masked rows; the sixteen
-// decoding warps touch only shared memory, so their fence before a stage is
-// published never waits for a load from global memory.
+// bfloat16 dy whose positions are evenly spaced: the bulk-copy form.  One
+// thread fetches codes and one dy (into the operand tile, swizzled) by TMA.
+// The decoding warps read their scales from global memory right after they
+// publish a stage, for the stage they take next, so that their fence before a
+// stage is published never waits for a load.  A stage still takes a warp a
+// few thousand cycles of waiting and decoding: five groups of four warps each
+// take every fifth stage.  A group owns one slot of the operand ring.  It
+// waits for the products of the slot's earlier stage first; those are done in
+// order, so by then every stage that used its next code slot before has
+// landed, and no wait is ever more than one phase ahead of its barrier.
+// The issuing thread waits for one barrier a stage: another thread reports
+// dy's arrival to it.
 // ---------------------------------------------------------------------------
+constexpr int kGroups = 5;                   // decoding groups and slots of the operand ring
+constexpr int kGroupWarps = 4;
+constexpr int kDecoders = kGroups * kGroupWarps;
+constexpr int kCodeSlots = 7;
 constexpr int kCodes = kStep * kTile;        // bytes of a stage's codes
-constexpr int kBulkStage = 2 * kOperand + kCodes;
-constexpr int kBulkStages = 5;
-constexpr int kBulkBytes = kBulkStages * kBulkStage + 1024;
-constexpr int kBulkThreads = 32 * (kWarps + 3);
-constexpr int kScaleLook = 4;                // stages whose scales are in flight
-constexpr int kGroups = 4;                   // decoding groups: each takes every fourth stage
+constexpr int kBulkBytes = kGroups * 2 * kOperand + kCodeSlots * kCodes + 1024;
+constexpr int kBulkThreads = 32 * (kDecoders + 4);
 
 __device__ __forceinline__ void expect_bytes(uint64_t* b, unsigned n) {
   asm volatile("{.reg .b64 t; mbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;}" ::"r"(
@@ -518,14 +525,13 @@ template <int CG>
 __global__ void __launch_bounds__(kBulkThreads, 1)
     weight_grad_bulk_kernel(const GradArgs a, const __grid_constant__ CUtensorMap dy_map,
                             const __grid_constant__ CUtensorMap code_map) {
-  constexpr int NS = kBulkStages, kCols = kTile * CG;
+  constexpr int NS = kGroups, NC = kCodeSlots, kCols = kTile * CG;
   extern __shared__ unsigned char raw[];
-  __shared__ uint64_t landed[NS], full[NS], empty[NS], ready;
-  __shared__ unsigned scale[NS][kStep];  // a row's four scale bytes
-  __shared__ unsigned masked[NS][2];     // rows to be cleared
+  __shared__ uint64_t code_landed[NC], code_free[NC], dy_landed[NS], full[NS], empty[NS], ready;
   __shared__ unsigned tmem_at;
   unsigned char* ring = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* code_ring = ring + NS * 2 * kOperand;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = CG == 1 ? 0 : (int)(blockIdx.x % CG);
   const int pairs_m = a.tiles_m / CG, tile = (int)blockIdx.x / CG;
@@ -536,15 +542,19 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
   const int steps = (count + kStep - 1) / kStep;
 
   if (tid == 0) {
+    for (int s = 0; s < NC; ++s) {
+      barrier_init(&code_landed[s], 1);
+      barrier_init(&code_free[s], kGroupWarps);
+    }
     for (int s = 0; s < NS; ++s) {
-      barrier_init(&landed[s], 2);  // the copies, and the scales
-      barrier_init(&full[s], kWarps / kGroups * CG);
+      barrier_init(&dy_landed[s], 1);
+      barrier_init(&full[s], (kGroupWarps + 1) * CG);  // each CTA's group, and its dy
       barrier_init(&empty[s], 1);
     }
     barrier_init(&ready, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kWarps) {
+  if (warp == kDecoders) {
     if (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                        smem_addr(&tmem_at)),
@@ -566,112 +576,132 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
   const unsigned tmem = tmem_at;
 
   bool ok = true;
-  if (warp < kWarps) {
-    constexpr int kPart = 32 * kWarps / kGroups, kRows = kPart / 16;
-    const int part = tid % kPart, col = part & 15, row0 = part >> 4;  // rows row0, + kRows, ...
-    const unsigned dst = (unsigned)(col >> 3) * kAtom + (unsigned)((col & 7) ^ (row0 & 7)) * 16 +
+  if (warp < kDecoders) {
+    // rows row0, row0 + 8, ...; a warp's sixteen rows are 2 w, 2 w + 1, + 8, ...
+    constexpr int kPart = 32 * kGroupWarps, kRows = kPart / 16, kPasses = kStep / kRows;
+    static_assert(kRows == 8, "the swizzle and the lanes' rows repeat every 8 rows");
+    const int part = tid % kPart, col = part & 15, row0 = part >> 4;
+    const unsigned dst = (unsigned)(col >> 3) * kAtom + (unsigned)((col & 7) ^ row0) * 16 +
                          (unsigned)row0 * 128;
-    for (int it = tid / kPart; it < steps; it += kGroups) {
-      const int slot = it % NS;
-      ok = __all_sync(~0u, barrier_wait(&landed[slot], (unsigned)(it / NS) & 1));
-      if (!ok) break;
-      unsigned char* base = ring + slot * kBulkStage;
-      const unsigned char* codes = base + 2 * kOperand + row0 * kTile + col * 8;
-      const unsigned off0 = masked[slot][0], off1 = masked[slot][1];
-#pragma unroll
-      for (int p = 0; p < kStep / kRows; ++p) {
-        const uint2 q = *reinterpret_cast<const uint2*>(codes + p * kRows * kTile);
-        const uint8_t byte = (uint8_t)(scale[slot][row0 + kRows * p] >> (col >> 2) * 8);
-        *reinterpret_cast<uint4*>(base + kOperand + dst + p * kRows * 128) = decode(q, byte);
+    const int slot = tid / kPart;
+    unsigned char* base = ring + slot * 2 * kOperand + dst;
+    // lane l < 16 brings the four scale bytes of row 2 w + l % 2 + 8 (l / 2)
+    const int my_row = (row0 & ~1) + (lane & 1) + 8 * (lane >> 1 & 7);
+    const int g0 = (td * CG + rank) * (kTile / kPackGroup);
+    const bool whole =
+        a.G % 4 == 0 && g0 + 4 <= a.G && reinterpret_cast<uintptr_t>(a.scales) % 4 == 0;
+    const int64_t b0 = first / a.T_;
+    const unsigned t0 = (unsigned)(first - b0 * a.T_);
+    unsigned scale = 0;
+    bool live = false;
+    const auto request = [&](int it) {
+      const int n = it * kStep + my_row;
+      scale = 0;
+      live = n < count;
+      if (live && a.lengths) {
+        const unsigned k = t0 + (unsigned)n, q = quotient(k, a.by_t);
+        live = (int64_t)(k - q * a.T_) < a.lengths[b0 + q];
       }
-      if (off0 | off1)
-#pragma unroll 1
-        for (int row = row0; row < kStep; row += kRows)
-          if ((row < 32 ? off0 : off1) >> (row & 31) & 1)
-            *reinterpret_cast<uint4*>(base + dst + (row - row0) * 128) = make_uint4(0, 0, 0, 0);
+      if (!live) return;
+      const uint8_t* src = a.scales + (first + n) * a.G + g0;
+      if (whole) {
+        scale = *reinterpret_cast<const unsigned*>(src);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (g0 + k < a.G) scale |= (unsigned)src[k] << 8 * k;
+      }
+    };
+    request(slot);
+    for (int it = slot; it < steps; it += kGroups) {
+      const int cs = it % NC;
+      const unsigned use = (unsigned)(it / NS);
+      if (use) ok = __all_sync(~0u, barrier_wait(&empty[slot], (use - 1) & 1));
+      ok = ok && __all_sync(~0u, barrier_wait(&code_landed[cs], (unsigned)(it / NC) & 1));
+      if (!ok) break;
+      const unsigned char* codes = code_ring + cs * kCodes + row0 * kTile + col * 8;
+      const unsigned on = __ballot_sync(~0u, live);
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const uint2 q = *reinterpret_cast<const uint2*>(codes + p * kRows * kTile);
+        const unsigned bytes = __shfl_sync(~0u, scale, (row0 & 1) + 2 * p);
+        *reinterpret_cast<uint4*>(base + kOperand + p * kRows * 128) =
+            decode(q, (uint8_t)(bytes >> (col >> 2) * 8));
+      }
+      __syncwarp();
+      if (lane == 0) barrier_arrive<1>(&code_free[cs]);
+      if ((on & 0xffffu) != 0xffffu) {  // clear the masked rows of dy
+        ok = __all_sync(~0u, barrier_wait(&dy_landed[slot], use & 1));
+        if (!ok) break;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p)
+          if (!(on >> ((row0 & 1) + 2 * p) & 1))
+            *reinterpret_cast<uint4*>(base + p * kRows * 128) = make_uint4(0, 0, 0, 0);
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) barrier_arrive<CG>(&full[slot]);
+      request(it + kGroups);
     }
-  } else if (warp == kWarps && lane == 0 && rank == 0) {
-    for (int it = 0; it < steps; ++it) {
-      const int slot = it % NS;
-      ok = barrier_wait(&full[slot], (unsigned)(it / NS) & 1);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const unsigned at = smem_addr(ring + slot * kBulkStage);
-#pragma unroll
-      for (int k = 0; k < kStep / 16; ++k)
-        product<CG>(tmem, operand(at + k * 2048), operand(at + kOperand + k * 2048),
-                    it > 0 || k > 0);
-      commit_to<CG>(&empty[slot]);
-    }
-    if (ok && steps) commit_to<CG>(&ready);
-  } else if (warp == kWarps + 1 && lane == 0) {
-    const int m0 = tm * kTile, d0 = (td * CG + rank) * kTile;
-    for (int it = 0; it < steps; ++it) {
-      const int slot = it % NS;
-      if (it >= NS) {
-        ok = barrier_wait(&empty[slot], (unsigned)(it / NS - 1) & 1);
+  } else if (warp == kDecoders) {
+    if (lane == 0 && rank == 0)
+      for (int it = 0; it < steps; ++it) {
+        const int slot = it % NS;
+        ok = barrier_wait(&full[slot], (unsigned)(it / NS) & 1);
         if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const unsigned at = smem_addr(ring + slot * 2 * kOperand);
+        const uint64_t ad = operand(at), bd = operand(at + kOperand);
+#pragma unroll
+        for (int k = 0; k < kStep / 16; ++k)  // 16 positions are 2048 bytes
+          product<CG>(tmem, ad + k * (2048 >> 4), bd + k * (2048 >> 4), it > 0 || k > 0);
+        commit_to<CG>(&empty[slot]);
+        if (it == steps - 1) commit_to<CG>(&ready);
       }
-      const unsigned at = smem_addr(ring + slot * kBulkStage);
-      const int n0 = (int)first + it * kStep;
-      expect_bytes(&landed[slot], kOperand + kCodes);
-      fetch_tile(at, &dy_map, m0, n0, &landed[slot]);
-      fetch_tile(at + kAtom, &dy_map, m0 + 64, n0, &landed[slot]);
-      fetch_tile(at + 2 * kOperand, &code_map, d0, n0, &landed[slot]);
+  } else if (warp == kDecoders + 1) {
+    if (lane == 0) {
+      const int m0 = tm * kTile;
+      int it = 0;
+      for (; it < steps; ++it) {
+        const int slot = it % NS;
+        if (it >= NS) {
+          ok = barrier_wait(&empty[slot], (unsigned)(it / NS - 1) & 1);
+          if (!ok) break;
+        }
+        const unsigned at = smem_addr(ring + slot * 2 * kOperand);
+        const int n0 = (int)first + it * kStep;
+        expect_bytes(&dy_landed[slot], kOperand);
+        fetch_tile(at, &dy_map, m0, n0, &dy_landed[slot]);
+        fetch_tile(at + kAtom, &dy_map, m0 + 64, n0, &dy_landed[slot]);
+      }
+      // no copy may still be in flight when the CTA's memory is given up
+      for (int k = it > NS ? it - NS : 0; k < it; ++k)
+        barrier_wait(&dy_landed[k % NS], (unsigned)(k / NS) & 1);
     }
-  } else if (warp == kWarps + 2) {
-    // rows lane and lane + 32 of a stage
-    const int g0 = (td * CG + rank) * (kTile / kPackGroup);
-    const bool whole = a.G % 4 == 0 && g0 + 4 <= a.G && reinterpret_cast<uintptr_t>(a.scales) % 4 == 0;
-    const int64_t b0 = first / a.T_;
-    const unsigned t0 = (unsigned)(first - b0 * a.T_);
-    struct Held {
-      unsigned v[2];
-      bool live[2];
-    } held[kScaleLook];
-    const auto request = [&](int it, Held& h) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int n = it * kStep + lane + 32 * p;
-        h.v[p] = 0;
-        h.live[p] = n < count;
-        if (h.live[p] && a.lengths) {
-          const unsigned k = t0 + (unsigned)n, q = quotient(k, a.by_t);
-          h.live[p] = (int64_t)(k - q * a.T_) < a.lengths[b0 + q];
+  } else if (warp == kDecoders + 2) {
+    if (lane == 0) {
+      const int d0 = (td * CG + rank) * kTile;
+      int it = 0;
+      for (; it < steps; ++it) {
+        const int cs = it % NC;
+        if (it >= NC) {
+          ok = barrier_wait(&code_free[cs], (unsigned)(it / NC - 1) & 1);
+          if (!ok) break;
         }
-        if (!h.live[p]) continue;
-        const uint8_t* src = a.scales + (first + n) * a.G + g0;
-        if (whole) {
-          h.v[p] = *reinterpret_cast<const unsigned*>(src);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (g0 + k < a.G) h.v[p] |= (unsigned)src[k] << 8 * k;
-        }
+        expect_bytes(&code_landed[cs], kCodes);
+        fetch_tile(smem_addr(code_ring + cs * kCodes), &code_map, d0, (int)first + it * kStep,
+                   &code_landed[cs]);
       }
-    };
-#pragma unroll
-    for (int u = 0; u < kScaleLook; ++u) request(u, held[u]);
-    for (int base = 0; base < steps && ok; base += kScaleLook)
-#pragma unroll
-      for (int u = 0; u < kScaleLook; ++u) {
-        const int it = base + u, slot = it % NS;
-        if (it >= steps || !ok) continue;
-        if (it >= NS)
-          ok = __all_sync(~0u, barrier_wait(&empty[slot], (unsigned)(it / NS - 1) & 1));
-        if (!ok) continue;
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          scale[slot][lane + 32 * p] = held[u].v[p];
-          const unsigned off = __ballot_sync(~0u, !held[u].live[p]);
-          if (lane == 0) masked[slot][p] = off;
-        }
-        __syncwarp();
-        if (lane == 0) barrier_arrive<1>(&landed[slot]);
-        request(it + kScaleLook, held[u]);
+      for (int k = it > NC ? it - NC : 0; k < it; ++k)
+        barrier_wait(&code_landed[k % NC], (unsigned)(k / NC) & 1);
+    }
+  } else {
+    if (lane == 0)
+      for (int it = 0; it < steps; ++it) {
+        const int slot = it % NS;
+        ok = barrier_wait(&dy_landed[slot], (unsigned)(it / NS) & 1);
+        if (!ok) break;
+        barrier_arrive<CG>(&full[slot]);
       }
   }
   __syncwarp();
@@ -697,15 +727,11 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
 #pragma unroll
       for (int k = 0; k < 16; ++k) out[(int64_t)(c + k) * kTile] = v[k];
     }
-  } else if (!ok && warp == kWarps + 1) {
-    // copies in flight must land before the CTA's memory is given up
-    for (int s = 0; s < NS; ++s)
-      for (unsigned ph = 0; ph < 2; ++ph) barrier_wait(&landed[s], ph);
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (CG > 1) sync_all<CG>();
-  if (warp == kWarps) {
+  if (warp == kDecoders) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (CG == 1)
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols));
