@@ -155,15 +155,13 @@ __global__ void __launch_bounds__(Layout<T, V, WR, PER>::kThreads) norm_forward_
       for (int k = 0; k < V; ++k) n[k] = live ? r[j][k] * rr * w2[k] : 0.f;
       put<T, V>(a.n.row(b, t), d[j], ok[j], n);
       if (a.codes) {  // the checkpoint holds what n holds after rounding
-        int8_t c[V];
+        Pack<int8_t, V> c;
+        Pack<T, V> rounded;
 #pragma unroll
-        for (int k = 0; k < V; ++k) n[k] = ok[j] ? to_f32(from_f32<T>(n[k])) : 0.f;
-        const uint8_t byte = pack_encode<T, V>(n, c);
+        for (int k = 0; k < V; ++k) rounded.v[k] = from_f32<T>(ok[j] ? n[k] : 0.f);
+        const uint8_t byte = pack_encode(rounded, c);
         if (d[j] < G * kPackGroup) {
-          Pack<int8_t, V> pc;
-#pragma unroll
-          for (int k = 0; k < V; ++k) pc.v[k] = c[k];
-          *reinterpret_cast<Pack<int8_t, V>*>(a.codes + row * G * kPackGroup + d[j]) = pc;
+          *reinterpret_cast<Pack<int8_t, V>*>(a.codes + row * G * kPackGroup + d[j]) = c;
           if (d[j] % kPackGroup == 0) a.scales[row * G + d[j] / kPackGroup] = byte;
         }
       }

@@ -63,6 +63,35 @@ inline bool seq_aligned(const semicrf_sequence& s, int64_t B, int64_t T, int ele
          (B <= 1 || s.batch_stride % n == 0) && (T <= 1 || s.time_stride % n == 0);
 }
 
+// Division by a fixed T for values below 2^31: multiply by a rounded-up
+// reciprocal and shift (Granlund and Montgomery).
+struct Divider {
+  unsigned d, mul, shift;
+};
+inline Divider make_divider(unsigned d) {
+  unsigned s = 0;
+  while ((1ull << s) < d) ++s;
+  return Divider{d, (unsigned)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+__device__ __forceinline__ unsigned quotient(unsigned n, const Divider& v) {
+  return (__umulhi(n, v.mul) + n) >> v.shift;
+}
+
+// Position n of a batch of sequences of T positions: its sequence and place there.
+struct Places {
+  int64_t T;
+  Divider by_t;
+  bool small;  // every n is below 2^31
+};
+inline Places make_places(int64_t B, int64_t T) {
+  const bool small = B * T < (1ll << 31);
+  return Places{T, make_divider(small && T ? (unsigned)T : 1u), small};
+}
+__device__ __forceinline__ void locate(const Places& p, int64_t n, int64_t& b, int64_t& t) {
+  b = p.small ? (int64_t)quotient((unsigned)n, p.by_t) : n / p.T;
+  t = n - b * p.T;
+}
+
 // Number of valid positions of sequence b (all T without lengths).
 __device__ __forceinline__ int64_t valid_length(const int64_t* lengths, int64_t b, int64_t T) {
   if (!lengths) return T;
@@ -104,30 +133,83 @@ __device__ __forceinline__ float pack_scale(uint8_t byte) {  // 255 (inf) times 
   return __int_as_float((int)byte << 23);
 }
 
+// The largest magnitude of a lane's values, as the bits of a float.
+template <class T, int V>
+__device__ __forceinline__ unsigned pack_top(const Pack<T, V>& v) {
+  unsigned top = 0;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    // 16-bit types order by their bits without the sign: two at a time
+    const unsigned* w = reinterpret_cast<const unsigned*>(v.v);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+#pragma unroll
+    for (int o = 1; o < kPackGroup / V; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(~0u, top, o));
+    const unsigned short one = (unsigned short)max(top & 0xffffu, top >> 16);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&one)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(to_f32(v.v[j])) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < kPackGroup / V; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+    return top;
+  }
+}
+
 // Codes of a group whose values lie V to a lane in 32 / V neighbouring lanes
 // (all lanes of the warp call this); returns the scale byte.
 template <class T, int V>
-__device__ __forceinline__ uint8_t pack_encode(const float (&v)[V], int8_t (&q)[V]) {
-  unsigned top = 0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 1; o < kPackGroup / V; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+__device__ __forceinline__ uint8_t pack_encode(const Pack<T, V>& v, Pack<int8_t, V>& q) {
   // top = m 2^p, 1/2 <= m < 1, exponent field p + 126: e is p - 7 where m <= 127/128, else p - 6
+  const unsigned top = pack_top(v);
   const int field = (int)(top >> 23);
-  int byte = field - 6 + ((top & 0x7fffffu) > 0x7e0000u);
-  byte = byte < 1 ? 1 : byte;
+  int byte = max(1, field - 6 + ((top & 0x7fffffu) > 0x7e0000u));
   if (top == 0) byte = 0;
   const bool finite = field < 255;
   if (!finite) byte = 255;
   const float inv = __int_as_float((254 - (finite ? byte : 254)) << 23);
-  const float most = fminf(127.f, floorf(largest_finite<T>() * inv));
+  // adding 1.5 * 2^23 rounds to the nearest integer, ties to even, into the low bits
+  int r[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float r = fminf(fmaxf(rintf(v[j] * inv), -most), most);
-    q[j] = finite ? (int8_t)(int)r : (int8_t)0;
+  for (int j = 0; j < V; ++j) r[j] = __float_as_int(fmaf(to_f32(v.v[j]), inv, 12582912.f));
+  const float most = floorf(largest_finite<T>() * inv);
+  if (!finite || most < 127.f) {  // the topmost scale of the type: no code past its largest value
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      r[j] = finite ? (int)fminf(fmaxf(rintf(to_f32(v.v[j]) * inv), -most), most) : 0;
+  }
+  if constexpr (V % 4 == 0) {
+    unsigned* w = reinterpret_cast<unsigned*>(q.v);
+#pragma unroll
+    for (int j = 0; j < V; j += 4)
+      w[j / 4] = __byte_perm(__byte_perm(r[j], r[j + 1], 0x0040),
+                             __byte_perm(r[j + 2], r[j + 3], 0x0040), 0x5410);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) q.v[j] = (int8_t)r[j];
   }
   return (uint8_t)byte;
+}
+
+// 8 codes to 8 bfloat16 values: code byte q = (q & 127) - (q & 128); either
+// part OR 0x4300 is a bfloat16 of 128 more, so their difference is q, exactly.
+__device__ __forceinline__ uint4 pack_decode(uint2 q, uint8_t byte) {
+  const __nv_bfloat162 unit = __bfloat162bfloat162(__float2bfloat16_rn(pack_scale(byte)));
+  unsigned o[4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned w = k ? q.y : q.x;
+    const unsigned lo = w & 0x7f7f7f7fu, hi = w & 0x80808080u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned pick = h ? 0x4342u : 0x4140u;  // two bytes, each below a 0x43
+      const unsigned a = __byte_perm(lo, 0x43434343u, pick), c = __byte_perm(hi, 0x43434343u, pick);
+      const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                               *reinterpret_cast<const __nv_bfloat162*>(&c)),
+                                       unit);
+      o[2 * k + h] = *reinterpret_cast<const unsigned*>(&v);
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 inline int launch_status() {

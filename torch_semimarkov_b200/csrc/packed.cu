@@ -3,68 +3,138 @@
 // Both directions are one pass, bound by memory: 2 + 1 + 1/32 bytes an
 // element for 16-bit activations.  A lane takes 16 bytes of a row, so the
 // lanes of a group of 32 channels are neighbours and its maximum is a few
-// shuffles.
+// shuffles.  A thread keeps its columns and takes kUnroll rows, all requested
+// before the first is used.
+
+#include <algorithm>
+#include <type_traits>
 
 #include "encoder_internal.cuh"
 
 namespace semicrf {
 namespace {
 
-template <class T, int V>
-__global__ void __launch_bounds__(256) pack_kernel(int64_t rows, int64_t T_, int64_t D, Seq<const T> x,
-                                                   const int64_t* __restrict__ lengths,
-                                                   int8_t* __restrict__ codes,
-                                                   uint8_t* __restrict__ scales) {
-  const int64_t G = pack_groups(D), per = G * (kPackGroup / V);
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t row = id / per, d = (id - row * per) * V;
-  const bool in = row < rows;  // lanes past the end still take part in the shuffles
-  float v[V] = {};
-  if (in) {
-    const int64_t b = row / T_, t = row - b * T_;
-    if (d < D && t < valid_length(lengths, b, T_)) {
-      const Pack<T, V> q = *reinterpret_cast<const Pack<T, V>*>(x.row(b, t) + d);
+constexpr int kThreads = 256, kUnroll = 4;
+
+// FLAT: every position is valid and all lie at one distance (x.st).
+template <class T, int V, bool FLAT>
+__global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, Places places, int64_t D,
+                                                        int64_t G, Seq<const T> x,
+                                                        const int64_t* __restrict__ lengths,
+                                                        int8_t* __restrict__ codes,
+                                                        uint8_t* __restrict__ scales) {
+  const int64_t first = ((int64_t)blockIdx.x * kUnroll) * blockDim.y + threadIdx.y;
+  const int64_t d = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
+  const int deep = blockDim.y;
+  const int left = (int)min((rows - first + deep - 1) / deep, (int64_t)kUnroll);  // rows here
+  const bool in = d < D;
+  Pack<T, V> q[kUnroll];
+  const T* src = x.p + first * x.st + d;
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = to_f32(q.v[k]);
+  for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) q[u].v[k] = from_f32<T>(0.f);
+    if (u < left && in) {
+      if (FLAT) {
+        q[u] = *reinterpret_cast<const Pack<T, V>*>(src);
+      } else {
+        int64_t b, t;
+        locate(places, first + u * deep, b, t);
+        if (!lengths || t < lengths[b])
+          q[u] = *reinterpret_cast<const Pack<T, V>*>(x.row(b, t) + d);
+      }
     }
+    src += deep * x.st;
   }
-  int8_t c[V];
-  const uint8_t byte = pack_encode<T, V>(v, c);
-  if (!in) return;
-  Pack<int8_t, V> pc;
+  const bool stored = d < G * kPackGroup, opens = d % kPackGroup == 0;
+  codes += first * G * kPackGroup + d;
+  scales += first * G + d / kPackGroup;
 #pragma unroll
-  for (int k = 0; k < V; ++k) pc.v[k] = c[k];
-  *reinterpret_cast<Pack<int8_t, V>*>(codes + row * G * kPackGroup + d) = pc;
-  if (d % kPackGroup == 0) scales[row * G + d / kPackGroup] = byte;
+  for (int u = 0; u < kUnroll; ++u) {
+    Pack<int8_t, V> c;
+    const uint8_t byte = pack_encode(q[u], c);  // lanes past the end hold zeros
+    if (u < left && stored) {
+      *reinterpret_cast<Pack<int8_t, V>*>(codes) = c;
+      if (opens) *scales = byte;
+    }
+    codes += deep * G * kPackGroup;
+    scales += deep * G;
+  }
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(256) unpack_kernel(int64_t rows, int64_t D,
-                                                     const int8_t* __restrict__ codes,
-                                                     const uint8_t* __restrict__ scales,
-                                                     T* __restrict__ out) {
-  const int64_t G = pack_groups(D), per = (D + V - 1) / V;
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t row = id / per, d = (id - row * per) * V;
-  if (row >= rows) return;
-  const float unit = pack_scale(scales[row * G + d / kPackGroup]);
-  const Pack<int8_t, V> c =
-      *reinterpret_cast<const Pack<int8_t, V>*>(codes + row * G * kPackGroup + d);
-  Pack<T, V> q;
+__global__ void __launch_bounds__(kThreads) unpack_kernel(int64_t rows, int64_t D, int64_t G,
+                                                          const int8_t* __restrict__ codes,
+                                                          const uint8_t* __restrict__ scales,
+                                                          T* __restrict__ out) {
+  const int64_t first = ((int64_t)blockIdx.x * kUnroll) * blockDim.y + threadIdx.y;
+  const int64_t d = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
+  const int deep = blockDim.y;
+  const int left = (int)min((rows - first + deep - 1) / deep, (int64_t)kUnroll);  // rows here
+  if (d >= D) return;
+  Pack<int8_t, V> c[kUnroll];
+  uint8_t byte[kUnroll];
+  codes += first * G * kPackGroup + d;
+  scales += first * G + d / kPackGroup;
 #pragma unroll
-  for (int k = 0; k < V; ++k) q.v[k] = from_f32<T>((float)c.v[k] * unit);
-  *reinterpret_cast<Pack<T, V>*>(out + row * D + d) = q;
+  for (int u = 0; u < kUnroll; ++u) {
+    if (u < left) {
+      byte[u] = *scales;
+      c[u] = *reinterpret_cast<const Pack<int8_t, V>*>(codes);
+    }
+    codes += deep * G * kPackGroup;
+    scales += deep * G;
+  }
+  out += first * D + d;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    if (u < left) {
+      Pack<T, V> q;
+      if constexpr (V == 8 && std::is_same<T, __nv_bfloat16>::value) {
+        *reinterpret_cast<uint4*>(&q) = pack_decode(*reinterpret_cast<const uint2*>(&c[u]), byte[u]);
+      } else {
+        const float unit = pack_scale(byte[u]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) q.v[k] = from_f32<T>((float)c[u].v[k] * unit);
+      }
+      *reinterpret_cast<Pack<T, V>*>(out) = q;
+    }
+    out += deep * D;
+  }
+}
+
+// A block as wide as a row's lane items (at most 256 of them), with as many
+// rows as fill its threads.  Items come in whole groups of 32 channels, so a
+// group never straddles two warps.
+struct Grid {
+  dim3 grid, block;
+  bool ok;
+};
+template <int V>
+Grid grid_of(int64_t rows, int64_t G) {
+  const int64_t per = G * (kPackGroup / V);
+  const unsigned wide = (unsigned)std::min<int64_t>(per, kThreads), deep = kThreads / wide;
+  const int64_t across = (per + wide - 1) / wide;
+  const int64_t down = (rows + (int64_t)deep * kUnroll - 1) / ((int64_t)deep * kUnroll);
+  return Grid{dim3((unsigned)down, (unsigned)across), dim3(wide, deep),
+              down <= 0x7fffffff && across <= 65535};
 }
 
 template <class T, int V>
 int launch_pack(int64_t B, int64_t T_, int64_t D, const semicrf_sequence& x,
                 const int64_t* lengths, int8_t* codes, uint8_t* scales, cudaStream_t stream) {
-  const int64_t n = B * T_ * pack_groups(D) * (kPackGroup / V);
-  const int64_t grid = (n + 255) / 256;
-  if (grid > 0x7fffffff) return SEMICRF_ERR_UNSUPPORTED;
-  if (grid)
-    pack_kernel<T, V><<<(unsigned)grid, 256, 0, stream>>>(B * T_, T_, D, as_seq<const T>(x),
-                                                          lengths, codes, scales);
+  const int64_t G = pack_groups(D);
+  const Grid g = grid_of<V>(B * T_, G);
+  if (!g.ok) return SEMICRF_ERR_UNSUPPORTED;
+  Seq<const T> xs = as_seq<const T>(x);
+  if (!lengths && (B == 1 || T_ == 1 || x.batch_stride == T_ * x.time_stride)) {
+    if (T_ == 1) xs.st = xs.sb;
+    pack_kernel<T, V, true><<<g.grid, g.block, 0, stream>>>(B * T_, Places{}, D, G, xs, nullptr,
+                                                            codes, scales);
+  } else {
+    pack_kernel<T, V, false><<<g.grid, g.block, 0, stream>>>(B * T_, make_places(B, T_), D, G, xs,
+                                                             lengths, codes, scales);
+  }
   return launch_status();
 }
 
@@ -80,12 +150,11 @@ int run_pack(int64_t B, int64_t T_, int64_t D, const semicrf_sequence& x, const 
 template <class T, int V>
 int launch_unpack(int64_t rows, int64_t D, const int8_t* codes, const uint8_t* scales, void* out,
                   cudaStream_t stream) {
-  const int64_t n = rows * ((D + V - 1) / V);
-  const int64_t grid = (n + 255) / 256;
-  if (grid > 0x7fffffff) return SEMICRF_ERR_UNSUPPORTED;
-  if (grid)
-    unpack_kernel<T, V><<<(unsigned)grid, 256, 0, stream>>>(rows, D, codes, scales,
-                                                            static_cast<T*>(out));
+  const int64_t G = pack_groups(D);
+  const Grid g = grid_of<V>(rows, G);
+  if (!g.ok) return SEMICRF_ERR_UNSUPPORTED;
+  unpack_kernel<T, V><<<g.grid, g.block, 0, stream>>>(rows, D, G, codes, scales,
+                                                      static_cast<T*>(out));
   return launch_status();
 }
 

@@ -61,20 +61,6 @@ struct Shape {
   static constexpr int kBytes = kStages * kStage + 1024;  // and room to align
 };
 
-// Division by a fixed T for values below 2^31: multiply by a rounded-up
-// reciprocal and shift (Granlund and Montgomery).
-struct Divider {
-  unsigned d, mul, shift;
-};
-Divider make_divider(unsigned d) {
-  unsigned s = 0;
-  while ((1ull << s) < d) ++s;
-  return Divider{d, (unsigned)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
-}
-__device__ __forceinline__ unsigned quotient(unsigned n, const Divider& v) {
-  return (__umulhi(n, v.mul) + n) >> v.shift;
-}
-
 struct GradArgs {
   int64_t N, M, Dp, G;  // positions, width of dy, code row bytes, scale row bytes
   int64_t run;          // positions of a tile, a multiple of kStep
@@ -188,28 +174,6 @@ __device__ __forceinline__ void read_columns(unsigned at, float (&f)[16]) {
 __device__ __forceinline__ uint64_t operand(unsigned addr) {
   return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(kAtom >> 4) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-
-// 8 codes to 8 bfloat16 values: code byte q = (q & 127) - (q & 128); either
-// part OR 0x4300 is a bfloat16 of 128 more, so their difference is q, exactly.
-__device__ __forceinline__ uint4 decode(uint2 q, uint8_t byte) {
-  const __nv_bfloat162 unit = __bfloat162bfloat162(__float2bfloat16_rn(pack_scale(byte)));
-  unsigned o[4];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const unsigned w = k ? q.y : q.x;
-    const unsigned lo = w & 0x7f7f7f7fu, hi = w & 0x80808080u;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const unsigned pick = h ? 0x4342u : 0x4140u;  // two bytes, each below a 0x43
-      const unsigned a = __byte_perm(lo, 0x43434343u, pick), c = __byte_perm(hi, 0x43434343u, pick);
-      const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
-                                               *reinterpret_cast<const __nv_bfloat162*>(&c)),
-                                       unit);
-      o[2 * k + h] = *reinterpret_cast<const unsigned*>(&v);
-    }
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // One value's pieces: each the leading 8 bits of what is left, by truncation,
@@ -382,7 +346,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
             *reinterpret_cast<uint4*>(at + j * kOperand) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        *reinterpret_cast<uint4*>(at + NP * kOperand) = decode(h.q[p], h.byte[p]);
+        *reinterpret_cast<uint4*>(at + NP * kOperand) = pack_decode(h.q[p], h.byte[p]);
       }
       if (ASYNC) asm volatile("cp.async.wait_group %0;" ::"n"(kLook - 1) : "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -626,7 +590,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
         const uint2 q = *reinterpret_cast<const uint2*>(codes + p * kRows * kTile);
         const unsigned bytes = __shfl_sync(~0u, scale, (row0 & 1) + 2 * p);
         *reinterpret_cast<uint4*>(base + kOperand + p * kRows * 128) =
-            decode(q, (uint8_t)(bytes >> (col >> 2) * 8));
+            pack_decode(q, (uint8_t)(bytes >> (col >> 2) * 8));
       }
       __syncwarp();
       if (lane == 0) barrier_arrive<1>(&code_free[cs]);
