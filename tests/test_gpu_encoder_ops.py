@@ -201,6 +201,10 @@ def test_recurrence_all_masked_and_empty():
     s0 = _normal(_gen(1), 2, 6)
     h, s = tsm.gated_linear_recurrence(nan, nan, s0, torch.tensor([0, 0]))
     assert torch.equal(h, torch.zeros_like(h)) and torch.equal(s, s0)
+    i = s0.clone().requires_grad_(True)
+    h, s = tsm.gated_linear_recurrence(nan, nan, i, torch.tensor([0, 0]))
+    (gi,) = torch.autograd.grad(s, i, 2 * s0)
+    assert torch.equal(gi, 2 * s0)
     x = torch.empty(2, 0, 6, device=dev, requires_grad=True)
     i = s0.clone().requires_grad_(True)
     h, s = tsm.gated_linear_recurrence(x, x, i)

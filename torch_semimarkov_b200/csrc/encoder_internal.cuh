@@ -99,14 +99,22 @@ __device__ __forceinline__ int64_t valid_length(const int64_t* lengths, int64_t 
   return n < 0 ? 0 : (n > T ? T : n);
 }
 
-// sigmoid(g) and sigmoid(-g), each to a few units of its own last place: with
-// e = exp(-|g|) both are quotients over 1 + e, so neither cancels.
+// sigmoid(g) and sigmoid(-g), each to a few units of its own last place:
+// with e = exp(-g) the first is 1 / (1 + e), the second e / (1 + e) for g > 0
+// and 1 minus the first else, so neither cancels.  e overflows to infinity
+// below g = -88, where the first is 0 and the second 1.  Two special-function
+// operations; their flushed subnormals are below 2^-126.
+__device__ __forceinline__ float exp_neg(float g) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  return e;
+}
+__device__ __forceinline__ void sigmoid_pair_of(float g, float e, float& pos, float& neg) {
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos) : "f"(1.f + e));
+  neg = g > 0.f ? e * pos : 1.f - pos;
+}
 __device__ __forceinline__ void sigmoid_pair(float g, float& pos, float& neg) {
-  const float e = __expf(-fabsf(g));
-  const float hi = __fdividef(1.f, 1.f + e);
-  const float lo = e * hi;
-  pos = g < 0.f ? lo : hi;
-  neg = g < 0.f ? hi : lo;
+  sigmoid_pair_of(g, exp_neg(g), pos, neg);
 }
 
 // ---------------------------------------------------------------------------

@@ -26,11 +26,10 @@
 // For float32 the leading piece is summed apart from the others and, every
 // 512 positions, moved from tensor memory to registers that round to nearest.
 
-#include <cuda.h>
-
 #include <algorithm>
 
 #include "encoder_internal.cuh"
+#include "tma.cuh"
 
 namespace semicrf {
 int device_sm_count();  // api.cu
@@ -43,7 +42,6 @@ constexpr int kAtom = kStep * 128;  // bytes of 64 channels of a stage: 64 rows 
 constexpr int kOperand = 2 * kAtom; // bytes of an operand of a stage
 constexpr int kWarps = 16;      // producers and readers of tensor memory; one more issues
 constexpr int kSegment = 8;     // float32: stages that tensor memory sums
-constexpr unsigned kWaitLimit = 1u << 20;
 
 template <class T>
 struct Form;  // pieces of a value; producer warps; warps that read tensor memory
@@ -76,12 +74,6 @@ struct GradArgs {
   float* partial;  // (runs, tiles_m, tiles_d, 128 CG, 128): a tile's columns one after another
 };
 
-__device__ __forceinline__ unsigned smem_addr(const void* p) {
-  return (unsigned)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void barrier_init(uint64_t* b, unsigned n) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n) : "memory");
-}
 __device__ __forceinline__ unsigned peer_addr(unsigned addr, unsigned rank) {
   unsigned r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -91,27 +83,11 @@ __device__ __forceinline__ unsigned peer_addr(unsigned addr, unsigned rank) {
 template <int CG>
 __device__ __forceinline__ void barrier_arrive(uint64_t* b) {
   if (CG == 1)
-    asm volatile("{.reg .b64 t; mbarrier.arrive.shared::cta.b64 t, [%0];}" ::"r"(smem_addr(b))
-                 : "memory");
+    barrier_arrive_here(b);
   else
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
                      peer_addr(smem_addr(b), 0))
                  : "memory");
-}
-// False when the phase does not complete within the limit.
-__device__ __forceinline__ bool barrier_wait(uint64_t* b, unsigned parity) {
-  for (unsigned k = 0; k < kWaitLimit; ++k) {
-    unsigned done;
-    asm volatile(
-        "{.reg .pred p;"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;"
-        "selp.u32 %0, 1, 0, p;}"
-        : "=r"(done)
-        : "r"(smem_addr(b)), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
 }
 // The barrier (of both CTAs of a pair) completes when the products issued so far have.
 template <int CG>
@@ -470,21 +446,6 @@ constexpr int kCodes = kStep * kTile;        // bytes of a stage's codes
 constexpr int kBulkBytes = kGroups * 2 * kOperand + kCodeSlots * kCodes + 1024;
 constexpr int kBulkThreads = 32 * (kDecoders + 4);
 
-__device__ __forceinline__ void expect_bytes(uint64_t* b, unsigned n) {
-  asm volatile("{.reg .b64 t; mbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;}" ::"r"(
-                   smem_addr(b)),
-               "r"(n)
-               : "memory");
-}
-__device__ __forceinline__ void fetch_tile(unsigned dst, const CUtensorMap* map, int x, int y,
-                                           uint64_t* b) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(smem_addr(b))
-      : "memory");
-}
-
 template <int CG>
 __global__ void __launch_bounds__(kBulkThreads, 1)
     weight_grad_bulk_kernel(const GradArgs a, const __grid_constant__ CUtensorMap dy_map,
@@ -770,34 +731,13 @@ int launch(const GradArgs& a, int runs, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? SEMICRF_OK : SEMICRF_ERR_CUDA;
 }
 
-// cuTensorMapEncodeTiled, looked up once: the library does not link libcuda.
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) !=
-            cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return fn;
-}
-
+// (width, rows) bytes or bfloat16 values, in boxes of one stage's positions
 bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t width,
               int64_t rows, int64_t row_bytes, int box, CUtensorMapSwizzle swizzle) {
-  const EncodeTiled encode = encode_tiled();
-  if (!encode) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
-  const cuuint32_t boxes[2] = {(cuuint32_t)box, (cuuint32_t)kStep}, ones[2] = {1, 1};
-  return encode(map, type, 2, const_cast<void*>(base), dims, strides, boxes, ones,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t boxes[2] = {(cuuint32_t)box, (cuuint32_t)kStep};
+  return make_tensor_map(map, type, 2, base, dims, strides, boxes, swizzle);
 }
 
 template <int CG>

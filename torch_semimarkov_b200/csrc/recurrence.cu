@@ -3,8 +3,8 @@
 //
 //   f = sigmoid(g),  h_u = f_u h_{u-1} + (1 - f_u) x_u
 //
-// u counts positions in scan order (t = u, or T-1-u when reversed); masked
-// positions have f = 1 and contribute nothing, so they pass the state on.
+// u counts positions in scan order (t = u; reversed, from the end of the last
+// chunk down); masked positions have f = 1 and contribute nothing, so they pass the state on.
 // Steps compose: (P, S) with h_out = P h_in + S, P the product of f, S the
 // result from zero.  f <= 1, so nothing overflows and no logarithm is needed.
 //
@@ -14,278 +14,401 @@
 // h_{u-1} is recomputed from the float32 state kept at the start of each
 // chunk, which is more exact than rereading the rounded h and one read less.
 //
-// The time axis is cut into chunks of kChunk positions.  A CTA of kWarps
-// warps owns one chunk of kTile channels: a warp owns kRun consecutive
-// positions, a lane two channels.  One pass composes each chunk, one joins
-// the chunks in order, one writes the outputs.
+// A CTA of eight warps walks a column (a sequence's tile of channels) in
+// chunks of 64 positions: a warp owns eight consecutive positions, a lane its
+// channels.  Each warp composes its positions, one barrier a chunk makes the
+// compositions known, and each warp goes from the state that entered the
+// chunk over the earlier warps' to its own start.  The next chunk's rows are
+// requested before the present one is joined, so loads are always in flight.
+//
+// Where there are fewer columns than CTAs fit on the device, a column's chunks
+// are cut into segments, one to a CTA.  A first launch composes each segment
+// but the last one; the walk then joins the segments before its own.  That
+// reads two of the tensors twice, against a device mostly idle.  (A single
+// pass in which CTAs wait for their predecessors' compositions was slower:
+// each held its registers through several dependent trips to L2.)
+// Every order of operations depends on sizes alone.
+
+#include <algorithm>
+#include <type_traits>
 
 #include "encoder_internal.cuh"
+#include "tma.cuh"
 
 namespace semicrf {
+int device_sm_count();  // api.cu
+
 namespace {
 
 constexpr int kRun = 8;                 // positions of a thread
 constexpr int kWarps = 8;               // threads along time
-constexpr int kChunk = kRun * kWarps;   // positions of a CTA
-constexpr int kLane = 2;                // channels of a thread
-constexpr int kTile = 32 * kLane;       // channels of a CTA
+constexpr int kChunk = kRun * kWarps;   // positions of a CTA at a time
 
 template <class T>
 struct ScanArgs {
-  int64_t B, T_, D, chunks, tiles;
+  int64_t B, T_, D;
+  int64_t chunks, per;  // chunks of a sequence, of a segment
+  int tiles, segments;
   bool reverse;
   Seq<const T> x, g, dh;
   Seq<T> h, dx, dg;
   const int64_t* lengths;
-  float2* agg;    // (B, chunks, D): a chunk's (P, S)
-  float* carry;   // (B, chunks, D): the state entering each chunk (forward)
-  float* gcarry;  // (B, chunks, D): mu entering each chunk from its successor (backward)
+  const float* first;  // (B, D): state before the first position / gradient of the last state
+  float* last;         // (B, D): state after the last / gradient of the first; may be null
+  float* carry;        // (B, chunks, D): the state entering each chunk; may be null (forward)
+  float2* composed;    // (B, segments, D)
 };
 
-// Where a CTA works: its sequence, chunk and channels.
-template <bool VEC>
+__device__ __forceinline__ float2 then(float2 a, float2 b) {  // b after a
+  return make_float2(b.x * a.x, fmaf(b.x, a.y, b.y));
+}
+
+// Where a CTA works.  A lane holds L channels: neighbours where rows can be
+// read as vectors, else 32 apart.  Slot lane + 32 j of a tile is lane's j-th.
+template <class T, int L, bool VEC>
 struct Place {
-  int64_t b, c, u0, len;
-  int d[kLane];
-  bool ok[kLane];
-  int lane, w;
-  template <class T>
-  __device__ Place(const ScanArgs<T>& a) {
-    const int64_t id = blockIdx.x;
-    const int64_t tile = id % a.tiles;
-    c = (id / a.tiles) % a.chunks;
-    b = id / a.tiles / a.chunks;
+  static constexpr int kTile = 32 * L;
+  int64_t b, len, d0;
+  int segment, lane, w;
+  bool ok[L];
+  __device__ explicit Place(const ScanArgs<T>& a) {
+    const int64_t id = blockIdx.x, tile = id % a.tiles, rest = id / a.tiles;
+    segment = (int)(rest % a.segments);
+    b = rest / a.segments;
     lane = threadIdx.x & 31;
     w = threadIdx.x >> 5;
-    u0 = c * kChunk + w * kRun;
     len = valid_length(a.lengths, b, a.T_);
+    d0 = tile * kTile;
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      d[j] = (int)(tile * kTile) + (VEC ? lane * kLane + j : lane + 32 * j);
-      ok[j] = d[j] < a.D;
-    }
+    for (int j = 0; j < L; ++j) ok[j] = channel(lane + 32 * j) < a.D;
   }
-  template <class T>
-  __device__ int64_t time(const ScanArgs<T>& a, int i) const {
-    return a.reverse ? a.T_ - 1 - (u0 + i) : u0 + i;
+  __device__ __forceinline__ int64_t channel(int slot) const {
+    return d0 + (VEC ? (slot & 31) * L + (slot >> 5) : slot);
   }
-  __device__ bool valid(int64_t t) const { return t >= 0 && t < len; }
+  __device__ __forceinline__ int64_t column0() const { return d0 + lane * (VEC ? L : 1); }
+  // position of scan index u
+  __device__ __forceinline__ int64_t time(const ScanArgs<T>& a, int64_t u) const {
+    return a.reverse ? a.chunks * kChunk - 1 - u : u;
+  }
+  // whether all of scan indexes [u, u + n) are valid positions
+  __device__ __forceinline__ bool whole(const ScanArgs<T>& a, int64_t u, int n) const {
+    const int64_t lo = a.reverse ? a.chunks * kChunk - u - n : u;
+    return lo + n <= len;
+  }
 };
 
-template <bool VEC, class T>
-__device__ __forceinline__ void load_row(const T* row, const int (&d)[kLane], const bool (&ok)[kLane],
-                                         bool live, float (&v)[kLane]) {
+template <bool VEC, class T, int L>
+__device__ __forceinline__ void load_lane(const T* p, const bool (&ok)[L], bool live,
+                                          Pack<T, L>& q) {
+#pragma unroll
+  for (int j = 0; j < L; ++j) q.v[j] = from_f32<T>(0.f);
   if (VEC) {
-    Pack<T, kLane> q;
-    if (live && ok[0]) {
-      q = *reinterpret_cast<const Pack<T, kLane>*>(row + d[0]);
-#pragma unroll
-      for (int j = 0; j < kLane; ++j) v[j] = to_f32(q.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kLane; ++j) v[j] = 0.f;
-    }
+    if (live && ok[0]) q = *reinterpret_cast<const Pack<T, L>*>(p);
   } else {
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) v[j] = live && ok[j] ? to_f32(row[d[j]]) : 0.f;
+    for (int j = 0; j < L; ++j)
+      if (live && ok[j]) q.v[j] = p[32 * j];
   }
 }
-
-template <bool VEC, class T>
-__device__ __forceinline__ void store_row(T* row, const int (&d)[kLane], const bool (&ok)[kLane],
-                                          const float (&v)[kLane]) {
+template <bool VEC, class T, int L>
+__device__ __forceinline__ void store_lane(T* p, const bool (&ok)[L], const float (&v)[L]) {
   if (VEC) {
     if (!ok[0]) return;
-    Pack<T, kLane> q;
+    Pack<T, L> q;
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) q.v[j] = from_f32<T>(v[j]);
-    *reinterpret_cast<Pack<T, kLane>*>(row + d[0]) = q;
+    for (int j = 0; j < L; ++j) q.v[j] = from_f32<T>(v[j]);
+    *reinterpret_cast<Pack<T, L>*>(p) = q;
   } else {
 #pragma unroll
-    for (int j = 0; j < kLane; ++j)
-      if (ok[j]) row[d[j]] = from_f32<T>(v[j]);
+    for (int j = 0; j < L; ++j)
+      if (ok[j]) p[32 * j] = from_f32<T>(v[j]);
   }
 }
 
-// Composes a chunk: (P, S) of the forward state, or with BWD of mu.
-template <class T, bool VEC, bool BWD>
-__global__ void __launch_bounds__(32 * kWarps) compose_kernel(ScanArgs<T> a) {
-  const Place<VEC> at(a);
-  __shared__ float2 part[kWarps][kTile];
-  float P[kLane], S[kLane];
+// kRun rows of one tensor, from scan index u on.
+template <bool VEC, class T, int L>
+__device__ __forceinline__ void load_run(const ScanArgs<T>& a, const Place<T, L, VEC>& at,
+                                         const Seq<const T>& s, int64_t u, bool whole,
+                                         Pack<T, L> (&q)[kRun]) {
+  const int64_t dir = a.reverse ? -1 : 1, t0 = at.time(a, u);
+  const T* p = s.row(at.b, t0) + at.column0();
 #pragma unroll
-  for (int j = 0; j < kLane; ++j) P[j] = 1.f, S[j] = 0.f;
-#pragma unroll
-  for (int k = 0; k < kRun; ++k) {
-    const int i = BWD ? kRun - 1 - k : k;
-    const int64_t t = at.time(a, i);
-    if (!at.valid(t)) continue;
-    float v[kLane], g[kLane];
-    load_row<VEC>(BWD ? a.dh.p ? a.dh.row(at.b, t) : nullptr : a.x.row(at.b, t), at.d, at.ok,
-                  !BWD || a.dh.p, v);
-    load_row<VEC>(a.g.row(at.b, t), at.d, at.ok, true, g);
-#pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      float f, n;
-      sigmoid_pair(g[j], f, n);
-      P[j] *= f;
-      S[j] = BWD ? f * (v[j] + S[j]) : fmaf(f, S[j], n * v[j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kLane; ++j) part[at.w][at.lane + 32 * j] = make_float2(P[j], S[j]);
-  __syncthreads();
-  if (at.w) return;
-#pragma unroll
-  for (int j = 0; j < kLane; ++j) {
-    float p = 1.f, s = 0.f;
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 q = part[BWD ? kWarps - 1 - w : w][at.lane + 32 * j];
-      s = fmaf(q.x, s, q.y);
-      p *= q.x;
-    }
-    if (at.ok[j]) a.agg[(at.b * a.chunks + at.c) * a.D + at.d[j]] = make_float2(p, s);
+  for (int i = 0; i < kRun; ++i) {
+    const int64_t t = t0 + dir * i;
+    load_lane<VEC>(p, at.ok, s.p && (whole || t < at.len), q[i]);
+    p += dir * s.st;
   }
 }
 
-// Joins the chunks of a channel in order.
-__global__ void join_kernel(int64_t B, int64_t chunks, int64_t D, bool descending,
-                            const float2* __restrict__ agg, const float* __restrict__ first,
-                            float* __restrict__ carry, float* __restrict__ last) {
-  const int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= B * D) return;
-  const int64_t base = n / D * chunks * D + n % D;
-  float s = first ? first[n] : 0.f;
+// The state that enters this CTA's segment: the segments before it, in order,
+// after `first`.  For slot tid of the tile.
+template <class T, int L, bool VEC>
+__device__ __forceinline__ float enter_segment(const ScanArgs<T>& a, const Place<T, L, VEC>& at,
+                                               bool descending, int64_t d) {
+  float state = a.first ? a.first[at.b * a.D + d] : 0.f;
+  const float2* p = a.composed + at.b * a.segments * a.D + d;
+  const int n = descending ? a.segments - 1 - at.segment : at.segment;
 #pragma unroll 8
-  for (int64_t k = 0; k < chunks; ++k) {
-    const int64_t i = base + (descending ? chunks - 1 - k : k) * D;
-    carry[i] = s;
-    const float2 q = agg[i];
-    s = fmaf(q.x, s, q.y);
+  for (int k = 0; k < n; ++k) {
+    const float2 q = p[(descending ? a.segments - 1 - k : k) * a.D];
+    state = fmaf(q.x, state, q.y);
   }
-  if (last) last[n] = s;
+  return state;
 }
 
-template <class T, bool VEC>
-__global__ void __launch_bounds__(32 * kWarps) forward_kernel(ScanArgs<T> a) {
-  const Place<VEC> at(a);
-  __shared__ float2 part[kWarps][kTile];
-  float f[kRun][kLane], b[kRun][kLane];
-  float P[kLane], S[kLane];
+// Composes every segment that another one follows: (P, S) of the state, or
+// with BWD of mu.  A warp composes one eighth of the segment's runs of eight
+// positions, in scan order.
+template <class T, int L, bool VEC, bool BWD>
+__global__ void __launch_bounds__(32 * kWarps) compose_kernel(const ScanArgs<T> a) {
+  using Pl = Place<T, L, VEC>;
+  const Pl at(a);
+  if (at.segment == (BWD ? 0 : a.segments - 1)) return;
+  __shared__ float2 part[kWarps][Pl::kTile];
+  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const int64_t runs = c1 - c0;  // of a warp: the segment has kWarps times as many
+  float2 sum[L];
 #pragma unroll
-  for (int j = 0; j < kLane; ++j) P[j] = 1.f, S[j] = 0.f;
-#pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    const int64_t t = at.time(a, i);
-    const bool live = at.valid(t);
-    float x[kLane], g[kLane];
-    load_row<VEC>(a.x.row(at.b, t), at.d, at.ok, live, x);
-    load_row<VEC>(a.g.row(at.b, t), at.d, at.ok, live, g);
-#pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      float n;
-      sigmoid_pair(g[j], f[i][j], n);
-      b[i][j] = live ? n * x[j] : 0.f;
-      if (!live) f[i][j] = 1.f;
-      P[j] *= f[i][j];
-      S[j] = fmaf(f[i][j], S[j], b[i][j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kLane; ++j) part[at.w][at.lane + 32 * j] = make_float2(P[j], S[j]);
-  __syncthreads();
-  float s[kLane];
-#pragma unroll
-  for (int j = 0; j < kLane; ++j) {
-    s[j] = at.ok[j] ? a.carry[(at.b * a.chunks + at.c) * a.D + at.d[j]] : 0.f;
-    for (int w = 0; w < at.w; ++w) {
-      const float2 q = part[w][at.lane + 32 * j];
-      s[j] = fmaf(q.x, s[j], q.y);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    const int64_t t = at.time(a, i);
-    if (t < 0 || t >= a.T_) continue;
-    float out[kLane];
-#pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      s[j] = fmaf(f[i][j], s[j], b[i][j]);
-      out[j] = at.valid(t) ? s[j] : 0.f;
-    }
-    store_row<VEC>(a.h.row(at.b, t), at.d, at.ok, out);
-  }
-}
-
-template <class T, bool VEC>
-__global__ void __launch_bounds__(32 * kWarps) backward_kernel(ScanArgs<T> a) {
-  const Place<VEC> at(a);
-  __shared__ float2 part[kWarps][kTile];
-  __shared__ float gpart[kWarps][kTile];
-  float f[kRun][kLane], n[kRun][kLane], x[kRun][kLane], dh[kRun][kLane];
-  float P[kLane], S[kLane];
-#pragma unroll
-  for (int j = 0; j < kLane; ++j) P[j] = 1.f, S[j] = 0.f;
-#pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    const int64_t t = at.time(a, i);
-    const bool live = at.valid(t);
-    float g[kLane];
-    load_row<VEC>(a.x.row(at.b, t), at.d, at.ok, live, x[i]);
-    load_row<VEC>(a.g.row(at.b, t), at.d, at.ok, live, g);
-    load_row<VEC>(a.dh.p ? a.dh.row(at.b, t) : nullptr, at.d, at.ok, live && a.dh.p, dh[i]);
-#pragma unroll
-    for (int j = 0; j < kLane; ++j) {
-      sigmoid_pair(g[j], f[i][j], n[i][j]);
-      if (!live) f[i][j] = 1.f, n[i][j] = 0.f;
-      P[j] *= f[i][j];
-      S[j] = fmaf(f[i][j], S[j], n[i][j] * x[i][j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kLane; ++j) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = kRun - 1; i >= 0; --i) m = f[i][j] * (dh[i][j] + m);
-    part[at.w][at.lane + 32 * j] = make_float2(P[j], S[j]);
-    gpart[at.w][at.lane + 32 * j] = m;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kLane; ++j) {
-    const int64_t k = (at.b * a.chunks + at.c) * a.D + at.d[j];
-    float s = at.ok[j] ? a.carry[k] : 0.f;
-    float mu = at.ok[j] ? a.gcarry[k] : 0.f;
-    for (int w = 0; w < at.w; ++w) {
-      const float2 q = part[w][at.lane + 32 * j];
-      s = fmaf(q.x, s, q.y);
-    }
-    for (int w = kWarps - 1; w > at.w; --w)
-      mu = fmaf(part[w][at.lane + 32 * j].x, mu, gpart[w][at.lane + 32 * j]);
+  for (int j = 0; j < L; ++j) sum[j] = make_float2(1.f, 0.f);
+  Pack<T, L> v[kRun], g[kRun];
+  const auto index = [&](int64_t r) {
+    return c0 * kChunk + (at.w * runs + (BWD ? runs - 1 - r : r)) * kRun;
+  };
+  const auto fetch = [&](int64_t r) {
+    const int64_t u = index(r);
+    const bool whole = at.whole(a, u, kRun);
+    load_run<VEC, T, L>(a, at, BWD ? a.dh : a.x, u, whole, v);
+    load_run<VEC, T, L>(a, at, a.g, u, whole, g);
+  };
+  fetch(0);
+  for (int64_t r = 0; r < runs; ++r) {
+    const int64_t u = index(r);
+    const bool whole = at.whole(a, u, kRun);
+    float f[kRun][L], s[kRun][L];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      const float before = s;
-      s = fmaf(f[i][j], s, n[i][j] * x[i][j]);
-      x[i][j] = before - x[i][j];
-    }
+      const int64_t t = at.time(a, u + i);
+      const bool live = whole || t < at.len;
 #pragma unroll
-    for (int i = kRun - 1; i >= 0; --i) {
-      const float lam = dh[i][j] + mu;
-      mu = f[i][j] * lam;
-      dh[i][j] = lam * n[i][j];              // dx
-      x[i][j] = mu * n[i][j] * x[i][j];      // dg
+      for (int j = 0; j < L; ++j) {
+        float n;
+        sigmoid_pair(to_f32(g[i].v[j]), f[i][j], n);
+        s[i][j] = BWD ? to_f32(v[i].v[j]) : n * to_f32(v[i].v[j]);
+        if (!live) f[i][j] = 1.f, s[i][j] = 0.f;
+      }
+    }
+    if (r + 1 < runs) fetch(r + 1);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      const int i = BWD ? kRun - 1 - k : k;
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        sum[j].y = BWD ? f[i][j] * (s[i][j] + sum[j].y) : fmaf(f[i][j], sum[j].y, s[i][j]);
+        sum[j].x *= f[i][j];
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    const int64_t t = at.time(a, i);
-    if (t < 0 || t >= a.T_) continue;
-    if (!at.valid(t)) {
+  for (int j = 0; j < L; ++j) part[at.w][at.lane + 32 * j] = sum[j];
+  __syncthreads();
+  const int tid = threadIdx.x;
+  if (tid >= Pl::kTile || at.channel(tid) >= a.D) return;
+  float2 own = make_float2(1.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < kLane; ++j) dh[i][j] = x[i][j] = 0.f;
+  for (int w = 0; w < kWarps; ++w) own = then(own, part[BWD ? kWarps - 1 - w : w][tid]);
+  a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
+}
+
+template <class T, int L, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps, 2) forward_kernel(const ScanArgs<T> a) {
+  using Pl = Place<T, L, VEC>;
+  constexpr int TILE = Pl::kTile;
+  __shared__ float2 part[2][kWarps][TILE];
+  __shared__ float enter[2][TILE];
+  const Pl at(a);
+  const int64_t dir = a.reverse ? -1 : 1;
+  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const int tid = threadIdx.x;
+  Pack<T, L> x[kRun], g[kRun];
+  const auto fetch = [&](int64_t c) {
+    const int64_t u = c * kChunk + at.w * kRun;
+    const bool whole = at.whole(a, c * kChunk, kChunk);
+    load_run<VEC, T, L>(a, at, a.x, u, whole, x);
+    load_run<VEC, T, L>(a, at, a.g, u, whole, g);
+  };
+  fetch(c0);
+  if (tid < TILE) {
+    const int64_t d = at.channel(tid);
+    enter[0][tid] = d < a.D ? enter_segment(a, at, false, d) : 0.f;
+  }
+  for (int64_t c = c0; c < c1; ++c) {
+    const int turn = (int)(c - c0) & 1;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
+    const bool whole = at.whole(a, c * kChunk, kChunk);
+    float f[kRun][L], s[kRun][L];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int64_t t = t0 + dir * i;
+      const bool live = whole || t < at.len;
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        float n;
+        sigmoid_pair(to_f32(g[i].v[j]), f[i][j], n);
+        s[i][j] = n * to_f32(x[i].v[j]);
+        if (!live) f[i][j] = 1.f, s[i][j] = 0.f;
+      }
     }
-    store_row<VEC>(a.dx.row(at.b, t), at.d, at.ok, dh[i]);
-    store_row<VEC>(a.dg.row(at.b, t), at.d, at.ok, x[i]);
+    if (c + 1 < c1) fetch(c + 1);
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      float2 q = make_float2(f[0][j], s[0][j]);
+#pragma unroll
+      for (int i = 1; i < kRun; ++i) q = then(q, make_float2(f[i][j], s[i][j]));
+      part[turn][at.w][at.lane + 32 * j] = q;
+    }
+    __syncthreads();
+    float h[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j) h[j] = enter[turn][at.lane + 32 * j];
+    if (a.carry && at.w == 0)
+#pragma unroll
+      for (int j = 0; j < L; ++j)
+        if (at.ok[j]) a.carry[(at.b * a.chunks + c) * a.D + at.channel(at.lane + 32 * j)] = h[j];
+    for (int w = 0; w < at.w; ++w)
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const float2 q = part[turn][w][at.lane + 32 * j];
+        h[j] = fmaf(q.x, h[j], q.y);
+      }
+    T* hp = a.h.row(at.b, t0) + at.column0();
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int64_t t = t0 + dir * i;
+      float out[L];
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        h[j] = fmaf(f[i][j], h[j], s[i][j]);
+        out[j] = whole || t < at.len ? h[j] : 0.f;
+      }
+      if (whole || t < a.T_) store_lane<VEC>(hp, at.ok, out);
+      hp += dir * a.h.st;
+    }
+    if (at.w == kWarps - 1)
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        enter[turn ^ 1][at.lane + 32 * j] = h[j];
+        if (a.last && c + 1 == a.chunks && at.ok[j])
+          a.last[at.b * a.D + at.channel(at.lane + 32 * j)] = h[j];
+      }
+  }
+}
+
+template <class T, int L, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps, 2) backward_kernel(const ScanArgs<T> a) {
+  using Pl = Place<T, L, VEC>;
+  constexpr int TILE = Pl::kTile;
+  __shared__ float2 part[2][kWarps][TILE];
+  __shared__ float mpart[2][kWarps][TILE];
+  __shared__ float enter[2][TILE];
+  const Pl at(a);
+  const int64_t dir = a.reverse ? -1 : 1;
+  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const int tid = threadIdx.x;
+  Pack<T, L> xq[kRun], gq[kRun], dq[kRun];
+  float before[L];  // the state entering the chunk
+  const auto fetch = [&](int64_t c) {
+    const int64_t u = c * kChunk + at.w * kRun;
+    const bool whole = at.whole(a, c * kChunk, kChunk);
+    load_run<VEC, T, L>(a, at, a.x, u, whole, xq);
+    load_run<VEC, T, L>(a, at, a.g, u, whole, gq);
+    load_run<VEC, T, L>(a, at, a.dh, u, whole, dq);
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+      before[j] = at.ok[j] ? a.carry[(at.b * a.chunks + c) * a.D + at.channel(at.lane + 32 * j)] : 0.f;
+  };
+  fetch(c1 - 1);
+  if (tid < TILE) {
+    const int64_t d = at.channel(tid);
+    enter[0][tid] = d < a.D ? enter_segment(a, at, true, d) : 0.f;
+  }
+  for (int64_t c = c1 - 1; c >= c0; --c) {
+    const int turn = (int)(c1 - 1 - c) & 1;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
+    const bool whole = at.whole(a, c * kChunk, kChunk);
+    float f[kRun][L], n[kRun][L], x[kRun][L], dh[kRun][L], h[L];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int64_t t = t0 + dir * i;
+      const bool live = whole || t < at.len;
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        sigmoid_pair(to_f32(gq[i].v[j]), f[i][j], n[i][j]);
+        if (!live) f[i][j] = 1.f, n[i][j] = 0.f;
+        x[i][j] = to_f32(xq[i].v[j]);
+        dh[i][j] = to_f32(dq[i].v[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < L; ++j) h[j] = before[j];
+    if (c > c0) fetch(c - 1);
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      float2 q = make_float2(1.f, 0.f);
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) q = then(q, make_float2(f[i][j], n[i][j] * x[i][j]));
+#pragma unroll
+      for (int i = kRun - 1; i >= 0; --i) m = f[i][j] * (dh[i][j] + m);
+      part[turn][at.w][at.lane + 32 * j] = q;
+      mpart[turn][at.w][at.lane + 32 * j] = m;
+    }
+    __syncthreads();
+    float mu[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const int slot = at.lane + 32 * j;
+      mu[j] = enter[turn][slot];
+      for (int w = 0; w < at.w; ++w) {
+        const float2 q = part[turn][w][slot];
+        h[j] = fmaf(q.x, h[j], q.y);
+      }
+      for (int w = kWarps - 1; w > at.w; --w)
+        mu[j] = fmaf(part[turn][w][slot].x, mu[j], mpart[turn][w][slot]);
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {  // x becomes h_{u-1} - x_u
+        const float prev = h[j];
+        h[j] = fmaf(f[i][j], h[j], n[i][j] * x[i][j]);
+        x[i][j] = prev - x[i][j];
+      }
+    }
+    T* xp = a.dx.row(at.b, t0 + dir * (kRun - 1)) + at.column0();
+    T* gp = a.dg.row(at.b, t0 + dir * (kRun - 1)) + at.column0();
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; --i) {
+      const int64_t t = t0 + dir * i;
+      const bool live = whole || t < at.len;
+      float dx[L], dg[L];
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const float lam = dh[i][j] + mu[j];
+        mu[j] = f[i][j] * lam;
+        dx[j] = live ? lam * n[i][j] : 0.f;
+        dg[j] = live ? mu[j] * n[i][j] * x[i][j] : 0.f;
+      }
+      if (whole || t < a.T_) {
+        store_lane<VEC>(xp, at.ok, dx);
+        store_lane<VEC>(gp, at.ok, dg);
+      }
+      xp -= dir * a.dx.st;
+      gp -= dir * a.dg.st;
+    }
+    if (at.w == 0)
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        enter[turn ^ 1][at.lane + 32 * j] = mu[j];
+        if (a.last && c == 0 && at.ok[j])
+          a.last[at.b * a.D + at.channel(at.lane + 32 * j)] = mu[j];
+      }
   }
 }
 
@@ -320,51 +443,512 @@ __global__ void step_kernel(int64_t B, int64_t D, const T* __restrict__ x, int64
   *reinterpret_cast<Pack<T, V>*>(h + b * D + d) = y;
 }
 
+// ---------------------------------------------------------------------------
+// The walk with its inputs brought by bulk copies: rows on 16-byte boundaries.
+// A producer thread keeps a ring of chunks of every input on their way to
+// shared memory; rows there lie at fixed offsets, so reading them costs no
+// address arithmetic, and nothing waits in registers.  A lane takes 8 bytes of
+// a row forward, 4 backward (three inputs and both factors fill the registers).
+// ---------------------------------------------------------------------------
+constexpr int kForwardLane = 8, kBackwardLane = 4;      // bytes
+constexpr int kForwardStages = 3, kBackwardStages = 3;  // chunks in the ring
+constexpr int box_bytes(int lane) { return 32 * lane * kChunk; }
+constexpr int ring_bytes(int lane, int tensors, int stages) {
+  return tensors * stages * box_bytes(lane) + 128;
+}
+
+__device__ __forceinline__ void compute_barrier() {
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
+}
+
+// A lane's part of row i of a warp's run, in scan order, in a tile in shared memory.
+template <class T, int L>
+__device__ __forceinline__ Pack<T, L> tile_row(const unsigned char* tile, int w, int lane, int i,
+                                               bool reverse) {
+  constexpr int kBytes = (int)sizeof(T) * L;
+  const int row = reverse ? kChunk - 1 - (w * kRun + i) : w * kRun + i;
+  return *reinterpret_cast<const Pack<T, L>*>(tile + (row * 32 + lane) * kBytes);
+}
+
+// Keeps the ring full: N tensors a chunk, `descending` in scan order for the backward.
+template <int BOX, class T, int N, int STAGES, class At>
+__device__ void produce(const ScanArgs<T>& a, const At& at, const CUtensorMap* const (&maps)[N],
+                        unsigned char* ring, uint64_t* full, uint64_t* empty, int64_t c0,
+                        int64_t c1, bool descending) {
+  int it = 0;
+  const int n = (int)(c1 - c0);
+  for (; it < n; ++it) {
+    const int slot = it % STAGES;
+    if (it >= STAGES && !barrier_wait(&empty[slot], (unsigned)(it / STAGES - 1) & 1)) break;
+    const int64_t c = descending ? c1 - 1 - it : c0 + it;
+    const int row = (int)(a.reverse ? a.chunks - 1 - c : c) * kChunk;
+    expect_bytes(&full[slot], N * BOX);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      fetch_tile(smem_addr(ring + (slot * N + k) * BOX), maps[k], (int)at.d0, row, (int)at.b,
+                 &full[slot]);
+  }
+  // no copy may still be in flight when the CTA's memory is given up
+  for (int k = it > STAGES ? it - STAGES : 0; k < it; ++k)
+    barrier_wait(&full[k % STAGES], (unsigned)(k / STAGES) & 1);
+}
+
+template <int STAGES>
+__device__ __forceinline__ void init_ring(uint64_t* full, uint64_t* empty) {
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      barrier_init(&full[s], 1);
+      barrier_init(&empty[s], kWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ unsigned char* align_ring(unsigned char* p) {
+  return reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(p) + 127) &
+                                          ~(uintptr_t)127);
+}
+
+// The forward walk, or with COMPOSE its (P, S) alone.
+template <class T, bool COMPOSE>
+__global__ void __launch_bounds__(32 * kWarps + 32, 2)
+    forward_bulk_kernel(const ScanArgs<T> a, const __grid_constant__ CUtensorMap x_map,
+                        const __grid_constant__ CUtensorMap g_map) {
+  constexpr int L = kForwardLane / (int)sizeof(T), TILE = 32 * L, ST = kForwardStages;
+  constexpr int kBox = box_bytes(kForwardLane);
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ float2 part[2][kWarps][TILE];
+  __shared__ float enter[2][TILE];
+  unsigned char* ring = align_ring(raw);
+  const Place<T, L, true> at(a);
+  if (COMPOSE && at.segment == a.segments - 1) return;
+  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const int tid = threadIdx.x;
+  init_ring<ST>(full, empty);
+  if (at.w == kWarps) {
+    const CUtensorMap* const maps[2] = {&x_map, &g_map};
+    if (at.lane == 0) produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, c0, c1, false);
+    return;
+  }
+  float2 own = make_float2(1.f, 0.f);
+  if (!COMPOSE && tid < TILE) {
+    const int64_t d = at.channel(tid);
+    enter[0][tid] = d < a.D ? enter_segment(a, at, false, d) : 0.f;
+  }
+  bool ok = true;
+  const int64_t step = a.reverse ? -a.h.st : a.h.st;
+  for (int64_t c = c0; c < c1; ++c) {
+    const int it = (int)(c - c0), slot = it % ST, turn = it & 1;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
+    const bool whole = at.whole(a, c * kChunk, kChunk);
+    if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
+    const unsigned char* xt = ring + slot * 2 * kBox;
+    float f[kRun][L], s[kRun][L];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const Pack<T, L> x = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
+      const Pack<T, L> g = tile_row<T, L>(xt + kBox, at.w, at.lane, i, a.reverse);
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        float n;
+        sigmoid_pair(to_f32(g.v[j]), f[i][j], n);
+        s[i][j] = n * to_f32(x.v[j]);
+      }
+    }
+    __syncwarp();
+    if (at.lane == 0) barrier_arrive_here(&empty[slot]);
+    if (!whole) {
+      const int64_t dir = a.reverse ? -1 : 1;
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        if (t0 + dir * i >= at.len)
+#pragma unroll
+          for (int j = 0; j < L; ++j) f[i][j] = 1.f, s[i][j] = 0.f;
+    }
+    if (!ok) f[0][0] = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      float2 q = make_float2(f[0][j], s[0][j]);
+#pragma unroll
+      for (int i = 1; i < kRun; ++i) q = then(q, make_float2(f[i][j], s[i][j]));
+      part[turn][at.w][at.lane + 32 * j] = q;
+    }
+    compute_barrier();
+    if (COMPOSE) {
+      if (tid < TILE)
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) own = then(own, part[turn][w][tid]);
+      continue;
+    }
+    float h[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j) h[j] = enter[turn][at.lane + 32 * j];
+    if (a.carry && at.w == 0)
+#pragma unroll
+      for (int j = 0; j < L; ++j)
+        if (at.ok[j]) a.carry[(at.b * a.chunks + c) * a.D + at.channel(at.lane + 32 * j)] = h[j];
+    for (int w = 0; w < at.w; ++w)
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const float2 q = part[turn][w][at.lane + 32 * j];
+        h[j] = fmaf(q.x, h[j], q.y);
+      }
+    T* hp = a.h.row(at.b, t0) + at.column0();
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+#pragma unroll
+        for (int j = 0; j < L; ++j) h[j] = fmaf(f[i][j], h[j], s[i][j]);
+        store_lane<true>(hp, at.ok, h);
+        hp += step;
+      }
+    } else {
+      const int64_t dir = a.reverse ? -1 : 1;
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        const int64_t t = t0 + dir * i;
+        float out[L];
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          h[j] = fmaf(f[i][j], h[j], s[i][j]);
+          out[j] = t < at.len ? h[j] : 0.f;
+        }
+        if (t < a.T_) store_lane<true>(hp, at.ok, out);
+        hp += step;
+      }
+    }
+    if (at.w == kWarps - 1)
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        enter[turn ^ 1][at.lane + 32 * j] = h[j];
+        if (a.last && c + 1 == a.chunks && at.ok[j])
+          a.last[at.b * a.D + at.channel(at.lane + 32 * j)] = h[j];
+      }
+  }
+  if (COMPOSE && tid < TILE && at.channel(tid) < a.D)
+    a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
+}
+
+// mu's (P, S) of every segment but the first.
+template <class T>
+__global__ void __launch_bounds__(32 * kWarps + 32, 2)
+    backward_compose_kernel(const ScanArgs<T> a, const __grid_constant__ CUtensorMap d_map,
+                            const __grid_constant__ CUtensorMap g_map) {
+  constexpr int L = kBackwardLane / (int)sizeof(T), TILE = 32 * L, ST = kBackwardStages;
+  constexpr int kBox = box_bytes(kBackwardLane);
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ float2 part[2][kWarps][TILE];
+  unsigned char* ring = align_ring(raw);
+  const Place<T, L, true> at(a);
+  if (at.segment == 0) return;
+  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const int tid = threadIdx.x;
+  init_ring<ST>(full, empty);
+  if (at.w == kWarps) {
+    const CUtensorMap* const maps[2] = {&d_map, &g_map};
+    if (at.lane == 0) produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, c0, c1, true);
+    return;
+  }
+  float2 own = make_float2(1.f, 0.f);
+  bool ok = true;
+  const int64_t dir = a.reverse ? -1 : 1;
+  for (int64_t c = c1 - 1; c >= c0; --c) {
+    const int it = (int)(c1 - 1 - c), slot = it % ST, turn = it & 1;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
+    const bool whole = at.whole(a, c * kChunk, kChunk);
+    if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
+    const unsigned char* dt = ring + slot * 2 * kBox;
+    float2 q[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j) q[j] = make_float2(ok ? 1.f : __uint_as_float(0x7fc00000u), 0.f);
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; --i) {
+      const Pack<T, L> d = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
+      const Pack<T, L> g = tile_row<T, L>(dt + kBox, at.w, at.lane, i, a.reverse);
+      if (!whole && t0 + dir * i >= at.len) continue;
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        float f, n;
+        sigmoid_pair(to_f32(g.v[j]), f, n);
+        q[j].x *= f;
+        q[j].y = f * (to_f32(d.v[j]) + q[j].y);
+      }
+    }
+    __syncwarp();
+    if (at.lane == 0) barrier_arrive_here(&empty[slot]);
+#pragma unroll
+    for (int j = 0; j < L; ++j) part[turn][at.w][at.lane + 32 * j] = q[j];
+    compute_barrier();
+    if (tid < TILE)
+#pragma unroll
+      for (int w = kWarps - 1; w >= 0; --w) own = then(own, part[turn][w][tid]);
+  }
+  if (tid < TILE && at.channel(tid) < a.D)
+    a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
+}
+
+template <class T>
+__global__ void __launch_bounds__(32 * kWarps + 32, 2)
+    backward_bulk_kernel(const ScanArgs<T> a, const __grid_constant__ CUtensorMap x_map,
+                         const __grid_constant__ CUtensorMap g_map,
+                         const __grid_constant__ CUtensorMap d_map) {
+  constexpr int L = kBackwardLane / (int)sizeof(T), TILE = 32 * L, ST = kBackwardStages;
+  constexpr int kBox = box_bytes(kBackwardLane);
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ float2 part[2][kWarps][TILE];
+  __shared__ float mpart[2][kWarps][TILE];
+  __shared__ float enter[2][TILE];
+  unsigned char* ring = align_ring(raw);
+  const Place<T, L, true> at(a);
+  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const int tid = threadIdx.x;
+  init_ring<ST>(full, empty);
+  if (at.w == kWarps) {
+    const CUtensorMap* const maps[3] = {&x_map, &g_map, &d_map};
+    if (at.lane == 0) produce<kBox, T, 3, ST>(a, at, maps, ring, full, empty, c0, c1, true);
+    return;
+  }
+  if (tid < TILE) {
+    const int64_t d = at.channel(tid);
+    enter[0][tid] = d < a.D ? enter_segment(a, at, true, d) : 0.f;
+  }
+  bool ok = true;
+  const int64_t dir = a.reverse ? -1 : 1;
+  for (int64_t c = c1 - 1; c >= c0; --c) {
+    const int it = (int)(c1 - 1 - c), slot = it % ST, turn = it & 1;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
+    const bool whole = at.whole(a, c * kChunk, kChunk);
+    float h[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+      h[j] = at.ok[j] ? a.carry[(at.b * a.chunks + c) * a.D + at.channel(at.lane + 32 * j)] : 0.f;
+    if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
+    const unsigned char* xt = ring + slot * 3 * kBox;
+    const unsigned char *gt = xt + kBox, *dt = gt + kBox;
+    // f and 1 - f of the run; masked positions have 1 and 0
+    float f[kRun][L], n[kRun][L];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const Pack<T, L> g = tile_row<T, L>(gt, at.w, at.lane, i, a.reverse);
+#pragma unroll
+      for (int j = 0; j < L; ++j) sigmoid_pair(to_f32(g.v[j]), f[i][j], n[i][j]);
+    }
+    const auto masked = [&](int i) { return !whole && t0 + dir * i >= at.len; };
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        if (masked(i))
+#pragma unroll
+          for (int j = 0; j < L; ++j) f[i][j] = 1.f, n[i][j] = 0.f;
+    }
+    if (!ok) f[0][0] = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+    {
+      float2 q[L];
+#pragma unroll
+      for (int j = 0; j < L; ++j) q[j] = make_float2(1.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        const Pack<T, L> x = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
+        const bool off = masked(i);
+#pragma unroll
+        for (int j = 0; j < L; ++j)
+          q[j] = then(q[j], make_float2(f[i][j], off ? 0.f : n[i][j] * to_f32(x.v[j])));
+      }
+      float m[L];
+#pragma unroll
+      for (int j = 0; j < L; ++j) m[j] = 0.f;
+#pragma unroll
+      for (int i = kRun - 1; i >= 0; --i) {
+        const Pack<T, L> d = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
+        const bool off = masked(i);
+#pragma unroll
+        for (int j = 0; j < L; ++j) m[j] = f[i][j] * ((off ? 0.f : to_f32(d.v[j])) + m[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        part[turn][at.w][at.lane + 32 * j] = q[j];
+        mpart[turn][at.w][at.lane + 32 * j] = m[j];
+      }
+    }
+    compute_barrier();
+    float mu[L], diff[kRun][L];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const int at_slot = at.lane + 32 * j;
+      mu[j] = enter[turn][at_slot];
+      for (int w = 0; w < at.w; ++w) {
+        const float2 q = part[turn][w][at_slot];
+        h[j] = fmaf(q.x, h[j], q.y);
+      }
+      for (int w = kWarps - 1; w > at.w; --w)
+        mu[j] = fmaf(part[turn][w][at_slot].x, mu[j], mpart[turn][w][at_slot]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const Pack<T, L> x = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        diff[i][j] = h[j] - to_f32(x.v[j]);
+        // f h + (1 - f) x, with the product that the composition used
+        h[j] = masked(i) ? h[j] : fmaf(f[i][j], h[j], n[i][j] * to_f32(x.v[j]));
+      }
+    }
+    const int64_t last = t0 + dir * (kRun - 1);
+    T* xp = a.dx.row(at.b, last) + at.column0();
+    T* gp = a.dg.row(at.b, last) + at.column0();
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; --i) {
+      const Pack<T, L> d = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
+      const bool off = masked(i);
+      float dx[L], dg[L];
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        const float lam = (off ? 0.f : to_f32(d.v[j])) + mu[j];
+        mu[j] = f[i][j] * lam;
+        dx[j] = off ? 0.f : lam * n[i][j];
+        dg[j] = off ? 0.f : mu[j] * n[i][j] * diff[i][j];
+      }
+      if (whole || t0 + dir * i < a.T_) {
+        store_lane<true>(xp, at.ok, dx);
+        store_lane<true>(gp, at.ok, dg);
+      }
+      xp -= dir * a.dx.st;
+      gp -= dir * a.dg.st;
+    }
+    __syncwarp();
+    if (at.lane == 0) barrier_arrive_here(&empty[slot]);
+    if (at.w == 0)
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        enter[turn ^ 1][at.lane + 32 * j] = mu[j];
+        if (a.last && c == 0 && at.ok[j])
+          a.last[at.b * a.D + at.channel(at.lane + 32 * j)] = mu[j];
+      }
+  }
+}
+
 int64_t chunks_of(int64_t T) { return (T + kChunk - 1) / kChunk; }
 
 template <class T>
-ScanArgs<T> scan_args(const semicrf_recurrence* p) {
+constexpr int forward_lane() { return kForwardLane / (int)sizeof(T); }
+template <class T>
+constexpr int backward_lane() { return kBackwardLane / (int)sizeof(T); }
+
+struct Cut {
+  int tiles, segments;
+  int64_t per;
+};
+// Segments: as many as fill the device's CTA slots once.
+Cut cut_of(int64_t B, int64_t T, int64_t D, int tile) {
+  Cut c;
+  c.tiles = (int)((D + tile - 1) / tile);
+  const int64_t columns = B * c.tiles, chunks = chunks_of(T), slots = 2 * device_sm_count();
+  const int64_t want = columns ? std::max<int64_t>(1, std::min(slots / columns, chunks)) : 1;
+  c.per = (chunks + want - 1) / want;
+  c.segments = c.per ? (int)((chunks + c.per - 1) / c.per) : 1;
+  return c;
+}
+
+template <class T>
+ScanArgs<T> scan_args(const semicrf_recurrence* p, int tile, void* workspace) {
+  const Cut c = cut_of(p->batch, p->T, p->D, tile);
   ScanArgs<T> a{};
   a.B = p->batch;
   a.T_ = p->T;
   a.D = p->D;
   a.chunks = chunks_of(p->T);
-  a.tiles = (p->D + kTile - 1) / kTile;
+  a.per = c.per;
+  a.tiles = c.tiles;
+  a.segments = c.segments;
   a.reverse = p->reverse != 0;
   a.x = as_seq<const T>(p->x);
   a.g = as_seq<const T>(p->gate);
   a.lengths = p->lengths;
+  a.composed = static_cast<float2*>(workspace);
   return a;
+}
+
+// Without positions the last state is the first.
+int copy_state(const semicrf_recurrence* p, const float* first, float* last, cudaStream_t stream) {
+  if (!last) return SEMICRF_OK;
+  const size_t bytes = sizeof(float) * p->batch * p->D;
+  const cudaError_t e = first ? cudaMemcpyAsync(last, first, bytes, cudaMemcpyDeviceToDevice, stream)
+                              : cudaMemsetAsync(last, 0, bytes, stream);
+  return e == cudaSuccess ? SEMICRF_OK : SEMICRF_ERR_CUDA;
+}
+
+template <class T, int L, bool VEC, bool BWD>
+int launch_scan(const ScanArgs<T>& a, cudaStream_t stream) {
+  const unsigned grid = (unsigned)(a.B * a.tiles * a.segments);
+  if (a.segments > 1) compose_kernel<T, L, VEC, BWD><<<grid, 32 * kWarps, 0, stream>>>(a);
+  if constexpr (BWD)
+    backward_kernel<T, L, VEC><<<grid, 32 * kWarps, 0, stream>>>(a);
+  else
+    forward_kernel<T, L, VEC><<<grid, 32 * kWarps, 0, stream>>>(a);
+  return launch_status();
+}
+
+// Whether bulk copies can read s: 16-byte rows, no two of them overlapping.
+bool bulk_readable(const semicrf_sequence& s, int64_t B, int64_t T, int64_t D, int elem) {
+  return s.data && T < (1ll << 30) && B < (1ll << 30) && seq_aligned(s, B, T, elem, 16 / elem) &&
+         (T == 1 || (s.time_stride >= D && s.time_stride < (1ll << 36))) &&
+         (B == 1 || (s.batch_stride >= D && s.batch_stride < (1ll << 36)));
+}
+
+template <class T>
+bool sequence_map(CUtensorMap* map, const semicrf_sequence& s, int64_t B, int64_t T_, int64_t D,
+                  int lane) {
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<T, __half>::value
+                                       ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint64_t row = (cuuint64_t)((D * sizeof(T) + 15) / 16 * 16);  // where there is one row
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)T_, (cuuint64_t)B};
+  const cuuint64_t strides[2] = {T_ == 1 ? row : (cuuint64_t)s.time_stride * sizeof(T),
+                                 B == 1 ? row : (cuuint64_t)s.batch_stride * sizeof(T)};
+  const cuuint32_t box[3] = {(cuuint32_t)(32 * lane), (cuuint32_t)kChunk, 1};
+  return make_tensor_map(map, type, 3, s.data, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <class K>
+bool allow_shared(K kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) ==
+         cudaSuccess;
 }
 
 template <class T>
 int run_forward(const semicrf_recurrence* p, const semicrf_sequence& h, float* final_state,
                 void* saved, void* workspace, cudaStream_t stream) {
-  ScanArgs<T> a = scan_args<T>(p);
+  if (p->T == 0) return copy_state(p, p->initial_state, final_state, stream);
+  constexpr int L = forward_lane<T>();
+  ScanArgs<T> a = scan_args<T>(p, 32 * L, workspace);
   a.h = as_seq<T>(h);
-  a.agg = static_cast<float2*>(workspace);
-  a.carry = saved ? static_cast<float*>(saved)
-                  : reinterpret_cast<float*>(a.agg + a.B * a.chunks * a.D);
-  const unsigned grid = (unsigned)(a.B * a.chunks * a.tiles);
-  const bool vec = p->D % kLane == 0 && seq_aligned(p->x, a.B, a.T_, sizeof(T), kLane) &&
-                   seq_aligned(p->gate, a.B, a.T_, sizeof(T), kLane) &&
-                   seq_aligned(h, a.B, a.T_, sizeof(T), kLane);
-  if (grid) {
-    if (vec)
-      compose_kernel<T, true, false><<<grid, 32 * kWarps, 0, stream>>>(a);
-    else
-      compose_kernel<T, false, false><<<grid, 32 * kWarps, 0, stream>>>(a);
+  a.first = p->initial_state;
+  a.last = final_state;
+  a.carry = static_cast<float*>(saved);
+  bool vec = p->D % L == 0;
+  for (const semicrf_sequence* s : {&p->x, &p->gate, &h})
+    vec = vec && seq_aligned(*s, a.B, a.T_, sizeof(T), L);
+  if (vec && bulk_readable(p->x, a.B, a.T_, a.D, sizeof(T)) &&
+      bulk_readable(p->gate, a.B, a.T_, a.D, sizeof(T))) {
+    CUtensorMap xm, gm;
+    const auto walk = forward_bulk_kernel<T, false>;
+    const auto compose = forward_bulk_kernel<T, true>;
+    constexpr int bytes = ring_bytes(kForwardLane, 2, kForwardStages);
+    if (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, L) ||
+        !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, L) || !allow_shared(walk, bytes) ||
+        !allow_shared(compose, bytes))
+      return SEMICRF_ERR_CUDA;
+    const unsigned grid = (unsigned)(a.B * a.tiles * a.segments);
+    if (a.segments > 1) compose<<<grid, 32 * kWarps + 32, bytes, stream>>>(a, xm, gm);
+    walk<<<grid, 32 * kWarps + 32, bytes, stream>>>(a, xm, gm);
+    return launch_status();
   }
-  const unsigned jg = (unsigned)((a.B * a.D + 127) / 128);
-  join_kernel<<<jg, 128, 0, stream>>>(a.B, a.chunks, a.D, false, a.agg, p->initial_state, a.carry,
-                                      final_state);
-  if (grid) {
-    if (vec)
-      forward_kernel<T, true><<<grid, 32 * kWarps, 0, stream>>>(a);
-    else
-      forward_kernel<T, false><<<grid, 32 * kWarps, 0, stream>>>(a);
-  }
-  return launch_status();
+  return vec ? launch_scan<T, L, true, false>(a, stream) : launch_scan<T, L, false, false>(a, stream);
 }
 
 template <class T>
@@ -372,35 +956,37 @@ int run_backward(const semicrf_recurrence* p, const void* saved, const semicrf_s
                  const float* grad_state, const semicrf_sequence& grad_x,
                  const semicrf_sequence& grad_gate, float* grad_initial, void* workspace,
                  cudaStream_t stream) {
-  ScanArgs<T> a = scan_args<T>(p);
+  if (p->T == 0) return copy_state(p, grad_state, grad_initial, stream);
+  constexpr int L = backward_lane<T>();
+  ScanArgs<T> a = scan_args<T>(p, 32 * L, workspace);
   a.dh = as_seq<const T>(grad_h);
   a.dx = as_seq<T>(grad_x);
   a.dg = as_seq<T>(grad_gate);
+  a.first = grad_state;
+  a.last = grad_initial;
   a.carry = const_cast<float*>(static_cast<const float*>(saved));
-  a.agg = static_cast<float2*>(workspace);
-  a.gcarry = reinterpret_cast<float*>(a.agg + a.B * a.chunks * a.D);
-  const unsigned grid = (unsigned)(a.B * a.chunks * a.tiles);
-  const bool vec = p->D % kLane == 0 && seq_aligned(p->x, a.B, a.T_, sizeof(T), kLane) &&
-                   seq_aligned(p->gate, a.B, a.T_, sizeof(T), kLane) &&
-                   seq_aligned(grad_h, a.B, a.T_, sizeof(T), kLane) &&
-                   seq_aligned(grad_x, a.B, a.T_, sizeof(T), kLane) &&
-                   seq_aligned(grad_gate, a.B, a.T_, sizeof(T), kLane);
-  if (grid) {
-    if (vec)
-      compose_kernel<T, true, true><<<grid, 32 * kWarps, 0, stream>>>(a);
-    else
-      compose_kernel<T, false, true><<<grid, 32 * kWarps, 0, stream>>>(a);
+  bool vec = p->D % L == 0;
+  for (const semicrf_sequence* s : {&p->x, &p->gate, &grad_h, &grad_x, &grad_gate})
+    vec = vec && seq_aligned(*s, a.B, a.T_, sizeof(T), L);
+  if (vec && bulk_readable(p->x, a.B, a.T_, a.D, sizeof(T)) &&
+      bulk_readable(p->gate, a.B, a.T_, a.D, sizeof(T)) &&
+      bulk_readable(grad_h, a.B, a.T_, a.D, sizeof(T))) {
+    CUtensorMap xm, gm, dm;
+    const auto walk = backward_bulk_kernel<T>;
+    const auto compose = backward_compose_kernel<T>;
+    constexpr int walk_bytes = ring_bytes(kBackwardLane, 3, kBackwardStages);
+    constexpr int compose_bytes = ring_bytes(kBackwardLane, 2, kBackwardStages);
+    if (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, L) ||
+        !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, L) ||
+        !sequence_map<T>(&dm, grad_h, a.B, a.T_, a.D, L) || !allow_shared(walk, walk_bytes) ||
+        !allow_shared(compose, compose_bytes))
+      return SEMICRF_ERR_CUDA;
+    const unsigned grid = (unsigned)(a.B * a.tiles * a.segments);
+    if (a.segments > 1) compose<<<grid, 32 * kWarps + 32, compose_bytes, stream>>>(a, dm, gm);
+    walk<<<grid, 32 * kWarps + 32, walk_bytes, stream>>>(a, xm, gm, dm);
+    return launch_status();
   }
-  const unsigned jg = (unsigned)((a.B * a.D + 127) / 128);
-  join_kernel<<<jg, 128, 0, stream>>>(a.B, a.chunks, a.D, true, a.agg, grad_state, a.gcarry,
-                                      grad_initial);
-  if (grid) {
-    if (vec)
-      backward_kernel<T, true><<<grid, 32 * kWarps, 0, stream>>>(a);
-    else
-      backward_kernel<T, false><<<grid, 32 * kWarps, 0, stream>>>(a);
-  }
-  return launch_status();
+  return vec ? launch_scan<T, L, true, true>(a, stream) : launch_scan<T, L, false, true>(a, stream);
 }
 
 template <class T>
@@ -432,7 +1018,13 @@ size_t recurrence_saved_bytes(const semicrf_recurrence* p) {
   return sizeof(float) * p->batch * chunks_of(p->T) * p->D;
 }
 size_t recurrence_workspace_bytes(const semicrf_recurrence* p) {
-  return (sizeof(float2) + sizeof(float)) * p->batch * chunks_of(p->T) * p->D;
+  const bool wide = p->dtype == SEMICRF_F32;
+  const int tiles[2] = {32 * (wide ? forward_lane<float>() : forward_lane<__half>()),
+                        32 * (wide ? backward_lane<float>() : backward_lane<__half>())};
+  int segments = 1;
+  for (const int tile : tiles)
+    segments = std::max(segments, cut_of(p->batch, p->T, p->D, tile).segments);
+  return sizeof(float2) * p->batch * segments * p->D;
 }
 
 int recurrence_forward(const semicrf_recurrence* p, const semicrf_sequence& h, float* final_state,
