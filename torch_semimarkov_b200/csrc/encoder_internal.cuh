@@ -99,22 +99,17 @@ __device__ __forceinline__ int64_t valid_length(const int64_t* lengths, int64_t 
   return n < 0 ? 0 : (n > T ? T : n);
 }
 
-// sigmoid(g) and sigmoid(-g), each to a few units of its own last place:
-// with e = exp(-g) the first is 1 / (1 + e), the second e / (1 + e) for g > 0
-// and 1 minus the first else, so neither cancels.  e overflows to infinity
-// below g = -88, where the first is 0 and the second 1.  Two special-function
-// operations; their flushed subnormals are below 2^-126.
-__device__ __forceinline__ float exp_neg(float g) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  return e;
-}
-__device__ __forceinline__ void sigmoid_pair_of(float g, float e, float& pos, float& neg) {
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos) : "f"(1.f + e));
-  neg = g > 0.f ? e * pos : 1.f - pos;
-}
+// sigmoid(g) and sigmoid(-g), each to two units of its own last place: with
+// e = exp(-g) they are 1 / (1 + e) and e / (1 + e), so neither cancels.  e is
+// held to 2^126, where the first is 2^-126; a NaN stays one.  Six operations,
+// two of them special functions.
 __device__ __forceinline__ void sigmoid_pair(float g, float& pos, float& neg) {
-  sigmoid_pair_of(g, exp_neg(g), pos, neg);
+  float e;
+  asm("{.reg .f32 t; min.NaN.f32 t, %1, 0f42FC0000; ex2.approx.ftz.f32 %0, t;}"
+      : "=f"(e)
+      : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos) : "f"(1.f + e));
+  neg = e * pos;
 }
 
 // ---------------------------------------------------------------------------

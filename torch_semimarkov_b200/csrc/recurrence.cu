@@ -510,6 +510,42 @@ __device__ __forceinline__ unsigned char* align_ring(unsigned char* p) {
                                           ~(uintptr_t)127);
 }
 
+// The chunks of a segment that hold valid positions, in scan order.  The other
+// chunks take no part in a walk: the state passes them unchanged.
+struct Range {
+  int64_t c0, c1;  // the segment's chunks
+  int64_t v0, v1;  // those with valid positions
+};
+template <class T, int L>
+__device__ __forceinline__ Range range_of(const ScanArgs<T>& a, const Place<T, L, true>& at) {
+  Range r;
+  r.c0 = at.segment * a.per;
+  r.c1 = min(r.c0 + a.per, a.chunks);
+  const int64_t n = (at.len + kChunk - 1) / kChunk;
+  r.v0 = a.reverse ? max(r.c0, a.chunks - n) : r.c0;
+  r.v1 = a.reverse ? r.c1 : min(r.c1, n);
+  if (r.v1 < r.v0) r.v1 = r.v0;
+  return r;
+}
+// Zeros in every row of the segment's other chunks, by the CTA's first 256 threads.
+template <class T, int L>
+__device__ void clear_rest(const ScanArgs<T>& a, const Place<T, L, true>& at, const Range& r,
+                           const Seq<T>& out) {
+  const int64_t rest = (r.c1 - r.c0) - (r.v1 - r.v0);
+  const float zero[L] = {};
+  for (int64_t k = 0; k < rest; ++k) {
+    const int64_t c = a.reverse ? r.c0 + k : r.v1 + k;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int64_t t = at.time(a, c * kChunk + at.w * kRun + i);
+      if (t < a.T_) store_lane<true>(out.row(at.b, t) + at.column0(), at.ok, zero);
+    }
+  }
+}
+
+struct Masked { static constexpr bool value = true; };
+struct Whole { static constexpr bool value = false; };
+
 // The forward walk, or with COMPOSE its (P, S) alone.
 template <class T, bool COMPOSE>
 __global__ void __launch_bounds__(32 * kWarps + 32, 2)
@@ -517,19 +553,21 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
                         const __grid_constant__ CUtensorMap g_map) {
   constexpr int L = kForwardLane / (int)sizeof(T), TILE = 32 * L, ST = kForwardStages;
   constexpr int kBox = box_bytes(kForwardLane);
+  constexpr int kParts = COMPOSE ? kWarps : kWarps - 1;  // the last warp's has no reader in a walk
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[ST], empty[ST];
-  __shared__ float2 part[2][kWarps][TILE];
-  __shared__ float enter[2][TILE];
+  __shared__ float2 part[2][kParts][TILE];
+  __shared__ float enter[2][COMPOSE ? 1 : TILE];
   unsigned char* ring = align_ring(raw);
   const Place<T, L, true> at(a);
   if (COMPOSE && at.segment == a.segments - 1) return;
-  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const Range range = range_of(a, at);
   const int tid = threadIdx.x;
   init_ring<ST>(full, empty);
   if (at.w == kWarps) {
     const CUtensorMap* const maps[2] = {&x_map, &g_map};
-    if (at.lane == 0) produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, c0, c1, false);
+    if (at.lane == 0)
+      produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, range.v0, range.v1, false);
     return;
   }
   float2 own = make_float2(1.f, 0.f);
@@ -539,10 +577,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
   }
   bool ok = true;
   const int64_t step = a.reverse ? -a.h.st : a.h.st;
-  for (int64_t c = c0; c < c1; ++c) {
-    const int it = (int)(c - c0), slot = it % ST, turn = it & 1;
-    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
-    const bool whole = at.whole(a, c * kChunk, kChunk);
+  int turn = 0;
+  const auto chunk = [&](int64_t c, auto kind) {
+    constexpr bool kMasked = decltype(kind)::value;
+    const int it = (int)(c - range.v0), slot = it % ST;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun), dir = a.reverse ? -1 : 1;
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
     const unsigned char* xt = ring + slot * 2 * kBox;
     float f[kRun][L], s[kRun][L];
@@ -555,32 +594,27 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
         float n;
         sigmoid_pair(to_f32(g.v[j]), f[i][j], n);
         s[i][j] = n * to_f32(x.v[j]);
+        if (kMasked && t0 + dir * i >= at.len) f[i][j] = 1.f, s[i][j] = 0.f;
       }
     }
     __syncwarp();
     if (at.lane == 0) barrier_arrive_here(&empty[slot]);
-    if (!whole) {
-      const int64_t dir = a.reverse ? -1 : 1;
-#pragma unroll
-      for (int i = 0; i < kRun; ++i)
-        if (t0 + dir * i >= at.len)
-#pragma unroll
-          for (int j = 0; j < L; ++j) f[i][j] = 1.f, s[i][j] = 0.f;
-    }
     if (!ok) f[0][0] = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+    if (COMPOSE || at.w < kParts)
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      float2 q = make_float2(f[0][j], s[0][j]);
+      for (int j = 0; j < L; ++j) {
+        float2 q = make_float2(f[0][j], s[0][j]);
 #pragma unroll
-      for (int i = 1; i < kRun; ++i) q = then(q, make_float2(f[i][j], s[i][j]));
-      part[turn][at.w][at.lane + 32 * j] = q;
-    }
+        for (int i = 1; i < kRun; ++i) q = then(q, make_float2(f[i][j], s[i][j]));
+        part[turn][at.w][at.lane + 32 * j] = q;
+      }
     compute_barrier();
     if (COMPOSE) {
       if (tid < TILE)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) own = then(own, part[turn][w][tid]);
-      continue;
+        for (int w = 0; w < kParts; ++w) own = then(own, part[turn][w][tid]);
+      turn ^= 1;
+      return;
     }
     float h[L];
 #pragma unroll
@@ -596,39 +630,38 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
         h[j] = fmaf(q.x, h[j], q.y);
       }
     T* hp = a.h.row(at.b, t0) + at.column0();
-    if (whole) {
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-#pragma unroll
-        for (int j = 0; j < L; ++j) h[j] = fmaf(f[i][j], h[j], s[i][j]);
-        store_lane<true>(hp, at.ok, h);
-        hp += step;
-      }
-    } else {
-      const int64_t dir = a.reverse ? -1 : 1;
-#pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        const int64_t t = t0 + dir * i;
-        float out[L];
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-          h[j] = fmaf(f[i][j], h[j], s[i][j]);
-          out[j] = t < at.len ? h[j] : 0.f;
-        }
-        if (t < a.T_) store_lane<true>(hp, at.ok, out);
-        hp += step;
-      }
-    }
-    if (at.w == kWarps - 1)
+    for (int i = 0; i < kRun; ++i) {
+      const int64_t t = t0 + dir * i;
+      float out[L];
 #pragma unroll
       for (int j = 0; j < L; ++j) {
-        enter[turn ^ 1][at.lane + 32 * j] = h[j];
-        if (a.last && c + 1 == a.chunks && at.ok[j])
-          a.last[at.b * a.D + at.channel(at.lane + 32 * j)] = h[j];
+        h[j] = fmaf(f[i][j], h[j], s[i][j]);
+        out[j] = kMasked && t >= at.len ? 0.f : h[j];
       }
+      if (!kMasked || t < a.T_) store_lane<true>(hp, at.ok, out);
+      hp += step;
+    }
+    turn ^= 1;
+    if (at.w == kWarps - 1)
+#pragma unroll
+      for (int j = 0; j < L; ++j) enter[turn][at.lane + 32 * j] = h[j];
+  };
+  for (int64_t c = range.v0; c < range.v1; ++c) {
+    if (at.whole(a, c * kChunk, kChunk))
+      chunk(c, Whole());
+    else
+      chunk(c, Masked());
   }
-  if (COMPOSE && tid < TILE && at.channel(tid) < a.D)
-    a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
+  if (COMPOSE) {
+    if (tid < TILE && at.channel(tid) < a.D)
+      a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
+    return;
+  }
+  clear_rest(a, at, range, a.h);
+  if (!a.last || at.segment != a.segments - 1) return;
+  compute_barrier();
+  if (tid < TILE && at.channel(tid) < a.D) a.last[at.b * a.D + at.channel(tid)] = enter[turn][tid];
 }
 
 // mu's (P, S) of every segment but the first.
@@ -644,21 +677,22 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
   unsigned char* ring = align_ring(raw);
   const Place<T, L, true> at(a);
   if (at.segment == 0) return;
-  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const Range range = range_of(a, at);
   const int tid = threadIdx.x;
   init_ring<ST>(full, empty);
   if (at.w == kWarps) {
     const CUtensorMap* const maps[2] = {&d_map, &g_map};
-    if (at.lane == 0) produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, c0, c1, true);
+    if (at.lane == 0)
+      produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, range.v0, range.v1, true);
     return;
   }
   float2 own = make_float2(1.f, 0.f);
   bool ok = true;
-  const int64_t dir = a.reverse ? -1 : 1;
-  for (int64_t c = c1 - 1; c >= c0; --c) {
-    const int it = (int)(c1 - 1 - c), slot = it % ST, turn = it & 1;
-    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
-    const bool whole = at.whole(a, c * kChunk, kChunk);
+  int turn = 0;
+  const auto chunk = [&](int64_t c, auto kind) {
+    constexpr bool kMasked = decltype(kind)::value;
+    const int it = (int)(range.v1 - 1 - c), slot = it % ST;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun), dir = a.reverse ? -1 : 1;
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
     const unsigned char* dt = ring + slot * 2 * kBox;
     float2 q[L];
@@ -668,7 +702,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     for (int i = kRun - 1; i >= 0; --i) {
       const Pack<T, L> d = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
       const Pack<T, L> g = tile_row<T, L>(dt + kBox, at.w, at.lane, i, a.reverse);
-      if (!whole && t0 + dir * i >= at.len) continue;
+      if (kMasked && t0 + dir * i >= at.len) continue;
 #pragma unroll
       for (int j = 0; j < L; ++j) {
         float f, n;
@@ -685,6 +719,13 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     if (tid < TILE)
 #pragma unroll
       for (int w = kWarps - 1; w >= 0; --w) own = then(own, part[turn][w][tid]);
+    turn ^= 1;
+  };
+  for (int64_t c = range.v1 - 1; c >= range.v0; --c) {
+    if (at.whole(a, c * kChunk, kChunk))
+      chunk(c, Whole());
+    else
+      chunk(c, Masked());
   }
   if (tid < TILE && at.channel(tid) < a.D)
     a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
@@ -704,12 +745,13 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
   __shared__ float enter[2][TILE];
   unsigned char* ring = align_ring(raw);
   const Place<T, L, true> at(a);
-  const int64_t c0 = at.segment * a.per, c1 = min(c0 + a.per, a.chunks);
+  const Range range = range_of(a, at);
   const int tid = threadIdx.x;
   init_ring<ST>(full, empty);
   if (at.w == kWarps) {
     const CUtensorMap* const maps[3] = {&x_map, &g_map, &d_map};
-    if (at.lane == 0) produce<kBox, T, 3, ST>(a, at, maps, ring, full, empty, c0, c1, true);
+    if (at.lane == 0)
+      produce<kBox, T, 3, ST>(a, at, maps, ring, full, empty, range.v0, range.v1, true);
     return;
   }
   if (tid < TILE) {
@@ -717,11 +759,12 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     enter[0][tid] = d < a.D ? enter_segment(a, at, true, d) : 0.f;
   }
   bool ok = true;
-  const int64_t dir = a.reverse ? -1 : 1;
-  for (int64_t c = c1 - 1; c >= c0; --c) {
-    const int it = (int)(c1 - 1 - c), slot = it % ST, turn = it & 1;
-    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun);
-    const bool whole = at.whole(a, c * kChunk, kChunk);
+  int turn = 0;
+  const auto chunk = [&](int64_t c, auto kind) {
+    constexpr bool kMasked = decltype(kind)::value;
+    const int it = (int)(range.v1 - 1 - c), slot = it % ST;
+    const int64_t t0 = at.time(a, c * kChunk + at.w * kRun), dir = a.reverse ? -1 : 1;
+    const auto off = [&](int i) { return kMasked && t0 + dir * i >= at.len; };
     float h[L];
 #pragma unroll
     for (int j = 0; j < L; ++j)
@@ -729,53 +772,37 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
     const unsigned char* xt = ring + slot * 3 * kBox;
     const unsigned char *gt = xt + kBox, *dt = gt + kBox;
-    // f and 1 - f of the run; masked positions have 1 and 0
-    float f[kRun][L], n[kRun][L];
+    // the factors and inputs of the run; masked positions have f = 1 and zeros
+    float f[kRun][L], n[kRun][L], x[kRun][L], d[kRun][L];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      const Pack<T, L> g = tile_row<T, L>(gt, at.w, at.lane, i, a.reverse);
-#pragma unroll
-      for (int j = 0; j < L; ++j) sigmoid_pair(to_f32(g.v[j]), f[i][j], n[i][j]);
-    }
-    const auto masked = [&](int i) { return !whole && t0 + dir * i >= at.len; };
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < kRun; ++i)
-        if (masked(i))
-#pragma unroll
-          for (int j = 0; j < L; ++j) f[i][j] = 1.f, n[i][j] = 0.f;
-    }
-    if (!ok) f[0][0] = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
-    {
-      float2 q[L];
-#pragma unroll
-      for (int j = 0; j < L; ++j) q[j] = make_float2(1.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < kRun; ++i) {
-        const Pack<T, L> x = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
-        const bool off = masked(i);
-#pragma unroll
-        for (int j = 0; j < L; ++j)
-          q[j] = then(q[j], make_float2(f[i][j], off ? 0.f : n[i][j] * to_f32(x.v[j])));
-      }
-      float m[L];
-#pragma unroll
-      for (int j = 0; j < L; ++j) m[j] = 0.f;
-#pragma unroll
-      for (int i = kRun - 1; i >= 0; --i) {
-        const Pack<T, L> d = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
-        const bool off = masked(i);
-#pragma unroll
-        for (int j = 0; j < L; ++j) m[j] = f[i][j] * ((off ? 0.f : to_f32(d.v[j])) + m[j]);
-      }
+      const Pack<T, L> gq = tile_row<T, L>(gt, at.w, at.lane, i, a.reverse);
+      const Pack<T, L> xq = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
+      const Pack<T, L> dq = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
 #pragma unroll
       for (int j = 0; j < L; ++j) {
-        part[turn][at.w][at.lane + 32 * j] = q[j];
-        mpart[turn][at.w][at.lane + 32 * j] = m[j];
+        sigmoid_pair(to_f32(gq.v[j]), f[i][j], n[i][j]);
+        x[i][j] = to_f32(xq.v[j]);
+        d[i][j] = to_f32(dq.v[j]);
+        if (off(i)) f[i][j] = 1.f, n[i][j] = x[i][j] = d[i][j] = 0.f;
       }
     }
+    __syncwarp();
+    if (at.lane == 0) barrier_arrive_here(&empty[slot]);
+    if (!ok) f[0][0] = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      float2 q = make_float2(f[0][j], n[0][j] * x[0][j]);
+#pragma unroll
+      for (int i = 1; i < kRun; ++i) q = then(q, make_float2(f[i][j], n[i][j] * x[i][j]));
+      float m = 0.f;
+#pragma unroll
+      for (int i = kRun - 1; i >= 0; --i) m = f[i][j] * (d[i][j] + m);
+      part[turn][at.w][at.lane + 32 * j] = q;
+      mpart[turn][at.w][at.lane + 32 * j] = m;
+    }
     compute_barrier();
-    float mu[L], diff[kRun][L];
+    float mu[L];
 #pragma unroll
     for (int j = 0; j < L; ++j) {
       const int at_slot = at.lane + 32 * j;
@@ -786,15 +813,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
       }
       for (int w = kWarps - 1; w > at.w; --w)
         mu[j] = fmaf(part[turn][w][at_slot].x, mu[j], mpart[turn][w][at_slot]);
-    }
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const Pack<T, L> x = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        diff[i][j] = h[j] - to_f32(x.v[j]);
-        // f h + (1 - f) x, with the product that the composition used
-        h[j] = masked(i) ? h[j] : fmaf(f[i][j], h[j], n[i][j] * to_f32(x.v[j]));
+      for (int i = 0; i < kRun; ++i) {  // x becomes h_{u-1} - x_u
+        const float before = h[j];
+        h[j] = fmaf(f[i][j], before, n[i][j] * x[i][j]);
+        x[i][j] = before - x[i][j];
       }
     }
     const int64_t last = t0 + dir * (kRun - 1);
@@ -802,33 +825,37 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     T* gp = a.dg.row(at.b, last) + at.column0();
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i) {
-      const Pack<T, L> d = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
-      const bool off = masked(i);
       float dx[L], dg[L];
 #pragma unroll
       for (int j = 0; j < L; ++j) {
-        const float lam = (off ? 0.f : to_f32(d.v[j])) + mu[j];
+        const float lam = d[i][j] + mu[j];
         mu[j] = f[i][j] * lam;
-        dx[j] = off ? 0.f : lam * n[i][j];
-        dg[j] = off ? 0.f : mu[j] * n[i][j] * diff[i][j];
+        dx[j] = off(i) ? 0.f : lam * n[i][j];
+        dg[j] = off(i) ? 0.f : mu[j] * n[i][j] * x[i][j];
       }
-      if (whole || t0 + dir * i < a.T_) {
+      if (!kMasked || t0 + dir * i < a.T_) {
         store_lane<true>(xp, at.ok, dx);
         store_lane<true>(gp, at.ok, dg);
       }
       xp -= dir * a.dx.st;
       gp -= dir * a.dg.st;
     }
-    __syncwarp();
-    if (at.lane == 0) barrier_arrive_here(&empty[slot]);
+    turn ^= 1;
     if (at.w == 0)
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        enter[turn ^ 1][at.lane + 32 * j] = mu[j];
-        if (a.last && c == 0 && at.ok[j])
-          a.last[at.b * a.D + at.channel(at.lane + 32 * j)] = mu[j];
-      }
+      for (int j = 0; j < L; ++j) enter[turn][at.lane + 32 * j] = mu[j];
+  };
+  for (int64_t c = range.v1 - 1; c >= range.v0; --c) {
+    if (at.whole(a, c * kChunk, kChunk))
+      chunk(c, Whole());
+    else
+      chunk(c, Masked());
   }
+  clear_rest(a, at, range, a.dx);
+  clear_rest(a, at, range, a.dg);
+  if (!a.last || at.segment != 0) return;
+  compute_barrier();
+  if (tid < TILE && at.channel(tid) < a.D) a.last[at.b * a.D + at.channel(tid)] = enter[turn][tid];
 }
 
 int64_t chunks_of(int64_t T) { return (T + kChunk - 1) / kChunk; }
