@@ -112,6 +112,52 @@ __device__ __forceinline__ void sigmoid_pair(float g, float& pos, float& neg) {
   neg = e * pos;
 }
 
+// Two channels at once: products and sums go two to an instruction.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  return __ffma2_rn(b, make_float2(-1.f, -1.f), a);  // exactly a - b rounded once
+}
+__device__ __forceinline__ void sigmoid_pair2(float2 g, float2& pos, float2& neg) {
+  const float2 t = __fmul2_rn(g, both(-1.4426950408889634f));
+  float2 e;
+  asm("{.reg .f32 t; min.NaN.f32 t, %1, 0f42FC0000; ex2.approx.ftz.f32 %0, t;}"
+      : "=f"(e.x)
+      : "f"(t.x));
+  asm("{.reg .f32 t; min.NaN.f32 t, %1, 0f42FC0000; ex2.approx.ftz.f32 %0, t;}"
+      : "=f"(e.y)
+      : "f"(t.y));
+  const float2 d = __fadd2_rn(e, both(1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos.y) : "f"(d.y));
+  neg = __fmul2_rn(e, pos);
+}
+template <class T>
+__device__ __forceinline__ float2 to_f32x2(const Pack<T, 2>& v) {
+  return make_float2(to_f32(v.v[0]), to_f32(v.v[1]));
+}
+template <>
+__device__ __forceinline__ float2 to_f32x2(const Pack<__half, 2>& v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <class T>
+__device__ __forceinline__ Pack<T, 2> from_f32x2(float2 v);
+template <>
+__device__ __forceinline__ Pack<float, 2> from_f32x2<float>(float2 v) {
+  Pack<float, 2> q;
+  q.v[0] = v.x, q.v[1] = v.y;
+  return q;
+}
+template <>
+__device__ __forceinline__ Pack<__nv_bfloat16, 2> from_f32x2<__nv_bfloat16>(float2 v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const Pack<__nv_bfloat16, 2>*>(&h);
+}
+template <>
+__device__ __forceinline__ Pack<__half, 2> from_f32x2<__half>(float2 v) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const Pack<__half, 2>*>(&h);
+}
+
 // ---------------------------------------------------------------------------
 // 8-bit checkpoints: 32 channels of a position share the scale 2^e, e + 127 in
 // a byte.  A power of two costs up to one bit against a free scale, and makes

@@ -447,27 +447,53 @@ __global__ void step_kernel(int64_t B, int64_t D, const T* __restrict__ x, int64
 // The walk with its inputs brought by bulk copies: rows on 16-byte boundaries.
 // A producer thread keeps a ring of chunks of every input on their way to
 // shared memory; rows there lie at fixed offsets, so reading them costs no
-// address arithmetic, and nothing waits in registers.  A lane takes 8 bytes of
-// a row forward, 4 backward (three inputs and both factors fill the registers).
+// address arithmetic, and nothing waits in registers.  A lane takes H pairs of
+// channels: two of 16-bit types forward, one else (the run's factors and, in
+// the backward, its inputs fill the registers).  Products and sums go two
+// channels to an instruction: issue slots are what comes next after DRAM.
 // ---------------------------------------------------------------------------
-constexpr int kForwardLane = 8, kBackwardLane = 4;      // bytes
-constexpr int kForwardStages = 3, kBackwardStages = 3;  // chunks in the ring
-constexpr int box_bytes(int lane) { return 32 * lane * kChunk; }
-constexpr int ring_bytes(int lane, int tensors, int stages) {
-  return tensors * stages * box_bytes(lane) + 128;
+template <class T>
+constexpr int forward_pairs() { return sizeof(T) == 2 ? 2 : 1; }
+constexpr int kBackwardPairs = 1;
+constexpr int box_bytes(int elem, int pairs) { return 64 * elem * pairs * kChunk; }
+// chunks in the ring: what lets two CTAs share an SM
+constexpr int kForwardStages = 3;
+template <class T>
+constexpr int backward_stages() { return sizeof(T) == 2 ? 3 : 2; }
+constexpr int ring_bytes(int elem, int pairs, int tensors, int stages) {
+  return tensors * stages * box_bytes(elem, pairs) + 128;
 }
 
 __device__ __forceinline__ void compute_barrier() {
   asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
 }
 
-// A lane's part of row i of a warp's run, in scan order, in a tile in shared memory.
-template <class T, int L>
-__device__ __forceinline__ Pack<T, L> tile_row(const unsigned char* tile, int w, int lane, int i,
-                                               bool reverse) {
-  constexpr int kBytes = (int)sizeof(T) * L;
+// A lane's pairs of row i of a warp's run, in scan order, in a tile in shared memory.
+template <class T, int H>
+__device__ __forceinline__ void tile_row(const unsigned char* tile, int w, int lane, int i,
+                                         bool reverse, float2 (&v)[H]) {
+  constexpr int kBytes = 2 * H * (int)sizeof(T);
   const int row = reverse ? kChunk - 1 - (w * kRun + i) : w * kRun + i;
-  return *reinterpret_cast<const Pack<T, L>*>(tile + (row * 32 + lane) * kBytes);
+  const Pack<Pack<T, 2>, H> q =
+      *reinterpret_cast<const Pack<Pack<T, 2>, H>*>(tile + (row * 32 + lane) * kBytes);
+#pragma unroll
+  for (int j = 0; j < H; ++j) v[j] = to_f32x2(q.v[j]);
+}
+template <class T, int H>
+__device__ __forceinline__ void store_pairs(T* p, bool ok, const float2 (&v)[H]) {
+  if (!ok) return;
+  Pack<Pack<T, 2>, H> q;
+#pragma unroll
+  for (int j = 0; j < H; ++j) q.v[j] = from_f32x2<T>(v[j]);
+  *reinterpret_cast<Pack<Pack<T, 2>, H>*>(p) = q;
+}
+
+// (P, S) of two channels
+struct Affine {
+  float2 P, S;
+};
+__device__ __forceinline__ Affine then(const Affine& a, const Affine& b) {  // b after a
+  return Affine{__fmul2_rn(b.P, a.P), __ffma2_rn(b.P, a.S, b.S)};
 }
 
 // Keeps the ring full: N tensors a chunk, `descending` in scan order for the backward.
@@ -516,8 +542,8 @@ struct Range {
   int64_t c0, c1;  // the segment's chunks
   int64_t v0, v1;  // those with valid positions
 };
-template <class T, int L>
-__device__ __forceinline__ Range range_of(const ScanArgs<T>& a, const Place<T, L, true>& at) {
+template <class T, class At>
+__device__ __forceinline__ Range range_of(const ScanArgs<T>& a, const At& at) {
   Range r;
   r.c0 = at.segment * a.per;
   r.c1 = min(r.c0 + a.per, a.chunks);
@@ -528,19 +554,29 @@ __device__ __forceinline__ Range range_of(const ScanArgs<T>& a, const Place<T, L
   return r;
 }
 // Zeros in every row of the segment's other chunks, by the CTA's first 256 threads.
-template <class T, int L>
-__device__ void clear_rest(const ScanArgs<T>& a, const Place<T, L, true>& at, const Range& r,
-                           const Seq<T>& out) {
+template <int H, class T, class At>
+__device__ void clear_rest(const ScanArgs<T>& a, const At& at, const Range& r, const Seq<T>& out) {
   const int64_t rest = (r.c1 - r.c0) - (r.v1 - r.v0);
-  const float zero[L] = {};
+  const float2 zero[H] = {};
   for (int64_t k = 0; k < rest; ++k) {
     const int64_t c = a.reverse ? r.c0 + k : r.v1 + k;
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
       const int64_t t = at.time(a, c * kChunk + at.w * kRun + i);
-      if (t < a.T_) store_lane<true>(out.row(at.b, t) + at.column0(), at.ok, zero);
+      if (t < a.T_) store_pairs(out.row(at.b, t) + at.column0(), at.ok[0], zero);
     }
   }
+}
+// First channel of pair number k = lane + 32 j of a tile.
+template <int H>
+__device__ __forceinline__ int pair_channel(int k) { return (k & 31) * 2 * H + 2 * (k >> 5); }
+
+// The state entering the segment, of the pair of channels that thread tid < 32 H looks after.
+template <int H, class T, class At>
+__device__ __forceinline__ float2 enter_pair(const ScanArgs<T>& a, const At& at, bool descending) {
+  const int64_t d = at.d0 + pair_channel<H>(threadIdx.x);
+  if (d >= a.D) return both(0.f);
+  return make_float2(enter_segment(a, at, descending, d), enter_segment(a, at, descending, d + 1));
 }
 
 struct Masked { static constexpr bool value = true; };
@@ -551,15 +587,15 @@ template <class T, bool COMPOSE>
 __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     forward_bulk_kernel(const ScanArgs<T> a, const __grid_constant__ CUtensorMap x_map,
                         const __grid_constant__ CUtensorMap g_map) {
-  constexpr int L = kForwardLane / (int)sizeof(T), TILE = 32 * L, ST = kForwardStages;
-  constexpr int kBox = box_bytes(kForwardLane);
+  constexpr int H = forward_pairs<T>(), PAIRS = 32 * H, ST = kForwardStages;
+  constexpr int kBox = box_bytes(sizeof(T), H);
   constexpr int kParts = COMPOSE ? kWarps : kWarps - 1;  // the last warp's has no reader in a walk
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[ST], empty[ST];
-  __shared__ float2 part[2][kParts][TILE];
-  __shared__ float enter[2][COMPOSE ? 1 : TILE];
+  __shared__ Affine part[2][kParts][PAIRS];
+  __shared__ float2 enter[2][COMPOSE ? 1 : PAIRS];
   unsigned char* ring = align_ring(raw);
-  const Place<T, L, true> at(a);
+  const Place<T, 2 * H, true> at(a);
   if (COMPOSE && at.segment == a.segments - 1) return;
   const Range range = range_of(a, at);
   const int tid = threadIdx.x;
@@ -570,11 +606,8 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
       produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, range.v0, range.v1, false);
     return;
   }
-  float2 own = make_float2(1.f, 0.f);
-  if (!COMPOSE && tid < TILE) {
-    const int64_t d = at.channel(tid);
-    enter[0][tid] = d < a.D ? enter_segment(a, at, false, d) : 0.f;
-  }
+  Affine own{both(1.f), both(0.f)};
+  if (!COMPOSE && tid < PAIRS) enter[0][tid] = enter_pair<H>(a, at, false);
   bool ok = true;
   const int64_t step = a.reverse ? -a.h.st : a.h.st;
   int turn = 0;
@@ -584,68 +617,70 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     const int64_t t0 = at.time(a, c * kChunk + at.w * kRun), dir = a.reverse ? -1 : 1;
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
     const unsigned char* xt = ring + slot * 2 * kBox;
-    float f[kRun][L], s[kRun][L];
+    Affine u[kRun][H];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      const Pack<T, L> x = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
-      const Pack<T, L> g = tile_row<T, L>(xt + kBox, at.w, at.lane, i, a.reverse);
+      float2 x[H], g[H];
+      tile_row<T>(xt, at.w, at.lane, i, a.reverse, x);
+      tile_row<T>(xt + kBox, at.w, at.lane, i, a.reverse, g);
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        float n;
-        sigmoid_pair(to_f32(g.v[j]), f[i][j], n);
-        s[i][j] = n * to_f32(x.v[j]);
-        if (kMasked && t0 + dir * i >= at.len) f[i][j] = 1.f, s[i][j] = 0.f;
+      for (int j = 0; j < H; ++j) {
+        float2 n;
+        sigmoid_pair2(g[j], u[i][j].P, n);
+        u[i][j].S = __fmul2_rn(n, x[j]);
+        if (kMasked && t0 + dir * i >= at.len) u[i][j] = Affine{both(1.f), both(0.f)};
       }
     }
     __syncwarp();
     if (at.lane == 0) barrier_arrive_here(&empty[slot]);
-    if (!ok) f[0][0] = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+    if (!ok) u[0][0].P.x = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
     if (COMPOSE || at.w < kParts)
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        float2 q = make_float2(f[0][j], s[0][j]);
+      for (int j = 0; j < H; ++j) {
+        Affine q = u[0][j];
 #pragma unroll
-        for (int i = 1; i < kRun; ++i) q = then(q, make_float2(f[i][j], s[i][j]));
+        for (int i = 1; i < kRun; ++i) q = then(q, u[i][j]);
         part[turn][at.w][at.lane + 32 * j] = q;
       }
     compute_barrier();
     if (COMPOSE) {
-      if (tid < TILE)
+      if (tid < PAIRS)
 #pragma unroll
         for (int w = 0; w < kParts; ++w) own = then(own, part[turn][w][tid]);
       turn ^= 1;
       return;
     }
-    float h[L];
+    float2 h[H];
 #pragma unroll
-    for (int j = 0; j < L; ++j) h[j] = enter[turn][at.lane + 32 * j];
-    if (a.carry && at.w == 0)
+    for (int j = 0; j < H; ++j) h[j] = enter[turn][at.lane + 32 * j];
+    if (a.carry && at.w == 0 && at.ok[0]) {
+      float* p = a.carry + (at.b * a.chunks + c) * a.D + at.column0();
 #pragma unroll
-      for (int j = 0; j < L; ++j)
-        if (at.ok[j]) a.carry[(at.b * a.chunks + c) * a.D + at.channel(at.lane + 32 * j)] = h[j];
+      for (int j = 0; j < H; ++j) p[2 * j] = h[j].x, p[2 * j + 1] = h[j].y;
+    }
     for (int w = 0; w < at.w; ++w)
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        const float2 q = part[turn][w][at.lane + 32 * j];
-        h[j] = fmaf(q.x, h[j], q.y);
+      for (int j = 0; j < H; ++j) {
+        const Affine q = part[turn][w][at.lane + 32 * j];
+        h[j] = __ffma2_rn(q.P, h[j], q.S);
       }
     T* hp = a.h.row(at.b, t0) + at.column0();
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
       const int64_t t = t0 + dir * i;
-      float out[L];
+      float2 out[H];
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        h[j] = fmaf(f[i][j], h[j], s[i][j]);
-        out[j] = kMasked && t >= at.len ? 0.f : h[j];
+      for (int j = 0; j < H; ++j) {
+        h[j] = __ffma2_rn(u[i][j].P, h[j], u[i][j].S);
+        out[j] = kMasked && t >= at.len ? both(0.f) : h[j];
       }
-      if (!kMasked || t < a.T_) store_lane<true>(hp, at.ok, out);
+      if (!kMasked || t < a.T_) store_pairs(hp, at.ok[0], out);
       hp += step;
     }
     turn ^= 1;
     if (at.w == kWarps - 1)
 #pragma unroll
-      for (int j = 0; j < L; ++j) enter[turn][at.lane + 32 * j] = h[j];
+      for (int j = 0; j < H; ++j) enter[turn][at.lane + 32 * j] = h[j];
   };
   for (int64_t c = range.v0; c < range.v1; ++c) {
     if (at.whole(a, c * kChunk, kChunk))
@@ -653,15 +688,22 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     else
       chunk(c, Masked());
   }
+  const int64_t d = at.d0 + pair_channel<H>(tid);
   if (COMPOSE) {
-    if (tid < TILE && at.channel(tid) < a.D)
-      a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
+    if (tid < PAIRS && d < a.D) {
+      float2* p = a.composed + (at.b * a.segments + at.segment) * a.D + d;
+      p[0] = make_float2(own.P.x, own.S.x);
+      p[1] = make_float2(own.P.y, own.S.y);
+    }
     return;
   }
-  clear_rest(a, at, range, a.h);
+  clear_rest<H>(a, at, range, a.h);
   if (!a.last || at.segment != a.segments - 1) return;
   compute_barrier();
-  if (tid < TILE && at.channel(tid) < a.D) a.last[at.b * a.D + at.channel(tid)] = enter[turn][tid];
+  if (tid < PAIRS && d < a.D) {
+    a.last[at.b * a.D + d] = enter[turn][tid].x;
+    a.last[at.b * a.D + d + 1] = enter[turn][tid].y;
+  }
 }
 
 // mu's (P, S) of every segment but the first.
@@ -669,13 +711,13 @@ template <class T>
 __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     backward_compose_kernel(const ScanArgs<T> a, const __grid_constant__ CUtensorMap d_map,
                             const __grid_constant__ CUtensorMap g_map) {
-  constexpr int L = kBackwardLane / (int)sizeof(T), TILE = 32 * L, ST = kBackwardStages;
-  constexpr int kBox = box_bytes(kBackwardLane);
+  constexpr int H = kBackwardPairs, PAIRS = 32 * H, ST = backward_stages<T>();
+  constexpr int kBox = box_bytes(sizeof(T), H);
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[ST], empty[ST];
-  __shared__ float2 part[2][kWarps][TILE];
+  __shared__ Affine part[2][kWarps][PAIRS];
   unsigned char* ring = align_ring(raw);
-  const Place<T, L, true> at(a);
+  const Place<T, 2 * H, true> at(a);
   if (at.segment == 0) return;
   const Range range = range_of(a, at);
   const int tid = threadIdx.x;
@@ -686,7 +728,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
       produce<kBox, T, 2, ST>(a, at, maps, ring, full, empty, range.v0, range.v1, true);
     return;
   }
-  float2 own = make_float2(1.f, 0.f);
+  Affine own{both(1.f), both(0.f)};
   bool ok = true;
   int turn = 0;
   const auto chunk = [&](int64_t c, auto kind) {
@@ -695,28 +737,30 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     const int64_t t0 = at.time(a, c * kChunk + at.w * kRun), dir = a.reverse ? -1 : 1;
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
     const unsigned char* dt = ring + slot * 2 * kBox;
-    float2 q[L];
+    Affine q[H];
 #pragma unroll
-    for (int j = 0; j < L; ++j) q[j] = make_float2(ok ? 1.f : __uint_as_float(0x7fc00000u), 0.f);
+    for (int j = 0; j < H; ++j)
+      q[j] = Affine{both(ok ? 1.f : __uint_as_float(0x7fc00000u)), both(0.f)};
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i) {
-      const Pack<T, L> d = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
-      const Pack<T, L> g = tile_row<T, L>(dt + kBox, at.w, at.lane, i, a.reverse);
+      float2 d[H], g[H];
+      tile_row<T>(dt, at.w, at.lane, i, a.reverse, d);
+      tile_row<T>(dt + kBox, at.w, at.lane, i, a.reverse, g);
       if (kMasked && t0 + dir * i >= at.len) continue;
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        float f, n;
-        sigmoid_pair(to_f32(g.v[j]), f, n);
-        q[j].x *= f;
-        q[j].y = f * (to_f32(d.v[j]) + q[j].y);
+      for (int j = 0; j < H; ++j) {
+        float2 f, n;
+        sigmoid_pair2(g[j], f, n);
+        q[j].P = __fmul2_rn(q[j].P, f);
+        q[j].S = __fmul2_rn(f, __fadd2_rn(d[j], q[j].S));
       }
     }
     __syncwarp();
     if (at.lane == 0) barrier_arrive_here(&empty[slot]);
 #pragma unroll
-    for (int j = 0; j < L; ++j) part[turn][at.w][at.lane + 32 * j] = q[j];
+    for (int j = 0; j < H; ++j) part[turn][at.w][at.lane + 32 * j] = q[j];
     compute_barrier();
-    if (tid < TILE)
+    if (tid < PAIRS)
 #pragma unroll
       for (int w = kWarps - 1; w >= 0; --w) own = then(own, part[turn][w][tid]);
     turn ^= 1;
@@ -727,8 +771,12 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     else
       chunk(c, Masked());
   }
-  if (tid < TILE && at.channel(tid) < a.D)
-    a.composed[(at.b * a.segments + at.segment) * a.D + at.channel(tid)] = own;
+  const int64_t d = at.d0 + pair_channel<H>(tid);
+  if (tid < PAIRS && d < a.D) {
+    float2* p = a.composed + (at.b * a.segments + at.segment) * a.D + d;
+    p[0] = make_float2(own.P.x, own.S.x);
+    p[1] = make_float2(own.P.y, own.S.y);
+  }
 }
 
 template <class T>
@@ -736,15 +784,15 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     backward_bulk_kernel(const ScanArgs<T> a, const __grid_constant__ CUtensorMap x_map,
                          const __grid_constant__ CUtensorMap g_map,
                          const __grid_constant__ CUtensorMap d_map) {
-  constexpr int L = kBackwardLane / (int)sizeof(T), TILE = 32 * L, ST = kBackwardStages;
-  constexpr int kBox = box_bytes(kBackwardLane);
+  constexpr int H = kBackwardPairs, PAIRS = 32 * H, ST = backward_stages<T>();
+  constexpr int kBox = box_bytes(sizeof(T), H);
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[ST], empty[ST];
-  __shared__ float2 part[2][kWarps][TILE];
-  __shared__ float mpart[2][kWarps][TILE];
-  __shared__ float enter[2][TILE];
+  __shared__ Affine part[2][kWarps][PAIRS];
+  __shared__ float2 mpart[2][kWarps][PAIRS];
+  __shared__ float2 enter[2][PAIRS];
   unsigned char* ring = align_ring(raw);
-  const Place<T, L, true> at(a);
+  const Place<T, 2 * H, true> at(a);
   const Range range = range_of(a, at);
   const int tid = threadIdx.x;
   init_ring<ST>(full, empty);
@@ -754,10 +802,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
       produce<kBox, T, 3, ST>(a, at, maps, ring, full, empty, range.v0, range.v1, true);
     return;
   }
-  if (tid < TILE) {
-    const int64_t d = at.channel(tid);
-    enter[0][tid] = d < a.D ? enter_segment(a, at, true, d) : 0.f;
-  }
+  if (tid < PAIRS) enter[0][tid] = enter_pair<H>(a, at, true);
   bool ok = true;
   int turn = 0;
   const auto chunk = [&](int64_t c, auto kind) {
@@ -765,59 +810,60 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     const int it = (int)(range.v1 - 1 - c), slot = it % ST;
     const int64_t t0 = at.time(a, c * kChunk + at.w * kRun), dir = a.reverse ? -1 : 1;
     const auto off = [&](int i) { return kMasked && t0 + dir * i >= at.len; };
-    float h[L];
+    float2 h[H] = {};
+    if (at.ok[0]) {
+      const float* p = a.carry + (at.b * a.chunks + c) * a.D + at.column0();
 #pragma unroll
-    for (int j = 0; j < L; ++j)
-      h[j] = at.ok[j] ? a.carry[(at.b * a.chunks + c) * a.D + at.channel(at.lane + 32 * j)] : 0.f;
+      for (int j = 0; j < H; ++j) h[j] = make_float2(p[2 * j], p[2 * j + 1]);
+    }
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / ST) & 1);
     const unsigned char* xt = ring + slot * 3 * kBox;
     const unsigned char *gt = xt + kBox, *dt = gt + kBox;
     // the factors and inputs of the run; masked positions have f = 1 and zeros
-    float f[kRun][L], n[kRun][L], x[kRun][L], d[kRun][L];
+    float2 f[kRun][H], n[kRun][H], x[kRun][H], d[kRun][H];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      const Pack<T, L> gq = tile_row<T, L>(gt, at.w, at.lane, i, a.reverse);
-      const Pack<T, L> xq = tile_row<T, L>(xt, at.w, at.lane, i, a.reverse);
-      const Pack<T, L> dq = tile_row<T, L>(dt, at.w, at.lane, i, a.reverse);
+      float2 g[H];
+      tile_row<T>(gt, at.w, at.lane, i, a.reverse, g);
+      tile_row<T>(xt, at.w, at.lane, i, a.reverse, x[i]);
+      tile_row<T>(dt, at.w, at.lane, i, a.reverse, d[i]);
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        sigmoid_pair(to_f32(gq.v[j]), f[i][j], n[i][j]);
-        x[i][j] = to_f32(xq.v[j]);
-        d[i][j] = to_f32(dq.v[j]);
-        if (off(i)) f[i][j] = 1.f, n[i][j] = x[i][j] = d[i][j] = 0.f;
+      for (int j = 0; j < H; ++j) {
+        sigmoid_pair2(g[j], f[i][j], n[i][j]);
+        if (off(i)) f[i][j] = both(1.f), n[i][j] = x[i][j] = d[i][j] = both(0.f);
       }
     }
     __syncwarp();
     if (at.lane == 0) barrier_arrive_here(&empty[slot]);
-    if (!ok) f[0][0] = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+    if (!ok) f[0][0].x = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      float2 q = make_float2(f[0][j], n[0][j] * x[0][j]);
+    for (int j = 0; j < H; ++j) {
+      Affine q{f[0][j], __fmul2_rn(n[0][j], x[0][j])};
 #pragma unroll
-      for (int i = 1; i < kRun; ++i) q = then(q, make_float2(f[i][j], n[i][j] * x[i][j]));
-      float m = 0.f;
+      for (int i = 1; i < kRun; ++i) q = then(q, Affine{f[i][j], __fmul2_rn(n[i][j], x[i][j])});
+      float2 m = both(0.f);
 #pragma unroll
-      for (int i = kRun - 1; i >= 0; --i) m = f[i][j] * (d[i][j] + m);
+      for (int i = kRun - 1; i >= 0; --i) m = __fmul2_rn(f[i][j], __fadd2_rn(d[i][j], m));
       part[turn][at.w][at.lane + 32 * j] = q;
       mpart[turn][at.w][at.lane + 32 * j] = m;
     }
     compute_barrier();
-    float mu[L];
+    float2 mu[H];
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
+    for (int j = 0; j < H; ++j) {
       const int at_slot = at.lane + 32 * j;
       mu[j] = enter[turn][at_slot];
       for (int w = 0; w < at.w; ++w) {
-        const float2 q = part[turn][w][at_slot];
-        h[j] = fmaf(q.x, h[j], q.y);
+        const Affine q = part[turn][w][at_slot];
+        h[j] = __ffma2_rn(q.P, h[j], q.S);
       }
       for (int w = kWarps - 1; w > at.w; --w)
-        mu[j] = fmaf(part[turn][w][at_slot].x, mu[j], mpart[turn][w][at_slot]);
+        mu[j] = __ffma2_rn(part[turn][w][at_slot].P, mu[j], mpart[turn][w][at_slot]);
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) {  // x becomes h_{u-1} - x_u
-        const float before = h[j];
-        h[j] = fmaf(f[i][j], before, n[i][j] * x[i][j]);
-        x[i][j] = before - x[i][j];
+      for (int i = 0; i < kRun; ++i) {  // x becomes (1 - f) (h_{u-1} - x_u)
+        const float2 before = h[j];
+        h[j] = __ffma2_rn(f[i][j], before, __fmul2_rn(n[i][j], x[i][j]));
+        x[i][j] = __fmul2_rn(n[i][j], sub2(before, x[i][j]));
       }
     }
     const int64_t last = t0 + dir * (kRun - 1);
@@ -825,17 +871,17 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     T* gp = a.dg.row(at.b, last) + at.column0();
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i) {
-      float dx[L], dg[L];
+      float2 dx[H], dg[H];
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        const float lam = d[i][j] + mu[j];
-        mu[j] = f[i][j] * lam;
-        dx[j] = off(i) ? 0.f : lam * n[i][j];
-        dg[j] = off(i) ? 0.f : mu[j] * n[i][j] * x[i][j];
+      for (int j = 0; j < H; ++j) {
+        const float2 lam = __fadd2_rn(d[i][j], mu[j]);
+        mu[j] = __fmul2_rn(f[i][j], lam);
+        dx[j] = off(i) ? both(0.f) : __fmul2_rn(lam, n[i][j]);
+        dg[j] = off(i) ? both(0.f) : __fmul2_rn(mu[j], x[i][j]);
       }
       if (!kMasked || t0 + dir * i < a.T_) {
-        store_lane<true>(xp, at.ok, dx);
-        store_lane<true>(gp, at.ok, dg);
+        store_pairs(xp, at.ok[0], dx);
+        store_pairs(gp, at.ok[0], dg);
       }
       xp -= dir * a.dx.st;
       gp -= dir * a.dg.st;
@@ -843,7 +889,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     turn ^= 1;
     if (at.w == 0)
 #pragma unroll
-      for (int j = 0; j < L; ++j) enter[turn][at.lane + 32 * j] = mu[j];
+      for (int j = 0; j < H; ++j) enter[turn][at.lane + 32 * j] = mu[j];
   };
   for (int64_t c = range.v1 - 1; c >= range.v0; --c) {
     if (at.whole(a, c * kChunk, kChunk))
@@ -851,19 +897,24 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
     else
       chunk(c, Masked());
   }
-  clear_rest(a, at, range, a.dx);
-  clear_rest(a, at, range, a.dg);
+  clear_rest<H>(a, at, range, a.dx);
+  clear_rest<H>(a, at, range, a.dg);
   if (!a.last || at.segment != 0) return;
   compute_barrier();
-  if (tid < TILE && at.channel(tid) < a.D) a.last[at.b * a.D + at.channel(tid)] = enter[turn][tid];
+  const int64_t d = at.d0 + pair_channel<H>(tid);
+  if (tid < PAIRS && d < a.D) {
+    a.last[at.b * a.D + d] = enter[turn][tid].x;
+    a.last[at.b * a.D + d + 1] = enter[turn][tid].y;
+  }
 }
 
 int64_t chunks_of(int64_t T) { return (T + kChunk - 1) / kChunk; }
 
+// Channels of a lane where rows are read by plain loads.
 template <class T>
-constexpr int forward_lane() { return kForwardLane / (int)sizeof(T); }
+constexpr int forward_lane() { return 2 * forward_pairs<T>(); }
 template <class T>
-constexpr int backward_lane() { return kBackwardLane / (int)sizeof(T); }
+constexpr int backward_lane() { return sizeof(T) == 2 ? 2 : 1; }
 
 struct Cut {
   int tiles, segments;
@@ -965,7 +1016,7 @@ int run_forward(const semicrf_recurrence* p, const semicrf_sequence& h, float* f
     CUtensorMap xm, gm;
     const auto walk = forward_bulk_kernel<T, false>;
     const auto compose = forward_bulk_kernel<T, true>;
-    constexpr int bytes = ring_bytes(kForwardLane, 2, kForwardStages);
+    constexpr int bytes = ring_bytes(sizeof(T), forward_pairs<T>(), 2, kForwardStages);
     if (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, L) ||
         !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, L) || !allow_shared(walk, bytes) ||
         !allow_shared(compose, bytes))
@@ -984,28 +1035,30 @@ int run_backward(const semicrf_recurrence* p, const void* saved, const semicrf_s
                  const semicrf_sequence& grad_gate, float* grad_initial, void* workspace,
                  cudaStream_t stream) {
   if (p->T == 0) return copy_state(p, grad_state, grad_initial, stream);
-  constexpr int L = backward_lane<T>();
-  ScanArgs<T> a = scan_args<T>(p, 32 * L, workspace);
+  constexpr int L = backward_lane<T>(), BL = 2 * kBackwardPairs;
+  bool vec = p->D % L == 0, bulk = p->D % BL == 0;
+  for (const semicrf_sequence* s : {&p->x, &p->gate, &grad_h, &grad_x, &grad_gate}) {
+    vec = vec && seq_aligned(*s, p->batch, p->T, sizeof(T), L);
+    bulk = bulk && seq_aligned(*s, p->batch, p->T, sizeof(T), BL);
+  }
+  for (const semicrf_sequence* s : {&p->x, &p->gate, &grad_h})
+    bulk = bulk && bulk_readable(*s, p->batch, p->T, p->D, sizeof(T));
+  ScanArgs<T> a = scan_args<T>(p, 32 * (bulk ? BL : L), workspace);
   a.dh = as_seq<const T>(grad_h);
   a.dx = as_seq<T>(grad_x);
   a.dg = as_seq<T>(grad_gate);
   a.first = grad_state;
   a.last = grad_initial;
   a.carry = const_cast<float*>(static_cast<const float*>(saved));
-  bool vec = p->D % L == 0;
-  for (const semicrf_sequence* s : {&p->x, &p->gate, &grad_h, &grad_x, &grad_gate})
-    vec = vec && seq_aligned(*s, a.B, a.T_, sizeof(T), L);
-  if (vec && bulk_readable(p->x, a.B, a.T_, a.D, sizeof(T)) &&
-      bulk_readable(p->gate, a.B, a.T_, a.D, sizeof(T)) &&
-      bulk_readable(grad_h, a.B, a.T_, a.D, sizeof(T))) {
+  if (bulk) {
     CUtensorMap xm, gm, dm;
     const auto walk = backward_bulk_kernel<T>;
     const auto compose = backward_compose_kernel<T>;
-    constexpr int walk_bytes = ring_bytes(kBackwardLane, 3, kBackwardStages);
-    constexpr int compose_bytes = ring_bytes(kBackwardLane, 2, kBackwardStages);
-    if (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, L) ||
-        !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, L) ||
-        !sequence_map<T>(&dm, grad_h, a.B, a.T_, a.D, L) || !allow_shared(walk, walk_bytes) ||
+    constexpr int walk_bytes = ring_bytes(sizeof(T), kBackwardPairs, 3, backward_stages<T>());
+    constexpr int compose_bytes = ring_bytes(sizeof(T), kBackwardPairs, 2, backward_stages<T>());
+    if (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, BL) ||
+        !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, BL) ||
+        !sequence_map<T>(&dm, grad_h, a.B, a.T_, a.D, BL) || !allow_shared(walk, walk_bytes) ||
         !allow_shared(compose, compose_bytes))
       return SEMICRF_ERR_CUDA;
     const unsigned grid = (unsigned)(a.B * a.tiles * a.segments);
@@ -1046,8 +1099,9 @@ size_t recurrence_saved_bytes(const semicrf_recurrence* p) {
 }
 size_t recurrence_workspace_bytes(const semicrf_recurrence* p) {
   const bool wide = p->dtype == SEMICRF_F32;
-  const int tiles[2] = {32 * (wide ? forward_lane<float>() : forward_lane<__half>()),
-                        32 * (wide ? backward_lane<float>() : backward_lane<__half>())};
+  const int tiles[3] = {32 * (wide ? forward_lane<float>() : forward_lane<__half>()),
+                        32 * (wide ? backward_lane<float>() : backward_lane<__half>()),
+                        64 * kBackwardPairs};
   int segments = 1;
   for (const int tile : tiles)
     segments = std::max(segments, cut_of(p->batch, p->T, p->D, tile).segments);
