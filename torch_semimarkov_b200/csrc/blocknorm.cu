@@ -9,11 +9,16 @@
 //   dz = (db w1 - zh sum(db w1 zh) / D) / rms(z)
 //   dw1 = sum_rows db zh,  ds = sum_rows d silu(g) b,  dw2 = sum_rows dn rh
 //
+// dw1 and ds share their sum over rows: A = sum d silu(g) zh gives dw1 = s A
+// and ds = w1 A, so two sums a channel are carried, and w1 and s enter the rows
+// only as their product.
+//
 // A row lies in the registers of WR warps, PER channels to a lane, so each
 // input is read once.  The backward recomputes r from the block's inputs in
 // 32 bits; it reads x where it would else read the rounded r.  Weight
 // gradients are summed per thread over the rows that its CTA walks, then over
-// the CTAs in a fixed order: no atomics.
+// the CTAs in a fixed order: no atomics.  Products and sums go two channels to
+// an instruction.
 
 #include <algorithm>
 
@@ -26,7 +31,8 @@ namespace {
 
 template <class T>
 struct NormArgs {
-  int64_t rows, T_, D;
+  int64_t rows, D;
+  Places places;
   float eps, inv_d;
   Seq<const T> x, z, g;
   Seq<T> r, n;
@@ -37,7 +43,7 @@ struct NormArgs {
   uint8_t* scales;
   Seq<const T> dr, dn;
   Seq<T> dx, dz, dg;
-  float* partial;  // (grid, 3, D)
+  float* partial;  // (grid, 2, D): A and the sum of dn rh
 };
 
 // Sums over the row's lanes; every lane gets the result.  `red` alternates
@@ -61,275 +67,310 @@ struct RowSum {
   }
 };
 
-template <class T, int V, int WR, int PER>
+// PER channels to a lane in vectors of V, WR warps to a row.
+template <class T, int V_, int WR_, int PER_>
 struct Layout {
-  static constexpr int J = PER / V;                      // vectors of a lane
-  static constexpr int kRows = WR >= 4 ? 1 : 4 / WR;     // rows that a CTA works on at once
-  static constexpr int kThreads = 32 * WR * kRows;
+  static constexpr int V = V_, WR = WR_, PER = PER_;
+  static constexpr int J = PER / V;                   // vectors of a lane
+  static constexpr int H = PER / 2;                   // pairs of a lane
+  static constexpr int NL = 32 * WR;                  // lanes of a row
+  static constexpr int kRows = WR >= 4 ? 1 : 4 / WR;  // rows that a CTA works on at once
+  static constexpr int kThreads = NL * kRows;
+  // channel of vector j of lane l
+  __device__ static __forceinline__ int channel(int j, int l) { return (j * NL + l) * V; }
+  // channel of half k of pair i of lane l
+  __device__ static __forceinline__ int channel_of(int i, int k, int l) {
+    const int e = 2 * i + k;
+    return channel(e / V, l) + e % V;
+  }
 };
 
-template <class T, int V>
-__device__ __forceinline__ void get(const T* row, int64_t d, bool ok, float (&v)[V]) {
-  Pack<T, V> q;
-  if (ok) q = *reinterpret_cast<const Pack<T, V>*>(row + d);
+// A lane's part of a row as it lies in memory, and as pairs.
+template <class T, class L>
+struct Held {
+  Pack<T, L::V> v[L::J];
+  __device__ __forceinline__ void get(const T* row, int l, const bool (&ok)[L::J], bool live) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] = ok ? to_f32(q.v[k]) : 0.f;
-}
-template <class T, int V>
-__device__ __forceinline__ void put(T* row, int64_t d, bool ok, const float (&v)[V]) {
-  if (!ok) return;
-  Pack<T, V> q;
+    for (int j = 0; j < L::J; ++j) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) q.v[k] = from_f32<T>(v[k]);
-  *reinterpret_cast<Pack<T, V>*>(row + d) = q;
-}
-template <int V>
-__device__ __forceinline__ void weights(const float* w, int64_t d, bool ok, float (&v)[V]) {
+      for (int k = 0; k < L::V; ++k) v[j].v[k] = from_f32<T>(0.f);
+      if (live && ok[j])
+        v[j] = *reinterpret_cast<const Pack<T, L::V>*>(row + L::channel(j, l));
+    }
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    Pack<T, 2> q;
+    q.v[0] = v[2 * i / L::V].v[2 * i % L::V];
+    q.v[1] = v[(2 * i + 1) / L::V].v[(2 * i + 1) % L::V];
+    return to_f32x2(q);
+  }
+  __device__ __forceinline__ void set(int i, float2 f) {
+    const Pack<T, 2> q = from_f32x2<T>(f);
+    v[2 * i / L::V].v[2 * i % L::V] = q.v[0];
+    v[(2 * i + 1) / L::V].v[(2 * i + 1) % L::V] = q.v[1];
+  }
+  __device__ __forceinline__ void put(T* row, int l, const bool (&ok)[L::J]) const {
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] = ok && w ? w[d + k] : 0.f;
-}
+    for (int j = 0; j < L::J; ++j)
+      if (ok[j]) *reinterpret_cast<Pack<T, L::V>*>(row + L::channel(j, l)) = v[j];
+  }
+};
 
-template <class T, int V, int WR, int PER, bool BRANCH>
-__global__ void __launch_bounds__(Layout<T, V, WR, PER>::kThreads) norm_forward_kernel(NormArgs<T> a) {
-  using L = Layout<T, V, WR, PER>;
-  constexpr int J = L::J;
-  __shared__ float red[L::kRows][2][WR];
-  const int group = threadIdx.x / (32 * WR), l = threadIdx.x % (32 * WR);
-  RowSum<WR> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
-  const int64_t G = pack_groups(a.D);
-  int64_t d[J];
-  bool ok[J];
+// The two weight vectors that rows need, s w1 and w2, by pair and lane: from
+// shared memory, or in the widest layout (64 KB of them) from global memory.
+template <class L, bool BRANCH>
+struct Weights {
+  static constexpr bool kShared = L::H * L::NL <= 2048;
+  static constexpr int kSize = kShared ? L::H * L::NL : 1;
+  float2 *sw_, *w2_;
+  const float *s, *w1, *w2g;
+  int64_t D;
+  int l;
+  __device__ __forceinline__ float2 from_global(int i, const float* p, const float* q) const {
+    const int d0 = L::channel_of(i, 0, l), d1 = L::channel_of(i, 1, l);
+    return make_float2(d0 < D ? (q ? p[d0] * q[d0] : p[d0]) : 0.f,
+                       d1 < D ? (q ? p[d1] * q[d1] : p[d1]) : 0.f);
+  }
+  __device__ __forceinline__ float2 sw(int i) const {
+    return kShared ? sw_[i * L::NL + l] : from_global(i, s, w1);
+  }
+  __device__ __forceinline__ float2 w2(int i) const {
+    return kShared ? w2_[i * L::NL + l] : from_global(i, w2g, nullptr);
+  }
+  template <class T>
+  __device__ Weights(const NormArgs<T>& a, float2* sw, float2* w2)
+      : sw_(sw), w2_(w2), s(a.s), w1(a.w1), w2g(a.w2), D(a.D) {
+    if (kShared)
+      for (int k = threadIdx.x; k < kSize; k += L::kThreads) {
+        l = k % L::NL;
+        w2[k] = from_global(k / L::NL, w2g, nullptr);
+        if (BRANCH) sw[k] = from_global(k / L::NL, s, w1);
+      }
+    __syncthreads();
+    l = threadIdx.x % L::NL;
+  }
+};
+
+template <class T, class L, bool BRANCH>
+__global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArgs<T> a) {
+  constexpr int H = L::H, NL = L::NL;
+  __shared__ float red[L::kRows][2][L::WR];
+  __shared__ float2 sw_at[BRANCH ? Weights<L, BRANCH>::kSize : 1], w2_at[Weights<L, BRANCH>::kSize];
+  const Weights<L, BRANCH> weight(a, sw_at, w2_at);
+  const int group = threadIdx.x / NL, l = threadIdx.x % NL;
+  RowSum<L::WR> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
+  bool ok[L::J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) d[j] = (int64_t)(j * 32 * WR + l) * V, ok[j] = d[j] < a.D;
+  for (int j = 0; j < L::J; ++j) ok[j] = L::channel(j, l) < a.D;
 
   for (int64_t row = (int64_t)blockIdx.x * L::kRows + group; row < a.rows;
        row += (int64_t)gridDim.x * L::kRows) {
-    const int64_t b = row / a.T_, t = row - b * a.T_;
-    const bool live = t < valid_length(a.lengths, b, a.T_);
-    float r[J][V];
-    float rz = 0.f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) get<T, V>(a.x.row(b, t), d[j], ok[j] && live, r[j]);
+    int64_t b, t;
+    locate(a.places, row, b, t);
+    const bool live = !a.lengths || t < a.lengths[b];
+    Held<T, L> x, z, g;
+    x.get(a.x.row(b, t), l, ok, live);
     if (BRANCH) {
-      float z[J][V], g[J][V];
-      float q = 0.f;
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        get<T, V>(a.z.row(b, t), d[j], ok[j] && live, z[j]);
-        get<T, V>(a.g.row(b, t), d[j], ok[j] && live, g[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int k = 0; k < V; ++k) q = fmaf(z[j][k], z[j][k], q);
-      rz = rsqrtf(row_sum(q) * a.inv_d + a.eps);
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        float w1[V], sc[V];
-        weights<V>(a.w1, d[j], ok[j], w1);
-        weights<V>(a.s, d[j], ok[j], sc);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          float sig, neg;
-          sigmoid_pair(g[j][k], sig, neg);
-          r[j][k] = fmaf(sc[k] * (g[j][k] * sig), z[j][k] * rz * w1[k], r[j][k]);
-        }
-      }
+      z.get(a.z.row(b, t), l, ok, live);
+      g.get(a.g.row(b, t), l, ok, live);
     }
-    float q = 0.f;
+    float rz = 0.f;
+    float2 r[H], q = both(0.f);
+    if (BRANCH) {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+      for (int i = 0; i < H; ++i) q = __ffma2_rn(z.pair(i), z.pair(i), q);
+      rz = rsqrtf(row_sum(q.x + q.y) * a.inv_d + a.eps);
+      q = both(0.f);
+    }
 #pragma unroll
-      for (int k = 0; k < V; ++k) q = fmaf(r[j][k], r[j][k], q);
-    const float rr = rsqrtf(row_sum(q) * a.inv_d + a.eps);
+    for (int i = 0; i < H; ++i) {
+      r[i] = x.pair(i);
+      if (BRANCH) {
+        float2 sig, neg;
+        sigmoid_pair2(g.pair(i), sig, neg);
+        const float2 u = __fmul2_rn(__fmul2_rn(g.pair(i), sig), weight.sw(i));
+        r[i] = __ffma2_rn(u, __fmul2_rn(z.pair(i), both(rz)), r[i]);
+      }
+      q = __ffma2_rn(r[i], r[i], q);
+    }
+    const float rr = rsqrtf(row_sum(q.x + q.y) * a.inv_d + a.eps);
     if (a.stats && l == 0) {
       a.stats[2 * row] = rz;
       a.stats[2 * row + 1] = rr;
     }
+    Held<T, L> out;
+    if (BRANCH) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float w2[V], n[V];
-      weights<V>(a.w2, d[j], ok[j], w2);
-      if (BRANCH) put<T, V>(a.r.row(b, t), d[j], ok[j], r[j]);
+      for (int i = 0; i < H; ++i) out.set(i, r[i]);
+      out.put(a.r.row(b, t), l, ok);
+    }
 #pragma unroll
-      for (int k = 0; k < V; ++k) n[k] = live ? r[j][k] * rr * w2[k] : 0.f;
-      put<T, V>(a.n.row(b, t), d[j], ok[j], n);
-      if (a.codes) {  // the checkpoint holds what n holds after rounding
-        Pack<int8_t, V> c;
-        Pack<T, V> rounded;
+    for (int i = 0; i < H; ++i)
+      out.set(i, live ? __fmul2_rn(__fmul2_rn(r[i], both(rr)), weight.w2(i)) : both(0.f));
+    out.put(a.n.row(b, t), l, ok);
+    if (a.codes) {  // the checkpoint of n as it was rounded
+      const int64_t G = pack_groups(a.D);
 #pragma unroll
-        for (int k = 0; k < V; ++k) rounded.v[k] = from_f32<T>(ok[j] ? n[k] : 0.f);
-        const uint8_t byte = pack_encode(rounded, c);
-        if (d[j] < G * kPackGroup) {
-          *reinterpret_cast<Pack<int8_t, V>*>(a.codes + row * G * kPackGroup + d[j]) = c;
-          if (d[j] % kPackGroup == 0) a.scales[row * G + d[j] / kPackGroup] = byte;
+      for (int j = 0; j < L::J; ++j) {
+        const int d = L::channel(j, l);
+        Pack<int8_t, L::V> c;
+        if (!ok[j])
+#pragma unroll
+          for (int k = 0; k < L::V; ++k) out.v[j].v[k] = from_f32<T>(0.f);
+        const uint8_t byte = pack_encode(out.v[j], c);
+        if (d < G * kPackGroup) {
+          *reinterpret_cast<Pack<int8_t, L::V>*>(a.codes + row * G * kPackGroup + d) = c;
+          if (d % kPackGroup == 0) a.scales[row * G + d / kPackGroup] = byte;
         }
       }
     }
   }
 }
 
-template <class T, int V, int WR, int PER, bool BRANCH>
-__global__ void __launch_bounds__(Layout<T, V, WR, PER>::kThreads) norm_backward_kernel(NormArgs<T> a) {
-  using L = Layout<T, V, WR, PER>;
-  constexpr int J = L::J;
-  __shared__ float red[L::kRows][2][WR];
-  __shared__ float sums[L::kRows > 1 ? 32 * WR * PER : 1];
-  const int group = threadIdx.x / (32 * WR), l = threadIdx.x % (32 * WR);
-  RowSum<WR> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
-  int64_t d[J];
-  bool ok[J];
+template <class T, class L, bool BRANCH>
+__global__ void __launch_bounds__(L::kThreads) norm_backward_kernel(const NormArgs<T> a) {
+  constexpr int H = L::H, NL = L::NL;
+  __shared__ float red[L::kRows][2][L::WR];
+  __shared__ float2 sw_at[BRANCH ? Weights<L, BRANCH>::kSize : 1], w2_at[Weights<L, BRANCH>::kSize];
+  __shared__ float2 sums[L::kRows > 1 ? H * NL : 1];
+  const Weights<L, BRANCH> weight(a, sw_at, w2_at);
+  const int group = threadIdx.x / NL, l = threadIdx.x % NL;
+  RowSum<L::WR> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
+  bool ok[L::J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) d[j] = (int64_t)(j * 32 * WR + l) * V, ok[j] = d[j] < a.D;
-  float acc[3][J][V];
+  for (int j = 0; j < L::J; ++j) ok[j] = L::channel(j, l) < a.D;
+  float2 acc[2][H];
 #pragma unroll
-  for (int m = 0; m < 3; ++m)
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int k = 0; k < V; ++k) acc[m][j][k] = 0.f;
+  for (int i = 0; i < H; ++i) acc[0][i] = acc[1][i] = both(0.f);
 
   for (int64_t row = (int64_t)blockIdx.x * L::kRows + group; row < a.rows;
        row += (int64_t)gridDim.x * L::kRows) {
-    const int64_t b = row / a.T_, t = row - b * a.T_;
-    const bool live = t < valid_length(a.lengths, b, a.T_);
-    const float zero[V] = {};
-    if (!live) {  // the whole row group takes this branch together
+    int64_t b, t;
+    locate(a.places, row, b, t);
+    Held<T, L> out;
+    if (a.lengths && t >= a.lengths[b]) {  // the whole row group takes this branch together
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        put<T, V>(a.dx.row(b, t), d[j], ok[j], zero);
-        if (BRANCH) {
-          put<T, V>(a.dz.row(b, t), d[j], ok[j], zero);
-          put<T, V>(a.dg.row(b, t), d[j], ok[j], zero);
-        }
+      for (int i = 0; i < H; ++i) out.set(i, both(0.f));
+      out.put(a.dx.row(b, t), l, ok);
+      if (BRANCH) {
+        out.put(a.dz.row(b, t), l, ok);
+        out.put(a.dg.row(b, t), l, ok);
       }
       continue;
     }
-    const float rz = a.stats[2 * row], rr = a.stats[2 * row + 1];
-    float r[J][V], z[J][V], g[J][V], dn[J][V], dr[J][V];
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      get<T, V>(a.x.row(b, t), d[j], ok[j], r[j]);
-      if (BRANCH) {
-        get<T, V>(a.z.row(b, t), d[j], ok[j], z[j]);
-        get<T, V>(a.g.row(b, t), d[j], ok[j], g[j]);
-      }
-      get<T, V>(a.dn.p ? a.dn.row(b, t) : nullptr, d[j], ok[j] && a.dn.p, dn[j]);
-      get<T, V>(a.dr.p ? a.dr.row(b, t) : nullptr, d[j], ok[j] && a.dr.p, dr[j]);
-    }
-    float q = 0.f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float w1[V], sc[V], w2[V];
-      weights<V>(a.w2, d[j], ok[j], w2);
-      if (BRANCH) {
-        weights<V>(a.w1, d[j], ok[j], w1);
-        weights<V>(a.s, d[j], ok[j], sc);
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (BRANCH) {
-          float sig, neg;
-          sigmoid_pair(g[j][k], sig, neg);
-          z[j][k] *= rz;
-          r[j][k] = fmaf(sc[k] * (g[j][k] * sig), z[j][k] * w1[k], r[j][k]);
-        }
-        r[j][k] *= rr;  // rh
-        acc[2][j][k] = fmaf(dn[j][k], r[j][k], acc[2][j][k]);
-        dn[j][k] *= w2[k];
-        q = fmaf(dn[j][k], r[j][k], q);
-      }
-    }
-    const float c2 = row_sum(q) * a.inv_d;
-    q = 0.f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float w1[V], sc[V];
-      if (BRANCH) {
-        weights<V>(a.w1, d[j], ok[j], w1);
-        weights<V>(a.s, d[j], ok[j], sc);
-      }
-      float dg[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float dd = fmaf(rr, dn[j][k] - r[j][k] * c2, dr[j][k]);
-        dr[j][k] = dd;
-        if (BRANCH) {
-          float sig, neg;
-          sigmoid_pair(g[j][k], sig, neg);
-          const float u = g[j][k] * sig, bn = z[j][k] * w1[k];
-          const float db = dd * sc[k] * u;
-          acc[0][j][k] = fmaf(db, z[j][k], acc[0][j][k]);
-          acc[1][j][k] = fmaf(dd * u, bn, acc[1][j][k]);
-          dg[k] = dd * sc[k] * bn * sig * fmaf(g[j][k], neg, 1.f);
-          dn[j][k] = db * w1[k];  // the row's db w1 takes dn's place
-          q = fmaf(dn[j][k], z[j][k], q);
-        }
-      }
-      put<T, V>(a.dx.row(b, t), d[j], ok[j], dr[j]);
-      if (BRANCH) put<T, V>(a.dg.row(b, t), d[j], ok[j], dg);
-    }
+    Held<T, L> x, z, g, dn, dr;
+    x.get(a.x.row(b, t), l, ok, true);
     if (BRANCH) {
-      const float c1 = row_sum(q) * a.inv_d;
+      z.get(a.z.row(b, t), l, ok, true);
+      g.get(a.g.row(b, t), l, ok, true);
+    }
+    dn.get(a.dn.row(b, t), l, ok, a.dn.p != nullptr);
+    dr.get(a.dr.row(b, t), l, ok, a.dr.p != nullptr);
+    const float2 rz = both(a.stats[2 * row]), rr = both(a.stats[2 * row + 1]);
+    float2 rh[H], sig[BRANCH ? H : 1], q = both(0.f);
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) dn[j][k] = rz * (dn[j][k] - z[j][k] * c1);
-        put<T, V>(a.dz.row(b, t), d[j], ok[j], dn[j]);
+    for (int i = 0; i < H; ++i) {
+      rh[i] = x.pair(i);
+      if (BRANCH) {
+        float2 neg;
+        sigmoid_pair2(g.pair(i), sig[i], neg);
+        const float2 u = __fmul2_rn(__fmul2_rn(g.pair(i), sig[i]), weight.sw(i));
+        rh[i] = __ffma2_rn(u, __fmul2_rn(z.pair(i), rz), rh[i]);
       }
+      rh[i] = __fmul2_rn(rh[i], rr);
+      acc[1][i] = __ffma2_rn(dn.pair(i), rh[i], acc[1][i]);
+      q = __ffma2_rn(__fmul2_rn(dn.pair(i), weight.w2(i)), rh[i], q);
+    }
+    const float2 c2 = both(-row_sum(q.x + q.y) * a.inv_d);
+    q = both(0.f);
+    Held<T, L> gate;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const float2 p = __fmul2_rn(dn.pair(i), weight.w2(i));
+      const float2 d = __ffma2_rn(rr, __ffma2_rn(rh[i], c2, p), dr.pair(i));
+      out.set(i, d);
+      if (BRANCH) {
+        const float2 zh = __fmul2_rn(z.pair(i), rz), gi = g.pair(i);
+        const float2 du = __fmul2_rn(d, __fmul2_rn(gi, sig[i]));
+        acc[0][i] = __ffma2_rn(du, zh, acc[0][i]);
+        // silu'(g) = sig (1 + g (1 - sig))
+        const float2 slope = __fmul2_rn(
+            sig[i], __ffma2_rn(gi, sub2(both(1.f), sig[i]), both(1.f)));
+        const float2 ds = __fmul2_rn(d, weight.sw(i));
+        gate.set(i, __fmul2_rn(__fmul2_rn(ds, zh), slope));
+        rh[i] = __fmul2_rn(du, weight.sw(i));  // db w1 takes rh's place
+        q = __ffma2_rn(rh[i], zh, q);
+      }
+    }
+    out.put(a.dx.row(b, t), l, ok);
+    if (BRANCH) {
+      gate.put(a.dg.row(b, t), l, ok);
+      const float2 c1 = both(-row_sum(q.x + q.y) * a.inv_d);
+#pragma unroll
+      for (int i = 0; i < H; ++i)
+        out.set(i, __fmul2_rn(rz, __ffma2_rn(__fmul2_rn(z.pair(i), rz), c1, rh[i])));
+      out.put(a.dz.row(b, t), l, ok);
     }
   }
 
   // the CTA's sums, its row groups added in order
 #pragma unroll
-  for (int m = BRANCH ? 0 : 2; m < 3; ++m) {
+  for (int m = BRANCH ? 0 : 1; m < 2; ++m) {
     if (L::kRows > 1) {
+#pragma unroll 1
       for (int turn = L::kRows - 1; turn > 0; --turn) {
         __syncthreads();
         if (group == turn)
 #pragma unroll
-          for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) sums[(j * V + k) * 32 * WR + l] = acc[m][j][k];
+          for (int i = 0; i < H; ++i) sums[i * NL + l] = acc[m][i];
         __syncthreads();
         if (group == turn - 1)
 #pragma unroll
-          for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) acc[m][j][k] += sums[(j * V + k) * 32 * WR + l];
+          for (int i = 0; i < H; ++i) acc[m][i] = __fadd2_rn(acc[m][i], sums[i * NL + l]);
       }
     }
     if (group == 0)
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (ok[j]) a.partial[((int64_t)blockIdx.x * 3 + m) * a.D + d[j] + k] = acc[m][j][k];
+      for (int i = 0; i < H; ++i) {
+        float* p = a.partial + ((int64_t)blockIdx.x * 2 + m) * a.D;
+        const int d0 = L::channel_of(i, 0, l), d1 = L::channel_of(i, 1, l);
+        if (d0 < a.D) p[d0] = acc[m][i].x;
+        if (d1 < a.D) p[d1] = acc[m][i].y;
+      }
   }
 }
 
-// Sums the CTAs' partials in a fixed order: a block takes 32 channels, its
-// eight rows of threads every eighth CTA.
-__global__ void norm_reduce_kernel(int64_t D, int first, int ctas,
-                                   const float* __restrict__ partial, float* __restrict__ out) {
-  __shared__ float part[8][33];
-  const int64_t n = (int64_t)blockIdx.x * 32 + threadIdx.x + first * D;
-  float s = 0.f;
-  if (n < 3 * D)
-    for (int c = threadIdx.y; c < ctas; c += 8) s += partial[(int64_t)c * 3 * D + n];
-  part[threadIdx.y][threadIdx.x] = s;
+// Sums the CTAs' partials in a fixed order: a block takes 32 channels of one
+// of the two sums, its 32 rows of threads every 32nd CTA.
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(int64_t D, int first, int ctas,
+                                                           const float* __restrict__ w1,
+                                                           const float* __restrict__ s,
+                                                           const float* __restrict__ partial,
+                                                           float* __restrict__ out) {
+  __shared__ float part[32][33];
+  const int m = blockIdx.y + first;
+  const int64_t d = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  float v = 0.f;
+  if (d < D)
+    for (int c = threadIdx.y; c < ctas; c += 32) v += partial[((int64_t)c * 2 + m) * D + d];
+  part[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
-  if (threadIdx.y || n >= 3 * D) return;
+  if (threadIdx.y || d >= D) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) s += part[k][threadIdx.x];
-  out[n] = s;
+  for (int k = 1; k < 32; ++k) v += part[k][threadIdx.x];
+  if (m) {
+    out[2 * D + d] = v;
+  } else {
+    out[d] = s[d] * v;
+    out[D + d] = w1[d] * v;
+  }
 }
 
 template <class T>
 NormArgs<T> norm_args(const semicrf_block_norm* p) {
   NormArgs<T> a{};
   a.rows = p->batch * p->T;
-  a.T_ = p->T;
+  a.places = make_places(p->batch, p->T);
   a.D = p->D;
   a.eps = p->eps;
   a.inv_d = 1.f / (float)p->D;
@@ -343,37 +384,50 @@ NormArgs<T> norm_args(const semicrf_block_norm* p) {
   return a;
 }
 
-int64_t backward_ctas(int64_t rows, int at_once) {
+// CTAs of a backward launch: four of 128 threads an SM, fewer larger ones.
+int64_t backward_ctas(int64_t rows, int at_once, int threads) {
   const int64_t all = (rows + at_once - 1) / at_once;
-  return std::max<int64_t>(1, std::min<int64_t>(all, 4 * device_sm_count()));
+  const int per_sm = std::max(1, 512 / threads);
+  return std::max<int64_t>(1, std::min<int64_t>(all, (int64_t)per_sm * device_sm_count()));
 }
 
-template <class T, int V, int WR, int PER, bool BRANCH>
+template <class T, class L, bool BRANCH>
 int launch(const NormArgs<T>& a, bool backward, float* grad_weights, cudaStream_t stream) {
-  using L = Layout<T, V, WR, PER>;
   if (!backward) {
     const int64_t all = (a.rows + L::kRows - 1) / L::kRows;
-    const unsigned grid = (unsigned)std::min<int64_t>(all, 16 * device_sm_count());
-    if (grid) norm_forward_kernel<T, V, WR, PER, BRANCH><<<grid, L::kThreads, 0, stream>>>(a);
+    const int64_t most = (int64_t)std::max(1, 1024 / L::kThreads) * device_sm_count();
+    const unsigned grid = (unsigned)std::min<int64_t>(all, most);
+    if (grid) norm_forward_kernel<T, L, BRANCH><<<grid, L::kThreads, 0, stream>>>(a);
     return launch_status();
   }
-  const int ctas = (int)backward_ctas(a.rows, L::kRows);
-  norm_backward_kernel<T, V, WR, PER, BRANCH><<<ctas, L::kThreads, 0, stream>>>(a);
-  const int first = BRANCH ? 0 : 2;
-  const unsigned rg = (unsigned)(((3 - first) * a.D + 31) / 32);
-  norm_reduce_kernel<<<rg, dim3(32, 8), 0, stream>>>(a.D, first, ctas, a.partial, grad_weights);
+  const int ctas = (int)backward_ctas(a.rows, L::kRows, L::kThreads);
+  norm_backward_kernel<T, L, BRANCH><<<ctas, L::kThreads, 0, stream>>>(a);
+  const int first = BRANCH ? 0 : 1;
+  const dim3 grid((unsigned)((a.D + 31) / 32), 2 - first);
+  norm_reduce_kernel<<<grid, dim3(32, 32), 0, stream>>>(a.D, first, ctas, a.w1, a.s, a.partial,
+                                                        grad_weights);
   return launch_status();
 }
 
-// The fewest warps whose registers hold a row: up to 16 channels a lane.
+// The fewest warps whose registers hold a row: 16 channels a lane where 16-bit
+// values lie packed, 8 else (16 above 4096, where 8 would want 32 warps).
 template <class T, int V, bool BRANCH>
 int launch_width(const NormArgs<T>& a, bool backward, float* gw, cudaStream_t s) {
-  if (a.D <= 256) return launch<T, V, 1, 8, BRANCH>(a, backward, gw, s);
-  if (a.D <= 512) return launch<T, V, 1, 16, BRANCH>(a, backward, gw, s);
-  if (a.D <= 1024) return launch<T, V, 2, 16, BRANCH>(a, backward, gw, s);
-  if (a.D <= 2048) return launch<T, V, 4, 16, BRANCH>(a, backward, gw, s);
-  if (a.D <= 4096) return launch<T, V, 8, 16, BRANCH>(a, backward, gw, s);
-  return launch<T, V, 16, 16, BRANCH>(a, backward, gw, s);
+  constexpr int W = V < 4 ? V : 4;
+  if (a.D <= 128) return launch<T, Layout<T, W, 1, 4>, BRANCH>(a, backward, gw, s);
+  if (a.D <= 256) return launch<T, Layout<T, V, 1, 8>, BRANCH>(a, backward, gw, s);
+  if (a.D > 4096) return launch<T, Layout<T, V, 16, 16>, BRANCH>(a, backward, gw, s);
+  if constexpr (V * sizeof(T) == 16 && sizeof(T) == 2) {
+    if (a.D <= 512) return launch<T, Layout<T, V, 1, 16>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 1024) return launch<T, Layout<T, V, 2, 16>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 2048) return launch<T, Layout<T, V, 4, 16>, BRANCH>(a, backward, gw, s);
+    return launch<T, Layout<T, V, 8, 16>, BRANCH>(a, backward, gw, s);
+  } else {
+    if (a.D <= 512) return launch<T, Layout<T, V, 2, 8>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 1024) return launch<T, Layout<T, V, 4, 8>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 2048) return launch<T, Layout<T, V, 8, 8>, BRANCH>(a, backward, gw, s);
+    return launch<T, Layout<T, V, 16, 8>, BRANCH>(a, backward, gw, s);
+  }
 }
 
 template <class T>
@@ -426,8 +480,8 @@ int run_backward(const semicrf_block_norm* p, const float* stats, const semicrf_
 }  // namespace
 
 size_t block_norm_workspace_bytes(const semicrf_block_norm* p) {
-  // at most one CTA a row, whatever the layout
-  return sizeof(float) * 3 * p->D * backward_ctas(p->batch * p->T, 1);
+  // the most CTAs that any layout launches
+  return sizeof(float) * 2 * p->D * backward_ctas(p->batch * p->T, 1, 128);
 }
 
 int block_norm_forward(const semicrf_block_norm* p, const semicrf_sequence& r,
