@@ -696,6 +696,34 @@ def test_packed_linear(dtype):
     assert torch.equal(gw, gw2)
 
 
+def test_calls_from_a_thread_without_a_context():
+    """As in autograd's worker threads: nothing in a call before the kernel's
+    launch may rely on a CUDA context that is current already."""
+    import threading
+
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(40)
+    x = _normal(g, 4, 10, 512, dtype=torch.bfloat16)
+    leaf = x.clone().requires_grad_(True)
+
+    def call():
+        h, _ = tsm.gated_linear_recurrence(leaf, leaf)
+        gx, = torch.autograd.grad(h, leaf, x)
+        w = tsm.packed_weight_grad(x, tsm.pack_activation(x))
+        return h.detach(), gx, w
+
+    for _ in range(3):
+        want = call()  # fills the allocator, so that the thread allocates nothing
+        got = []
+        t = threading.Thread(target=lambda: got.append(call()))
+        t.start()
+        t.join()
+        for a, b in zip(want, got[0]):
+            assert torch.equal(a, b)
+        del got
+
+
 # ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------

@@ -566,7 +566,9 @@ def float_vector(t, name: str, shape, device) -> torch.Tensor:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     if t.shape != torch.Size(shape):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t.to(torch.float32).contiguous()
+    if t.dtype != torch.float32:
+        t = t.to(torch.float32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def valid_lengths(lengths, B: int, T: int, device) -> Optional[torch.Tensor]:
@@ -582,7 +584,14 @@ def valid_lengths(lengths, B: int, T: int, device) -> Optional[torch.Tensor]:
         lo, hi = int(lengths.min()), int(lengths.max())
         if lo < 0 or hi > T:
             raise ValueError(f"lengths must lie in [0, {T}], got [{lo}, {hi}]")
-    return lengths.to(device=device, dtype=torch.int64).contiguous()
+    if lengths.dtype != torch.int64 or lengths.device != device:
+        lengths = lengths.to(device=device, dtype=torch.int64)
+    return lengths.contiguous()
+
+
+def _raw_stream(device) -> int:
+    """The current stream's handle, without the stream object _stream makes."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _sequence(t: Optional[torch.Tensor]) -> SemicrfSequence:
@@ -614,6 +623,18 @@ def _on(device):
     return torch.cuda.device(device)
 
 
+def first_order(backward):
+    """Marks an autograd backward as differentiable once.  torch's
+    once_differentiable costs as much as the call it wraps and only matters
+    when a graph of the backward is being built."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def choose(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return choose
+
+
 def _recurrence(x, gate, initial_state, lengths, reverse) -> SemicrfRecurrence:
     B, T, D = x.shape
     return SemicrfRecurrence(B, T, D, ACTIVATION_DTYPES[x.dtype], int(bool(reverse)),
@@ -627,12 +648,12 @@ def recurrence_forward(x, gate, initial_state, lengths, reverse, want_saved):
     dev = x.device
     p = _recurrence(x, gate, initial_state, lengths, reverse)
     with _on(dev):
-        h = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        h = torch.empty_like(x)
         state = torch.empty((B, D), dtype=torch.float32, device=dev)
         saved = _scratch(lib.semicrf_recurrence_saved_size(p), dev) if want_saved else None
         ws = _scratch(lib.semicrf_recurrence_workspace_size(p), dev)
         st = lib.semicrf_recurrence_forward(p, _sequence(h), state.data_ptr(), _addr(saved),
-                                            ws.data_ptr(), ws.numel(), _stream(dev))
+                                            ws.data_ptr(), ws.numel(), _raw_stream(dev))
         check(st, "semicrf_recurrence_forward")
     return h, state, saved
 
@@ -644,13 +665,12 @@ def recurrence_backward(x, gate, lengths, reverse, saved, grad_h, grad_state, wa
     dev = x.device
     p = _recurrence(x, gate, None, lengths, reverse)
     with _on(dev):
-        gx = torch.empty((B, T, D), dtype=x.dtype, device=dev)
-        gg = torch.empty((B, T, D), dtype=x.dtype, device=dev)
+        gx, gg = torch.empty_like(x), torch.empty_like(gate)
         gi = torch.empty((B, D), dtype=torch.float32, device=dev) if want_initial else None
         ws = _scratch(lib.semicrf_recurrence_workspace_size(p), dev)
         st = lib.semicrf_recurrence_backward(p, saved.data_ptr(), _sequence(grad_h),
                                              _addr(grad_state), _sequence(gx), _sequence(gg),
-                                             _addr(gi), ws.data_ptr(), ws.numel(), _stream(dev))
+                                             _addr(gi), ws.data_ptr(), ws.numel(), _raw_stream(dev))
         check(st, "semicrf_recurrence_backward")
     return gx, gg, gi
 
@@ -663,11 +683,11 @@ def recurrence_step(x, gate, state, active, state_out):
     with _on(dev):
         h = torch.empty((B, D), dtype=x.dtype, device=dev)
         if state_out is None:
-            state_out = torch.empty((B, D), dtype=torch.float32, device=dev)
+            state_out = torch.empty_like(state)
         st = lib.semicrf_recurrence_step(B, D, ACTIVATION_DTYPES[x.dtype], x.data_ptr(),
                                          x.stride(0), gate.data_ptr(), gate.stride(0),
                                          _addr(active), state.data_ptr(), state_out.data_ptr(),
-                                         h.data_ptr(), _stream(dev))
+                                         h.data_ptr(), _raw_stream(dev))
         check(st, "semicrf_recurrence_step")
     return h, state_out
 
@@ -698,13 +718,13 @@ def block_norm_forward(residual, branch, gate, branch_weight, residual_scale, ne
     p = _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
                     eps)
     with _on(dev):
-        out = None if branch is None else torch.empty((B, T, D), dtype=residual.dtype, device=dev)
-        normed = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+        out = None if branch is None else torch.empty_like(residual)
+        normed = torch.empty_like(residual)
         stats = (torch.empty((B, T, 2), dtype=torch.float32, device=dev) if want_statistics
                  else None)
         codes, scales = packed_buffers(B, T, D, dev) if pack else (None, None)
         st = lib.semicrf_block_norm_forward(p, _sequence(out), _sequence(normed), _addr(stats),
-                                            _addr(codes), _addr(scales), _stream(dev))
+                                            _addr(codes), _addr(scales), _raw_stream(dev))
         check(st, "semicrf_block_norm_forward")
     return out, normed, stats, codes, scales
 
@@ -719,17 +739,16 @@ def block_norm_backward(residual, branch, gate, branch_weight, residual_scale, n
     p = _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
                     eps)
     with _on(dev):
-        gr = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+        gr = torch.empty_like(residual)
         gb = gg = None
         if branch is not None:
-            gb = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
-            gg = torch.empty((B, T, D), dtype=residual.dtype, device=dev)
+            gb, gg = torch.empty_like(branch), torch.empty_like(gate)
         gw = torch.empty((3, D), dtype=torch.float32, device=dev)
         ws = _scratch(lib.semicrf_block_norm_workspace_size(p), dev)
         st = lib.semicrf_block_norm_backward(p, stats.data_ptr(), _sequence(grad_out),
                                              _sequence(grad_normed), _sequence(gr), _sequence(gb),
                                              _sequence(gg), gw.data_ptr(), ws.data_ptr(),
-                                             ws.numel(), _stream(dev))
+                                             ws.numel(), _raw_stream(dev))
         check(st, "semicrf_block_norm_backward")
     return gr, gb, gg, gw
 
@@ -742,7 +761,7 @@ def pack(x, lengths):
     with _on(dev):
         codes, scales = packed_buffers(B, T, D, dev)
         st = lib.semicrf_pack(B, T, D, ACTIVATION_DTYPES[x.dtype], _sequence(x), _addr(lengths),
-                              codes.data_ptr(), scales.data_ptr(), _stream(dev))
+                              codes.data_ptr(), scales.data_ptr(), _raw_stream(dev))
         check(st, "semicrf_pack")
     return codes, scales
 
@@ -755,7 +774,7 @@ def unpack(codes, scales, D: int, dtype):
     with _on(dev):
         out = torch.empty((B, T, D), dtype=dtype, device=dev)
         st = lib.semicrf_unpack(B * T, D, ACTIVATION_DTYPES[dtype], codes.data_ptr(),
-                                scales.data_ptr(), out.data_ptr(), _stream(dev))
+                                scales.data_ptr(), out.data_ptr(), _raw_stream(dev))
         check(st, "semicrf_unpack")
     return out
 
@@ -772,6 +791,6 @@ def packed_weight_grad(grad_output, codes, scales, D: int, lengths, out_dtype):
         st = lib.semicrf_packed_weight_grad(B, T, D, M, dt, _sequence(grad_output),
                                             codes.data_ptr(), scales.data_ptr(), _addr(lengths),
                                             ACTIVATION_DTYPES[out_dtype], out.data_ptr(),
-                                            ws.data_ptr(), ws.numel(), _stream(dev))
+                                            ws.data_ptr(), ws.numel(), _raw_stream(dev))
         check(st, "semicrf_packed_weight_grad")
     return out

@@ -13,7 +13,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .packed import PackedActivation
@@ -40,7 +39,7 @@ class _BlockNorm(torch.autograd.Function):
         return out, normed, codes, scales
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, grad_out, grad_normed, _codes, _scales):
         residual, branch, gate, w1, scale, w2, lengths, stats = ctx.saved_tensors
         if grad_out is not None:

@@ -21,8 +21,10 @@
 // an instruction.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "encoder_internal.cuh"
+#include "tma.cuh"
 
 namespace semicrf {
 int device_sm_count();  // api.cu
@@ -76,6 +78,10 @@ struct Layout {
   static constexpr int NL = 32 * WR;                  // lanes of a row
   static constexpr int kRows = WR >= 4 ? 1 : 4 / WR;  // rows that a CTA works on at once
   static constexpr int kThreads = NL * kRows;
+  // CTAs of the backward on an SM: 12 warps of 16 channels a lane (168 registers),
+  // 16 of 8 (128), 24 of 4 (80)
+  static constexpr int kWarpsPerSm = PER == 16 ? 12 : PER == 8 ? 16 : 24;
+  static constexpr int kPerSm = NL * kRows < 32 * kWarpsPerSm ? 32 * kWarpsPerSm / kThreads : 1;
   // channel of vector j of lane l
   __device__ static __forceinline__ int channel(int j, int l) { return (j * NL + l) * V; }
   // channel of half k of pair i of lane l
@@ -151,45 +157,152 @@ struct Weights {
   }
 };
 
-template <class T, class L, bool BRANCH>
+// How a row's inputs reach the pairs that are worked on.  Plain: into
+// registers.  Where a lane's vectors are 16 bytes, asynchronous copies keep the
+// next rows on their way to shared memory: it takes some 40 KB in flight on an
+// SM to keep HBM busy, and the sums and factors leave no registers for that.
+// A lane reads only what it copied itself, so no barrier is involved.
+enum Input { kX, kZ, kG, kDn, kDr };
+
+template <class T, class L, int N>
+struct PlainRows {
+  static constexpr int kSlots = 0;
+  Held<T, L> held[N];
+  __device__ __forceinline__ float2 pair(int k, int i) const { return held[k].pair(i); }
+};
+template <class T, class L, int N>
+struct RingRows {
+  static constexpr int kSlotBytes = N * L::J * L::kThreads * 16;
+  static constexpr int kSlots = 3 * kSlotBytes <= 96 * 1024 ? 3 : 2 * kSlotBytes <= 200 * 1024 ? 2 : 0;
+  unsigned char* at;  // this thread's part of the present slot
+  __device__ __forceinline__ float2 pair(int k, int i) const {
+    const int j = 2 * i / L::V;
+    const Pack<T, L::V> v =
+        *reinterpret_cast<const Pack<T, L::V>*>(at + (k * L::J + j) * L::kThreads * 16);
+    Pack<T, 2> q;
+    q.v[0] = v.v[2 * i % L::V];
+    q.v[1] = v.v[2 * i % L::V + 1];
+    return to_f32x2(q);
+  }
+};
+
+// Requests a row of N tensors into a slot of the ring: one group of copies a
+// row, whatever it holds.
+template <int N, class T, class L>
+__device__ __forceinline__ void request_row(const NormArgs<T>& a, const Seq<const T> (&src)[N],
+                                            unsigned char* ring, int slot, int64_t row, int l,
+                                            const bool (&ok)[L::J], L) {
+  int64_t b, t;
+  bool live = row < a.rows;
+  if (live) {
+    locate(a.places, row, b, t);
+    live = !a.lengths || t < a.lengths[b];
+  }
+  if (live)
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int j = 0; j < L::J; ++j) {
+        const bool has = src[k].p && ok[j];
+        asm volatile(
+            "cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(
+                ring + slot * RingRows<T, L, N>::kSlotBytes +
+                ((k * L::J + j) * L::kThreads + threadIdx.x) * 16)),
+            "l"(has ? src[k].row(b, t) + L::channel(j, l) : a.x.p), "r"(has ? 16 : 0)
+            : "memory");
+      }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// The checkpoint of n as it was rounded.
+template <class T, class L>
+__device__ __forceinline__ void put_codes(const NormArgs<T>& a, int64_t row, int l,
+                                          const bool (&ok)[L::J], const Held<T, L>& n) {
+  const int64_t G = pack_groups(a.D);
+#pragma unroll
+  for (int j = 0; j < L::J; ++j) {
+    const int d = L::channel(j, l);
+    Pack<T, L::V> v = n.v[j];
+    if (!ok[j])
+#pragma unroll
+      for (int k = 0; k < L::V; ++k) v.v[k] = from_f32<T>(0.f);
+    Pack<int8_t, L::V> c;
+    const uint8_t byte = pack_encode(v, c);
+    if (d < G * kPackGroup) {
+      *reinterpret_cast<Pack<int8_t, L::V>*>(a.codes + row * G * kPackGroup + d) = c;
+      if (d % kPackGroup == 0) a.scales[row * G + d / kPackGroup] = byte;
+    }
+  }
+}
+
+template <class T, class L, bool BRANCH, bool RING>
 __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArgs<T> a) {
   constexpr int H = L::H, NL = L::NL;
+  using Rows = typename std::conditional<RING, RingRows<T, L, 3>, PlainRows<T, L, 3>>::type;
+  constexpr int SLOTS = Rows::kSlots;
+  extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[L::kRows][2][L::WR];
   __shared__ float2 sw_at[BRANCH ? Weights<L, BRANCH>::kSize : 1], w2_at[Weights<L, BRANCH>::kSize];
-  const Weights<L, BRANCH> weight(a, sw_at, w2_at);
   const int group = threadIdx.x / NL, l = threadIdx.x % NL;
   RowSum<L::WR> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
   bool ok[L::J];
 #pragma unroll
   for (int j = 0; j < L::J; ++j) ok[j] = L::channel(j, l) < a.D;
 
-  for (int64_t row = (int64_t)blockIdx.x * L::kRows + group; row < a.rows;
-       row += (int64_t)gridDim.x * L::kRows) {
+  const Seq<const T> src[3] = {a.x, a.z, a.g};
+  const int64_t first = (int64_t)blockIdx.x * L::kRows + group;
+  const int64_t stride = (int64_t)gridDim.x * L::kRows;
+  Rows in;
+  const auto request = [&](int64_t row, int slot) {
+    if constexpr (RING) request_row<3>(a, src, ring, slot, row, l, ok, L());
+  };
+#pragma unroll
+  for (int k = 0; k < SLOTS - 1; ++k) request(first + k * stride, k);
+  const Weights<L, BRANCH> weight(a, sw_at, w2_at);
+  int slot = 0;
+  for (int64_t row = first; row < a.rows; row += stride) {
     int64_t b, t;
     locate(a.places, row, b, t);
     const bool live = !a.lengths || t < a.lengths[b];
-    Held<T, L> x, z, g;
-    x.get(a.x.row(b, t), l, ok, live);
-    if (BRANCH) {
-      z.get(a.z.row(b, t), l, ok, live);
-      g.get(a.g.row(b, t), l, ok, live);
+    if constexpr (RING) {
+      request(row + (SLOTS - 1) * stride, slot == 0 ? SLOTS - 1 : slot - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS > 0 ? SLOTS - 1 : 0) : "memory");
+      in.at = ring + slot * Rows::kSlotBytes + threadIdx.x * 16;
+      slot = slot == SLOTS - 1 ? 0 : slot + 1;
+    }
+    Held<T, L> out;
+    if (!live) {  // the whole row group takes this branch together
+#pragma unroll
+      for (int i = 0; i < H; ++i) out.set(i, both(0.f));
+      if (BRANCH) out.put(a.r.row(b, t), l, ok);
+      out.put(a.n.row(b, t), l, ok);
+      if (a.codes) put_codes<T, L>(a, row, l, ok, out);
+      continue;
+    }
+    if constexpr (!RING) {
+#pragma unroll
+      for (int k = 0; k < (BRANCH ? 3 : 1); ++k) in.held[k].get(src[k].row(b, t), l, ok, true);
     }
     float rz = 0.f;
     float2 r[H], q = both(0.f);
     if (BRANCH) {
 #pragma unroll
-      for (int i = 0; i < H; ++i) q = __ffma2_rn(z.pair(i), z.pair(i), q);
+      for (int i = 0; i < H; ++i) {
+        const float2 z = in.pair(kZ, i);
+        q = __ffma2_rn(z, z, q);
+      }
       rz = rsqrtf(row_sum(q.x + q.y) * a.inv_d + a.eps);
       q = both(0.f);
     }
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      r[i] = x.pair(i);
+      r[i] = in.pair(kX, i);
       if (BRANCH) {
         float2 sig, neg;
-        sigmoid_pair2(g.pair(i), sig, neg);
-        const float2 u = __fmul2_rn(__fmul2_rn(g.pair(i), sig), weight.sw(i));
-        r[i] = __ffma2_rn(u, __fmul2_rn(z.pair(i), both(rz)), r[i]);
+        const float2 g = in.pair(kG, i);
+        sigmoid_pair2(g, sig, neg);
+        const float2 u = __fmul2_rn(__fmul2_rn(g, sig), weight.sw(i));
+        r[i] = __ffma2_rn(u, __fmul2_rn(in.pair(kZ, i), both(rz)), r[i]);
       }
       q = __ffma2_rn(r[i], r[i], q);
     }
@@ -198,38 +311,25 @@ __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArg
       a.stats[2 * row] = rz;
       a.stats[2 * row + 1] = rr;
     }
-    Held<T, L> out;
     if (BRANCH) {
 #pragma unroll
       for (int i = 0; i < H; ++i) out.set(i, r[i]);
       out.put(a.r.row(b, t), l, ok);
     }
 #pragma unroll
-    for (int i = 0; i < H; ++i)
-      out.set(i, live ? __fmul2_rn(__fmul2_rn(r[i], both(rr)), weight.w2(i)) : both(0.f));
+    for (int i = 0; i < H; ++i) out.set(i, __fmul2_rn(__fmul2_rn(r[i], both(rr)), weight.w2(i)));
     out.put(a.n.row(b, t), l, ok);
-    if (a.codes) {  // the checkpoint of n as it was rounded
-      const int64_t G = pack_groups(a.D);
-#pragma unroll
-      for (int j = 0; j < L::J; ++j) {
-        const int d = L::channel(j, l);
-        Pack<int8_t, L::V> c;
-        if (!ok[j])
-#pragma unroll
-          for (int k = 0; k < L::V; ++k) out.v[j].v[k] = from_f32<T>(0.f);
-        const uint8_t byte = pack_encode(out.v[j], c);
-        if (d < G * kPackGroup) {
-          *reinterpret_cast<Pack<int8_t, L::V>*>(a.codes + row * G * kPackGroup + d) = c;
-          if (d % kPackGroup == 0) a.scales[row * G + d / kPackGroup] = byte;
-        }
-      }
-    }
+    if (a.codes) put_codes<T, L>(a, row, l, ok, out);
   }
+  if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <class T, class L, bool BRANCH>
-__global__ void __launch_bounds__(L::kThreads) norm_backward_kernel(const NormArgs<T> a) {
+template <class T, class L, bool BRANCH, bool RING>
+__global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_backward_kernel(const NormArgs<T> a) {
   constexpr int H = L::H, NL = L::NL;
+  using Rows = typename std::conditional<RING, RingRows<T, L, 5>, PlainRows<T, L, 5>>::type;
+  constexpr int SLOTS = Rows::kSlots;
+  extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[L::kRows][2][L::WR];
   __shared__ float2 sw_at[BRANCH ? Weights<L, BRANCH>::kSize : 1], w2_at[Weights<L, BRANCH>::kSize];
   __shared__ float2 sums[L::kRows > 1 ? H * NL : 1];
@@ -243,12 +343,38 @@ __global__ void __launch_bounds__(L::kThreads) norm_backward_kernel(const NormAr
 #pragma unroll
   for (int i = 0; i < H; ++i) acc[0][i] = acc[1][i] = both(0.f);
 
-  for (int64_t row = (int64_t)blockIdx.x * L::kRows + group; row < a.rows;
-       row += (int64_t)gridDim.x * L::kRows) {
+  const Seq<const T> src[5] = {a.x, a.z, a.g, a.dn, a.dr};
+  const int64_t first = (int64_t)blockIdx.x * L::kRows + group;
+  const int64_t stride = (int64_t)gridDim.x * L::kRows;
+  Rows in;
+  const auto request = [&](int64_t row, int slot) {
+    if constexpr (RING) request_row<5>(a, src, ring, slot, row, l, ok, L());
+  };
+  float next_z = 0.f, next_r = 0.f;
+  if (RING) {
+#pragma unroll
+    for (int k = 0; k < SLOTS - 1; ++k) request(first + k * stride, k);
+    if (first < a.rows) next_z = a.stats[2 * first], next_r = a.stats[2 * first + 1];
+  }
+  int slot = 0;
+  for (int64_t row = first; row < a.rows; row += stride) {
     int64_t b, t;
     locate(a.places, row, b, t);
+    const bool live = !a.lengths || t < a.lengths[b];
+    float2 rz, rr;
+    if constexpr (RING) {
+      request(row + (SLOTS - 1) * stride, slot == 0 ? SLOTS - 1 : slot - 1);
+      rz = both(next_z), rr = both(next_r);
+      if (row + stride < a.rows) {
+        next_z = a.stats[2 * (row + stride)];
+        next_r = a.stats[2 * (row + stride) + 1];
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS > 0 ? SLOTS - 1 : 0) : "memory");
+      in.at = ring + slot * Rows::kSlotBytes + threadIdx.x * 16;
+      slot = slot == SLOTS - 1 ? 0 : slot + 1;
+    }
     Held<T, L> out;
-    if (a.lengths && t >= a.lengths[b]) {  // the whole row group takes this branch together
+    if (!live) {  // the whole row group takes this branch together
 #pragma unroll
       for (int i = 0; i < H; ++i) out.set(i, both(0.f));
       out.put(a.dx.row(b, t), l, ok);
@@ -258,46 +384,45 @@ __global__ void __launch_bounds__(L::kThreads) norm_backward_kernel(const NormAr
       }
       continue;
     }
-    Held<T, L> x, z, g, dn, dr;
-    x.get(a.x.row(b, t), l, ok, true);
-    if (BRANCH) {
-      z.get(a.z.row(b, t), l, ok, true);
-      g.get(a.g.row(b, t), l, ok, true);
+    if constexpr (!RING) {
+#pragma unroll
+      for (int k = 0; k < 5; ++k)
+        if (BRANCH || (k != kZ && k != kG))
+          in.held[k].get(src[k].row(b, t), l, ok, src[k].p != nullptr);
+      rz = both(a.stats[2 * row]), rr = both(a.stats[2 * row + 1]);
     }
-    dn.get(a.dn.row(b, t), l, ok, a.dn.p != nullptr);
-    dr.get(a.dr.row(b, t), l, ok, a.dr.p != nullptr);
-    const float2 rz = both(a.stats[2 * row]), rr = both(a.stats[2 * row + 1]);
     float2 rh[H], sig[BRANCH ? H : 1], q = both(0.f);
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      rh[i] = x.pair(i);
+      rh[i] = in.pair(kX, i);
       if (BRANCH) {
         float2 neg;
-        sigmoid_pair2(g.pair(i), sig[i], neg);
-        const float2 u = __fmul2_rn(__fmul2_rn(g.pair(i), sig[i]), weight.sw(i));
-        rh[i] = __ffma2_rn(u, __fmul2_rn(z.pair(i), rz), rh[i]);
+        const float2 g = in.pair(kG, i);
+        sigmoid_pair2(g, sig[i], neg);
+        rh[i] = __ffma2_rn(__fmul2_rn(__fmul2_rn(g, sig[i]), weight.sw(i)),
+                           __fmul2_rn(in.pair(kZ, i), rz), rh[i]);
       }
       rh[i] = __fmul2_rn(rh[i], rr);
-      acc[1][i] = __ffma2_rn(dn.pair(i), rh[i], acc[1][i]);
-      q = __ffma2_rn(__fmul2_rn(dn.pair(i), weight.w2(i)), rh[i], q);
+      const float2 dn = in.pair(kDn, i);
+      acc[1][i] = __ffma2_rn(dn, rh[i], acc[1][i]);
+      q = __ffma2_rn(__fmul2_rn(dn, weight.w2(i)), rh[i], q);
     }
     const float2 c2 = both(-row_sum(q.x + q.y) * a.inv_d);
     q = both(0.f);
     Held<T, L> gate;
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      const float2 p = __fmul2_rn(dn.pair(i), weight.w2(i));
-      const float2 d = __ffma2_rn(rr, __ffma2_rn(rh[i], c2, p), dr.pair(i));
+      const float2 p = __fmul2_rn(in.pair(kDn, i), weight.w2(i));
+      const float2 d = __ffma2_rn(rr, __ffma2_rn(rh[i], c2, p), in.pair(kDr, i));
       out.set(i, d);
       if (BRANCH) {
-        const float2 zh = __fmul2_rn(z.pair(i), rz), gi = g.pair(i);
-        const float2 du = __fmul2_rn(d, __fmul2_rn(gi, sig[i]));
+        const float2 zh = __fmul2_rn(in.pair(kZ, i), rz), g = in.pair(kG, i);
+        const float2 du = __fmul2_rn(d, __fmul2_rn(g, sig[i]));
         acc[0][i] = __ffma2_rn(du, zh, acc[0][i]);
         // silu'(g) = sig (1 + g (1 - sig))
-        const float2 slope = __fmul2_rn(
-            sig[i], __ffma2_rn(gi, sub2(both(1.f), sig[i]), both(1.f)));
-        const float2 ds = __fmul2_rn(d, weight.sw(i));
-        gate.set(i, __fmul2_rn(__fmul2_rn(ds, zh), slope));
+        const float2 slope =
+            __fmul2_rn(sig[i], __ffma2_rn(g, sub2(both(1.f), sig[i]), both(1.f)));
+        gate.set(i, __fmul2_rn(__fmul2_rn(__fmul2_rn(d, weight.sw(i)), zh), slope));
         rh[i] = __fmul2_rn(du, weight.sw(i));  // db w1 takes rh's place
         q = __ffma2_rn(rh[i], zh, q);
       }
@@ -308,10 +433,11 @@ __global__ void __launch_bounds__(L::kThreads) norm_backward_kernel(const NormAr
       const float2 c1 = both(-row_sum(q.x + q.y) * a.inv_d);
 #pragma unroll
       for (int i = 0; i < H; ++i)
-        out.set(i, __fmul2_rn(rz, __ffma2_rn(__fmul2_rn(z.pair(i), rz), c1, rh[i])));
+        out.set(i, __fmul2_rn(rz, __ffma2_rn(__fmul2_rn(in.pair(kZ, i), rz), c1, rh[i])));
       out.put(a.dz.row(b, t), l, ok);
     }
   }
+  if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
 
   // the CTA's sums, its row groups added in order
 #pragma unroll
@@ -340,24 +466,27 @@ __global__ void __launch_bounds__(L::kThreads) norm_backward_kernel(const NormAr
   }
 }
 
-// Sums the CTAs' partials in a fixed order: a block takes 32 channels of one
-// of the two sums, its 32 rows of threads every 32nd CTA.
-__global__ void __launch_bounds__(1024) norm_reduce_kernel(int64_t D, int first, int ctas,
-                                                           const float* __restrict__ w1,
-                                                           const float* __restrict__ s,
-                                                           const float* __restrict__ partial,
-                                                           float* __restrict__ out) {
-  __shared__ float part[32][33];
-  const int m = blockIdx.y + first;
-  const int64_t d = (int64_t)blockIdx.x * 32 + threadIdx.x;
+// Sums the CTAs' partials in a fixed order: a block takes 8 channels of one of
+// the two sums, its 32 rows of threads every 32nd CTA.
+__global__ void __launch_bounds__(256) norm_reduce_kernel(int64_t D, int first, int ctas,
+                                                          const float* __restrict__ w1,
+                                                          const float* __restrict__ s,
+                                                          const float* __restrict__ partial,
+                                                          float* __restrict__ out) {
+  __shared__ float part[32][9];
+  const int m = blockIdx.y + first, x = threadIdx.x & 7, y = threadIdx.x >> 3;
+  const int64_t d = (int64_t)blockIdx.x * 8 + x;
   float v = 0.f;
-  if (d < D)
-    for (int c = threadIdx.y; c < ctas; c += 32) v += partial[((int64_t)c * 2 + m) * D + d];
-  part[threadIdx.y][threadIdx.x] = v;
+  if (d < D) {
+    const float* p = partial + m * D + d;
+#pragma unroll 8
+    for (int c = y; c < ctas; c += 32) v += p[(int64_t)c * 2 * D];
+  }
+  part[y][x] = v;
   __syncthreads();
-  if (threadIdx.y || d >= D) return;
+  if (y || d >= D) return;
 #pragma unroll
-  for (int k = 1; k < 32; ++k) v += part[k][threadIdx.x];
+  for (int k = 1; k < 32; ++k) v += part[k][x];
   if (m) {
     out[2 * D + d] = v;
   } else {
@@ -384,10 +513,10 @@ NormArgs<T> norm_args(const semicrf_block_norm* p) {
   return a;
 }
 
-// CTAs of a backward launch: four of 128 threads an SM, fewer larger ones.
-int64_t backward_ctas(int64_t rows, int at_once, int threads) {
+// CTAs of a backward launch: what is resident at once, so that each walks an
+// equal share of the rows.
+int64_t backward_ctas(int64_t rows, int at_once, int per_sm) {
   const int64_t all = (rows + at_once - 1) / at_once;
-  const int per_sm = std::max(1, 512 / threads);
   return std::max<int64_t>(1, std::min<int64_t>(all, (int64_t)per_sm * device_sm_count()));
 }
 
@@ -397,14 +526,26 @@ int launch(const NormArgs<T>& a, bool backward, float* grad_weights, cudaStream_
     const int64_t all = (a.rows + L::kRows - 1) / L::kRows;
     const int64_t most = (int64_t)std::max(1, 1024 / L::kThreads) * device_sm_count();
     const unsigned grid = (unsigned)std::min<int64_t>(all, most);
-    if (grid) norm_forward_kernel<T, L, BRANCH><<<grid, L::kThreads, 0, stream>>>(a);
+    constexpr bool kRing = BRANCH && L::V * sizeof(T) == 16 && RingRows<T, L, 3>::kSlots > 0;
+    const auto kernel = norm_forward_kernel<T, L, BRANCH, kRing>;
+    constexpr int bytes = kRing ? RingRows<T, L, 3>::kSlots * RingRows<T, L, 3>::kSlotBytes : 0;
+    if (bytes && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      bytes) != cudaSuccess)
+      return SEMICRF_ERR_CUDA;
+    if (grid) kernel<<<grid, L::kThreads, bytes, stream>>>(a);
     return launch_status();
   }
-  const int ctas = (int)backward_ctas(a.rows, L::kRows, L::kThreads);
-  norm_backward_kernel<T, L, BRANCH><<<ctas, L::kThreads, 0, stream>>>(a);
+  const int ctas = (int)backward_ctas(a.rows, L::kRows, L::kPerSm);
+  constexpr bool kRing = BRANCH && L::V * sizeof(T) == 16 && RingRows<T, L, 5>::kSlots > 0;
+  const auto kernel = norm_backward_kernel<T, L, BRANCH, kRing>;
+  constexpr int bytes = kRing ? RingRows<T, L, 5>::kSlots * RingRows<T, L, 5>::kSlotBytes : 0;
+  if (bytes && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+                   cudaSuccess)
+    return SEMICRF_ERR_CUDA;
+  kernel<<<ctas, L::kThreads, bytes, stream>>>(a);
   const int first = BRANCH ? 0 : 1;
-  const dim3 grid((unsigned)((a.D + 31) / 32), 2 - first);
-  norm_reduce_kernel<<<grid, dim3(32, 32), 0, stream>>>(a.D, first, ctas, a.w1, a.s, a.partial,
+  const dim3 grid((unsigned)((a.D + 7) / 8), 2 - first);
+  norm_reduce_kernel<<<grid, 256, 0, stream>>>(a.D, first, ctas, a.w1, a.s, a.partial,
                                                         grad_weights);
   return launch_status();
 }
@@ -419,7 +560,9 @@ int launch_width(const NormArgs<T>& a, bool backward, float* gw, cudaStream_t s)
   if (a.D > 4096) return launch<T, Layout<T, V, 16, 16>, BRANCH>(a, backward, gw, s);
   if constexpr (V * sizeof(T) == 16 && sizeof(T) == 2) {
     if (a.D <= 512) return launch<T, Layout<T, V, 1, 16>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 768) return launch<T, Layout<T, V, 3, 8>, BRANCH>(a, backward, gw, s);
     if (a.D <= 1024) return launch<T, Layout<T, V, 2, 16>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 1536) return launch<T, Layout<T, V, 3, 16>, BRANCH>(a, backward, gw, s);
     if (a.D <= 2048) return launch<T, Layout<T, V, 4, 16>, BRANCH>(a, backward, gw, s);
     return launch<T, Layout<T, V, 8, 16>, BRANCH>(a, backward, gw, s);
   } else {
@@ -481,7 +624,7 @@ int run_backward(const semicrf_block_norm* p, const float* stats, const semicrf_
 
 size_t block_norm_workspace_bytes(const semicrf_block_norm* p) {
   // the most CTAs that any layout launches
-  return sizeof(float) * 2 * p->D * backward_ctas(p->batch * p->T, 1, 128);
+  return sizeof(float) * 2 * p->D * backward_ctas(p->batch * p->T, 1, 6);
 }
 
 int block_norm_forward(const semicrf_block_norm* p, const semicrf_sequence& r,

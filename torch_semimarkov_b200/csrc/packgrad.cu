@@ -744,12 +744,14 @@ template <int CG>
 int launch_bulk(const GradArgs& a, int runs, cudaStream_t stream) {
   const auto kernel = weight_grad_bulk_kernel<CG>;
   CUtensorMap dy, codes;
-  if (!make_map(&dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.dy, a.M, a.N, a.st * 2, 64,
+  // the runtime's call comes first: it gives a thread that has none yet the
+  // device's context, which encoding a map needs
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkBytes) !=
+          cudaSuccess ||
+      !make_map(&dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.dy, a.M, a.N, a.st * 2, 64,
                 CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_map(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.Dp, a.N, a.Dp, kTile,
-                CU_TENSOR_MAP_SWIZZLE_NONE) ||
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkBytes) !=
-          cudaSuccess)
+                CU_TENSOR_MAP_SWIZZLE_NONE))
     return SEMICRF_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.tiles_m * a.tiles_d), (unsigned)runs);

@@ -1017,9 +1017,11 @@ int run_forward(const semicrf_recurrence* p, const semicrf_sequence& h, float* f
     const auto walk = forward_bulk_kernel<T, false>;
     const auto compose = forward_bulk_kernel<T, true>;
     constexpr int bytes = ring_bytes(sizeof(T), forward_pairs<T>(), 2, kForwardStages);
-    if (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, L) ||
-        !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, L) || !allow_shared(walk, bytes) ||
-        !allow_shared(compose, bytes))
+    // the runtime's calls come first: they give a thread that has none yet the
+    // device's context, which encoding a map needs
+    if (!allow_shared(walk, bytes) || !allow_shared(compose, bytes) ||
+        !sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, L) ||
+        !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, L))
       return SEMICRF_ERR_CUDA;
     const unsigned grid = (unsigned)(a.B * a.tiles * a.segments);
     if (a.segments > 1) compose<<<grid, 32 * kWarps + 32, bytes, stream>>>(a, xm, gm);
@@ -1056,10 +1058,10 @@ int run_backward(const semicrf_recurrence* p, const void* saved, const semicrf_s
     const auto compose = backward_compose_kernel<T>;
     constexpr int walk_bytes = ring_bytes(sizeof(T), kBackwardPairs, 3, backward_stages<T>());
     constexpr int compose_bytes = ring_bytes(sizeof(T), kBackwardPairs, 2, backward_stages<T>());
-    if (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, BL) ||
+    if (!allow_shared(walk, walk_bytes) || !allow_shared(compose, compose_bytes) ||
+        !sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, BL) ||
         !sequence_map<T>(&gm, p->gate, a.B, a.T_, a.D, BL) ||
-        !sequence_map<T>(&dm, grad_h, a.B, a.T_, a.D, BL) || !allow_shared(walk, walk_bytes) ||
-        !allow_shared(compose, compose_bytes))
+        !sequence_map<T>(&dm, grad_h, a.B, a.T_, a.D, BL))
       return SEMICRF_ERR_CUDA;
     const unsigned grid = (unsigned)(a.B * a.tiles * a.segments);
     if (a.segments > 1) compose<<<grid, 32 * kWarps + 32, compose_bytes, stream>>>(a, dm, gm);

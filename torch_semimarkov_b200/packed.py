@@ -12,7 +12,6 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -59,7 +58,6 @@ def _check(p: PackedActivation):
                            "activation is on the CPU)")
 
 
-@torch.no_grad()
 def pack_activation(x: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> PackedActivation:
     """Store x (batch, T, channels) in 8 bits.  Positions past a sequence's
     length are stored as zeros, whatever they hold."""
@@ -69,7 +67,6 @@ def pack_activation(x: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> 
     return PackedActivation(codes, scales, x.shape[2], x.dtype)
 
 
-@torch.no_grad()
 def packed_weight_grad(grad_output: torch.Tensor, packed: PackedActivation,
                        lengths: Optional[torch.Tensor] = None,
                        dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -102,7 +99,7 @@ class _PackedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, grad):
         weight, codes, scales, lengths = ctx.saved_tensors
         grad = _lib.activation(grad, "grad_output")

@@ -13,7 +13,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -33,7 +32,7 @@ class _GatedLinearRecurrence(torch.autograd.Function):
         return h, state
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, grad_h, grad_state):
         x, gate, lengths, saved = ctx.saved_tensors
         if grad_h is not None:
@@ -87,7 +86,6 @@ def gated_linear_recurrence(
     return h, state
 
 
-@torch.no_grad()
 def gated_linear_recurrence_step(
     x: torch.Tensor,
     gate: torch.Tensor,
