@@ -17,16 +17,13 @@
 // tile takes a run of positions; the runs' partial results are summed in
 // order by a second kernel.
 //
-// Roles: producer warps fill a ring of stages of 64 positions, dy by 16-byte
-// asynchronous copies straight into the swizzled tile (bfloat16 rows on
-// 16-byte boundaries) or through registers, codes through registers; both
-// are requested kLook stages before they are needed.  One thread issues the
-// products.  The tensor cores truncate their float32 sums (measured: 1.8e-8
-// of the result for each 16 positions), which is nothing beside 16-bit dy.
-// For float32 the leading piece is summed apart from the others and, every
-// 512 positions, moved from tensor memory to registers that round to nearest.
+// The tensor cores truncate their float32 sums (measured: 1.8e-8 of the result
+// for each 16 positions), which is nothing beside 16-bit dy.  For float32 the
+// leading piece is summed apart from the others and, every 512 positions,
+// moved from tensor memory to registers that round to nearest.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "encoder_internal.cuh"
 #include "tma.cuh"
@@ -40,22 +37,31 @@ constexpr int kTile = 128;      // channels of dy, and of x, that a CTA brings
 constexpr int kStep = 64;       // positions of a stage
 constexpr int kAtom = kStep * 128;  // bytes of 64 channels of a stage: 64 rows of 128
 constexpr int kOperand = 2 * kAtom; // bytes of an operand of a stage
-constexpr int kWarps = 16;      // producers and readers of tensor memory; one more issues
-constexpr int kSegment = 8;     // float32: stages that tensor memory sums
+constexpr int kReaders = 16;    // bulk form: warps that read tensor memory
+constexpr int kGroupWarps = 4;  // warps that produce a stage together
 
 template <class T>
-struct Form;  // pieces of a value; producer warps; warps that read tensor memory
+struct Form;  // pieces of a value; positions of a stage; warps that produce, that read tensor
+              // memory, and both (one more issues)
 template <>
-struct Form<__nv_bfloat16> { static constexpr int pieces = 1, producers = 16, readers = 16; };
+struct Form<__nv_bfloat16> {
+  static constexpr int pieces = 1, step = 32, producers = 16, readers = 16, warps = 16;
+};
 template <>
-struct Form<__half> { static constexpr int pieces = 2, producers = 16, readers = 16; };
+struct Form<__half> {
+  static constexpr int pieces = 2, step = 32, producers = 16, readers = 16, warps = 16;
+};
 template <>
-struct Form<float> { static constexpr int pieces = 3, producers = 8, readers = 8; };
+struct Form<float> {
+  static constexpr int pieces = 3, step = 32, producers = 8, readers = 8, warps = 16;
+};
 
 template <class T>
 struct Shape {
+  static constexpr int kAtom = Form<T>::step * 128;
+  static constexpr int kOperand = 2 * kAtom;
   static constexpr int kStage = (Form<T>::pieces + 1) * kOperand;
-  static constexpr int kStages = 200 * 1024 / kStage < 6 ? 200 * 1024 / kStage : 6;
+  static constexpr int kStages = 200 * 1024 / kStage < 8 ? 200 * 1024 / kStage : 8;
   static constexpr int kBytes = kStages * kStage + 1024;  // and room to align
 };
 
@@ -65,6 +71,7 @@ struct GradArgs {
   const void* dy;
   int64_t sb, st;
   bool vec;             // rows of dy start on 16-byte boundaries
+  bool flat;            // position n of all sequences lies n * st from the first
   const int8_t* codes;
   const uint8_t* scales;
   const int64_t* lengths;
@@ -146,36 +153,67 @@ __device__ __forceinline__ void read_columns(unsigned at, float (&f)[16]) {
   for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(v[k]);
 }
 // Shared-memory operand, MN-major, 128-byte swizzle: 64 channels are one row
-// of 128 bytes, 8 positions 1024 bytes, the next 64 channels kAtom further.
-__device__ __forceinline__ uint64_t operand(unsigned addr) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(kAtom >> 4) << 16) |
+// of 128 bytes, 8 positions 1024 bytes, the next 64 channels `atom` further.
+__device__ __forceinline__ uint64_t operand(unsigned addr, int atom) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(atom >> 4) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// One value's pieces: each the leading 8 bits of what is left, by truncation,
-// so no piece overflows and the last leaves nothing.
-template <int NP>
-__device__ __forceinline__ void cut(float v, unsigned short (&piece)[NP]) {
+// Eight values' pieces, two to a word: each the leading 8 bits of what is
+// left, by truncation, so no piece overflows and the last leaves nothing.  An
+// infinity has itself and zeros (what is left of it is NaN, whose larger
+// partner 0 is taken); a NaN is made to show in the leading piece.
+template <int NP, class T>
+__device__ __forceinline__ void cut(const Pack<T, 8>& v, uint4 (&piece)[NP]) {
+  if constexpr (NP == 1) {
+    piece[0] = *reinterpret_cast<const uint4*>(&v);
+  } else {
 #pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const unsigned bits = __float_as_uint(v) & 0xffff0000u;
-    piece[k] = (unsigned short)(bits >> 16);
-    v = isinf(v) ? 0.f : v - __uint_as_float(bits);
+    for (int k = 0; k < 4; ++k) {
+      unsigned rest[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float f = to_f32(v.v[2 * k + h]);
+        if (NP == 3) f += 0.f;  // any NaN to the one whose leading bits are set
+        rest[h] = __float_as_uint(f);
+      }
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const unsigned w = __byte_perm(rest[0], rest[1], 0x7632);
+        (&piece[j].x)[k] = w;
+        if (j + 1 < NP)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float f = __uint_as_float(rest[h]);
+            const float left = fmaxf(fabsf(f - __uint_as_float(rest[h] & 0xffff0000u)), 0.f);
+            rest[h] = __float_as_uint(left) | (rest[h] & 0x80000000u);
+          }
+      }
+    }
   }
 }
 
-template <class T, int CG, bool ASYNC>
-__global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const GradArgs a) {
+// dy of any type, stride and alignment, through registers.  Groups of four
+// warps take the stages in turn.  A group publishes a stage, then requests the
+// one it takes next, whose loads arrive while the other groups' stages are
+// worked off.  (A fence before publishing waits for every load in flight, so a
+// warp must not have any of its own then.)  A group waits for the products of
+// the stage that used its slot before; products are done in order and there
+// are no more groups than slots, so that wait is never more than one phase
+// ahead of its barrier.
+template <class T, int CG>
+__global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kernel(const GradArgs a) {
   using F = Form<T>;
   using S = Shape<T>;
-  constexpr int NP = F::pieces, NS = S::kStages;
-  constexpr int kRowsPass = 2 * F::producers, kPasses = kStep / kRowsPass;
-  constexpr int kLook = ASYNC ? 3 : 1;  // stages requested ahead
+  constexpr int NP = F::pieces, NS = S::kStages, STEP = F::step, W = F::warps;
+  constexpr int kGroups = F::producers / kGroupWarps, kPart = 32 * kGroupWarps;
+  constexpr int kPasses = STEP / 8;     // 16 threads a row, 8 rows at once
+  constexpr int kSegment = 512 / STEP;  // float32: stages that tensor memory sums
   constexpr bool kApart = NP == 3;      // float32: segments, lower pieces apart
   constexpr int kCols = kTile * CG;     // columns of the accumulator
   constexpr int kTmem = kApart ? 512 : kCols;
   static_assert(!kApart || CG == 1, "tensor memory holds two segments and the lower pieces");
-  static_assert(kLook < NS, "a requested stage must not wait for an unpublished one");
+  static_assert(kGroups <= NS, "see above");
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[NS], empty[NS], ready[2], taken[2];
   __shared__ unsigned tmem_at;
@@ -188,11 +226,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
   const int64_t first = blockIdx.y * a.run;
   const int64_t left = a.N - first;
   const int count = (int)(left < a.run ? (left < 0 ? 0 : left) : a.run);
-  const int steps = (count + kStep - 1) / kStep;
+  const int steps = (count + STEP - 1) / STEP;
 
   if (tid == 0) {
     for (int s = 0; s < NS; ++s) {
-      barrier_init(&full[s], F::producers * CG);
+      barrier_init(&full[s], kGroupWarps * CG);
       barrier_init(&empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -201,7 +239,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kWarps) {
+  if (warp == W) {
     if (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                        smem_addr(&tmem_at)),
@@ -225,123 +263,120 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
   bool ok = true;
   if (warp < F::producers) {
     // this thread's 8 channels of dy and of x, and its first row of a stage
-    const int col = tid & 15, row0 = tid >> 4;
+    const int group = tid / kPart, col = tid & 15, row0 = tid % kPart >> 4;
     const int64_t m = (int64_t)tm * kTile + col * 8;
     const int64_t d = ((int64_t)td * CG + rank) * kTile + col * 8;
     const bool has_m = m < a.M, has_d = d < a.Dp;
     const unsigned width = !has_m ? 0u : (unsigned)(a.M - m < 8 ? a.M - m : 8);
-    // where its 16-byte piece of a row lies; later passes are a multiple of 8 rows on
-    const unsigned dst = (unsigned)(col >> 3) * kAtom + (unsigned)((col & 7) ^ (row0 & 7)) * 16 +
+    // where its 16-byte piece of a row lies; later passes are 8 rows on
+    const unsigned dst = (unsigned)(col >> 3) * S::kAtom + (unsigned)((col & 7) ^ row0) * 16 +
                          (unsigned)row0 * 128;
-    const T* dy = static_cast<const T*>(a.dy) + (has_m ? m : 0);
-    const int8_t* codes = a.codes + (first + row0) * a.Dp + (has_d ? d : 0);
-    const uint8_t* scales = a.scales + (first + row0) * a.G + (has_d ? d / kPackGroup : 0);
-    // the sequence and position of row0 of the stage that is requested next
-    int64_t b = (first + row0) / a.T_;
-    unsigned t = (unsigned)(first + row0 - b * a.T_);
-
-    struct Held {
+    const int64_t start = first + group * STEP + row0;
+    const T* const dy0 = static_cast<const T*>(a.dy) + (has_m ? m : 0);
+    const int8_t* const codes0 = a.codes + (has_d ? d : 0);
+    const uint8_t* const scales0 = a.scales + (has_d ? d / kPackGroup : 0);
+    // the row of pass 0 of the stage that is requested next: in the tensors
+    // (dy where its positions are at one distance), and its sequence and position
+    const T* dy = dy0 + start * a.st;
+    const int8_t* codes = codes0 + start * a.Dp;
+    const uint8_t* scales = scales0 + start * a.G;
+    const bool placed = a.lengths || !a.flat;
+    int64_t b = placed ? start / a.T_ : 0;
+    unsigned t = (unsigned)(start - b * a.T_);
+    // WIDE: every row holds whole 16-byte pieces.  Else values are loaded, and
+    // held, one by one: packing them is work for when they have arrived.
+    const auto produce = [&](auto kind) {
+      constexpr bool kWide = decltype(kind)::value;
+      struct Values {
+        Pack<T, 8> whole;
+        T single[8];
+      } v[kPasses];
       uint2 q[kPasses];
-      uint8_t byte[kPasses];
-      Pack<T, 8> v[ASYNC ? 1 : kPasses];
-    } held[kLook];
-
-    const auto request = [&](int j, Held& h) {
-      if (j < steps) {
-        const int slot = j % NS;
-        if (j >= NS) {
-          ok = __all_sync(~0u, barrier_wait(&empty[slot], (unsigned)(j / NS - 1) & 1));
-          if (!ok) return;
-        }
+      unsigned byte[kPasses];
+      unsigned valid = 0;  // bit p: the row of pass p counts
+      const auto request = [&](int it) {
+        valid = 0;
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
-          unsigned tt = t + p * kRowsPass;
-          int64_t bb = b;
-          if (tt >= a.T_) {
-            const unsigned q = quotient(tt, a.by_t);
-            bb += q;
-            tt -= q * a.T_;
+          bool live = it * STEP + row0 + p * 8 < count;
+          const T* src = dy + p * 8 * a.st;
+          if (placed) {
+            unsigned tt = t + p * 8;
+            int64_t bb = b;
+            if (tt >= a.T_) {
+              const unsigned k = quotient(tt, a.by_t);
+              bb += k;
+              tt -= k * a.T_;
+            }
+            live = live && (!a.lengths || (int64_t)tt < a.lengths[bb]);
+            if (!a.flat) src = dy0 + bb * a.sb + (int64_t)tt * a.st;
           }
-          const bool live = j * kStep + row0 + p * kRowsPass < count &&
-                            (!a.lengths || (int64_t)tt < a.lengths[bb]);
-          const T* src = dy + bb * a.sb + (int64_t)tt * a.st;
-          if (ASYNC) {
-            const unsigned bytes = live ? 2 * width : 0u;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                             smem_addr(ring + slot * S::kStage + dst + p * kRowsPass * 128)),
-                         "l"(bytes ? src : static_cast<const T*>(a.dy)), "r"(bytes)
-                         : "memory");
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) h.v[p].v[k] = from_f32<T>(0.f);
-            if (live && a.vec && width == 8) {
-              constexpr int V = 16 / sizeof(T);
+          if (!live) continue;
+          valid |= 1u << p;
+          if (kWide) {
+            constexpr int V = 16 / sizeof(T);
+            if (has_m)
 #pragma unroll
               for (int k = 0; k < 8; k += V)
-                *reinterpret_cast<Pack<T, V>*>(&h.v[p].v[k]) =
+                *reinterpret_cast<Pack<T, V>*>(&v[p].whole.v[k]) =
                     *reinterpret_cast<const Pack<T, V>*>(src + k);
-            } else if (live) {
+          } else {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (k < width) h.v[p].v[k] = src[k];
-            }
+            for (int k = 0; k < 8; ++k)
+              if (k < width) v[p].single[k] = src[k];
           }
-          h.q[p] = make_uint2(0, 0);
-          h.byte[p] = 0;
-          if (live && has_d) {
-            h.q[p] = *reinterpret_cast<const uint2*>(codes + p * kRowsPass * a.Dp);
-            h.byte[p] = scales[p * kRowsPass * a.G];
+          if (has_d) {
+            q[p] = *reinterpret_cast<const uint2*>(codes + p * 8 * a.Dp);
+            byte[p] = scales[p * 8 * a.G];
           }
         }
-        codes += kStep * a.Dp;
-        scales += kStep * a.G;
-        t += kStep;
-        if (t >= a.T_) {
-          const unsigned q = quotient(t, a.by_t);
-          b += q;
-          t -= q * a.T_;
+        dy += kGroups * STEP * a.st;
+        codes += kGroups * STEP * a.Dp;
+        scales += kGroups * STEP * a.G;
+        t += kGroups * STEP;
+        if (placed && t >= a.T_) {
+          const unsigned k = quotient(t, a.by_t);
+          b += k;
+          t -= k * a.T_;
         }
+      };
+      if (group < steps) request(group);
+      for (int it = group; it < steps; it += kGroups) {
+        const int slot = it % NS;
+        if (it >= NS) {
+          ok = __all_sync(~0u, barrier_wait(&empty[slot], (unsigned)(it / NS - 1) & 1));
+          if (!ok) break;
+        }
+        unsigned char* base = ring + slot * S::kStage + dst;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          unsigned char* at = base + p * 8 * 128;
+          const bool live = valid >> p & 1;
+          if (!kWide)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              v[p].whole.v[k] = k < width ? v[p].single[k] : from_f32<T>(0.f);
+          uint4 piece[NP];
+          cut<NP>(v[p].whole, piece);
+#pragma unroll
+          for (int j = 0; j < NP; ++j)
+            *reinterpret_cast<uint4*>(at + j * S::kOperand) =
+                live && has_m ? piece[j] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(at + NP * S::kOperand) =
+              live && has_d ? pack_decode(q[p], (uint8_t)byte[p]) : make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) barrier_arrive<CG>(&full[slot]);
+        if (it + kGroups < steps) request(it + kGroups);
       }
-      if (ASYNC) asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const auto publish = [&](int it, Held& h) {
-      unsigned char* base = ring + it % NS * S::kStage + dst;
-#pragma unroll
-      for (int p = 0; p < kPasses; ++p) {
-        unsigned char* at = base + p * kRowsPass * 128;
-        if (!ASYNC) {
-          unsigned short piece[8][NP];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) cut<NP>(to_f32(h.v[p].v[k]), piece[k]);
-#pragma unroll
-          for (int j = 0; j < NP; ++j) {
-            unsigned w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = (unsigned)piece[2 * k][j] | ((unsigned)piece[2 * k + 1][j] << 16);
-            *reinterpret_cast<uint4*>(at + j * kOperand) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        *reinterpret_cast<uint4*>(at + NP * kOperand) = pack_decode(h.q[p], h.byte[p]);
-      }
-      if (ASYNC) asm volatile("cp.async.wait_group %0;" ::"n"(kLook - 1) : "memory");
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) barrier_arrive<CG>(&full[it % NS]);
-    };
-
-#pragma unroll
-    for (int u = 0; u < kLook; ++u) request(u, held[u]);
-    for (int it = 0; it < steps && ok; it += kLook)
-#pragma unroll
-      for (int u = 0; u < kLook; ++u)
-        if (it + u < steps && ok) {
-          publish(it + u, held[u]);
-          request(it + u + kLook, held[u]);
-        }
-    if (ASYNC) asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == kWarps && lane == 0 && rank == 0) {
-    for (int it = 0; it < steps && ok; ++it) {
+    if (a.vec && a.M % 8 == 0)
+      produce(std::true_type());
+    else
+      produce(std::false_type());
+  } else if (warp == W && lane == 0 && rank == 0) {
+    for (int it = 0; it < steps; ++it) {
       const int slot = it % NS, segment = it / kSegment, buffer = kApart ? segment & 1 : 0;
       const bool opens = kApart ? it % kSegment == 0 : it == 0;
       if (kApart && opens && segment >= 2)
@@ -351,11 +386,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned at = smem_addr(ring + slot * S::kStage);
 #pragma unroll
-      for (int k = 0; k < kStep / 16; ++k) {
-        const uint64_t bd = operand(at + NP * kOperand + k * 2048);
+      for (int k = 0; k < STEP / 16; ++k) {
+        const uint64_t bd = operand(at + NP * S::kOperand + k * 2048, S::kAtom);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-          const uint64_t ad = operand(at + j * kOperand + k * 2048);
+          const uint64_t ad = operand(at + j * S::kOperand + k * 2048, S::kAtom);
           if (kApart)
             product<CG>(tmem + (j ? 2 * kCols : buffer * kCols), ad, bd,
                         j ? it > 0 || k > 0 || j > 1 : !opens || k > 0);
@@ -372,10 +407,10 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
 
   // Tensor memory to the partial result: a warp reads its 32 lanes (rows of
   // the tile) and a share of the columns; a column's rows are contiguous.
-  if (warp >= kWarps - F::readers && warp < kWarps) {
+  if (warp >= W - F::readers && warp < W) {
     constexpr int kShare = kCols / (F::readers / 4);
     static_assert(kShare % 16 == 0, "a warp reads 16 columns at once");
-    const int quarter = warp & 3, c0 = (warp - (kWarps - F::readers)) / 4 * kShare;
+    const int quarter = warp & 3, c0 = (warp - (W - F::readers)) / 4 * kShare;
     const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
     float sum[kShare];
 #pragma unroll
@@ -415,7 +450,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (CG > 1) sync_all<CG>();
-  if (warp == kWarps) {
+  if (warp == W) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (CG == 1)
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem));
@@ -439,7 +474,6 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 1) weight_grad_kernel(const 
 // dy's arrival to it.
 // ---------------------------------------------------------------------------
 constexpr int kGroups = 5;                   // decoding groups and slots of the operand ring
-constexpr int kGroupWarps = 4;
 constexpr int kDecoders = kGroups * kGroupWarps;
 constexpr int kCodeSlots = 7;
 constexpr int kCodes = kStep * kTile;        // bytes of a stage's codes
@@ -576,7 +610,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned at = smem_addr(ring + slot * 2 * kOperand);
-        const uint64_t ad = operand(at), bd = operand(at + kOperand);
+        const uint64_t ad = operand(at, kAtom), bd = operand(at + kOperand, kAtom);
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k)  // 16 positions are 2048 bytes
           product<CG>(tmem, ad + k * (2048 >> 4), bd + k * (2048 >> 4), it > 0 || k > 0);
@@ -631,8 +665,8 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
   }
   __syncwarp();
 
-  if (warp < kWarps) {
-    constexpr int kShare = kCols / 4;
+  if (warp < kReaders) {
+    constexpr int kShare = kCols / (kReaders / 4);
     const int quarter = warp & 3, c0 = (warp >> 2) * kShare;
     const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
     const bool good = !steps || __all_sync(~0u, barrier_wait(&ready, 0));
@@ -710,16 +744,16 @@ Plan plan(int64_t N, int64_t D, int64_t M, int dtype) {
   return p;
 }
 
-template <class T, int CG, bool ASYNC>
+template <class T, int CG>
 int launch(const GradArgs& a, int runs, cudaStream_t stream) {
-  const auto kernel = weight_grad_kernel<T, CG, ASYNC>;
+  const auto kernel = weight_grad_kernel<T, CG>;
   constexpr int bytes = Shape<T>::kBytes;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
       cudaSuccess)
     return SEMICRF_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.tiles_m * a.tiles_d), (unsigned)runs);
-  cfg.blockDim = dim3(32 * kWarps + 32);
+  cfg.blockDim = dim3(32 * Form<T>::warps + 32);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -768,10 +802,9 @@ int launch_bulk(const GradArgs& a, int runs, cudaStream_t stream) {
                                                                        : SEMICRF_ERR_CUDA;
 }
 
-template <class T, bool ASYNC>
+template <class T>
 int launch_group(const GradArgs& a, const Plan& p, cudaStream_t stream) {
-  return p.group == 2 ? launch<T, 2, ASYNC>(a, p.runs, stream)
-                      : launch<T, 1, ASYNC>(a, p.runs, stream);
+  return p.group == 2 ? launch<T, 2>(a, p.runs, stream) : launch<T, 1>(a, p.runs, stream);
 }
 
 }  // namespace
@@ -800,29 +833,27 @@ int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
   a.codes = codes;
   a.scales = scales;
   a.vec = seq_aligned(dy, B, T, dtype == SEMICRF_F32 ? 4 : 2, dtype == SEMICRF_F32 ? 4 : 8);
+  a.flat = B == 1 || T == 1 || a.sb == T * a.st;
   a.lengths = lengths;
   a.T_ = (unsigned)std::max<int64_t>(T, 1);
   a.by_t = make_divider(a.T_);
   a.tiles_m = p.tiles_m;
   a.tiles_d = p.tiles_d;
   a.partial = static_cast<float*>(workspace);
-  // the distance between positions where it is one and the same
-  const int64_t row = T > 1 ? a.st : B > 1 ? a.sb : (M + 7) / 8 * 8;
+  if (a.flat) a.st = T > 1 ? a.st : B > 1 ? a.sb : (M + 7) / 8 * 8;
   int st;
   switch (dtype) {
-    case SEMICRF_F32: st = launch<float, 1, false>(a, p.runs, stream); break;
+    case SEMICRF_F32: st = launch<float, 1>(a, p.runs, stream); break;
     case SEMICRF_BF16:
       // bulk copies want aligned rows at one distance, and a row index in 31 bits
       if (a.vec && a.N && a.N < (1ll << 31) - kStep && reinterpret_cast<uintptr_t>(codes) % 16 == 0 &&
-          (B == 1 || T == 1 || a.sb == T * a.st) && row >= M && row < (1ll << 36)) {
-        a.st = row;
+          a.flat && a.st >= M && a.st < (1ll << 36)) {
         st = p.group == 2 ? launch_bulk<2>(a, p.runs, stream) : launch_bulk<1>(a, p.runs, stream);
       } else {
-        st = a.vec ? launch_group<__nv_bfloat16, true>(a, p, stream)
-                   : launch_group<__nv_bfloat16, false>(a, p, stream);
+        st = launch_group<__nv_bfloat16>(a, p, stream);
       }
       break;
-    default: st = launch_group<__half, false>(a, p, stream);
+    default: st = launch_group<__half>(a, p, stream);
   }
   if (st != SEMICRF_OK) return st;
   const dim3 grid((unsigned)((M + 31) / 32), (unsigned)((D + 31) / 32));
