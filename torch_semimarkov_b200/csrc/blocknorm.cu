@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArg
       if (BRANCH) {
         float2 sig, neg;
         const float2 g = in.pair(kG, i);
-        sigmoid_pair2(g, sig, neg);
+        sigmoid_pair2<T>(g, sig, neg);
         const float2 u = __fmul2_rn(__fmul2_rn(g, sig), weight.sw(i));
         r[i] = __ffma2_rn(u, __fmul2_rn(in.pair(kZ, i), both(rz)), r[i]);
       }
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_backward_kernel(c
       if (BRANCH) {
         float2 neg;
         const float2 g = in.pair(kG, i);
-        sigmoid_pair2(g, sig[i], neg);
+        sigmoid_pair2<T>(g, sig[i], neg);
         rh[i] = __ffma2_rn(__fmul2_rn(__fmul2_rn(g, sig[i]), weight.sw(i)),
                            __fmul2_rn(in.pair(kZ, i), rz), rh[i]);
       }

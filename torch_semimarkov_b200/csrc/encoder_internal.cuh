@@ -99,17 +99,28 @@ __device__ __forceinline__ int64_t valid_length(const int64_t* lengths, int64_t 
   return n < 0 ? 0 : (n > T ? T : n);
 }
 
-// sigmoid(g) and sigmoid(-g), each to two units of its own last place: with
-// e = exp(-g) they are 1 / (1 + e) and e / (1 + e), so neither cancels.  e is
-// held to 2^126, where the first is 2^-126; a NaN stays one.  Six operations,
-// two of them special functions.
-__device__ __forceinline__ void sigmoid_pair(float g, float& pos, float& neg) {
+// sigmoid(g) and sigmoid(-g): with e = exp(-g) they are 1 / (1 + e) and
+// e / (1 + e), so neither cancels.  e is held to 2^126, where the first is
+// 2^-126; a NaN stays one.  Six operations, two of them special functions.
+// Two errors are taken back where they count.  The rounding of g / ln 2 puts e
+// off by |g| 2^-24 of itself: for float32 activations T the remainder is kept
+// and added.  The approximate reciprocal errs to one side, which over the
+// hundreds of positions that a gate near 1 remembers adds up (8e-7 of the
+// state, against 3e-7): in a CHAIN, and for float32, it gets one Newton step.
+constexpr float kInvLn2 = 1.4426950408889634f, kInvLn2Low = 1.925963033500907e-8f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_capped(float t) {
   float e;
   asm("{.reg .f32 t; min.NaN.f32 t, %1, 0f42FC0000; ex2.approx.ftz.f32 %0, t;}"
       : "=f"(e)
-      : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos) : "f"(1.f + e));
-  neg = e * pos;
+      : "f"(t));
+  return e;
+}
+__device__ __forceinline__ float reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 // Two channels at once: products and sums go two to an instruction.
@@ -117,20 +128,38 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 sub2(float2 a, float2 b) {
   return __ffma2_rn(b, make_float2(-1.f, -1.f), a);  // exactly a - b rounded once
 }
+template <class T, bool CHAIN = false>
 __device__ __forceinline__ void sigmoid_pair2(float2 g, float2& pos, float2& neg) {
-  const float2 t = __fmul2_rn(g, both(-1.4426950408889634f));
-  float2 e;
-  asm("{.reg .f32 t; min.NaN.f32 t, %1, 0f42FC0000; ex2.approx.ftz.f32 %0, t;}"
-      : "=f"(e.x)
-      : "f"(t.x));
-  asm("{.reg .f32 t; min.NaN.f32 t, %1, 0f42FC0000; ex2.approx.ftz.f32 %0, t;}"
-      : "=f"(e.y)
-      : "f"(t.y));
+  const float2 t = __fmul2_rn(g, both(-kInvLn2));
+  float2 e = make_float2(exp2_capped(t.x), exp2_capped(t.y));
+  if (sizeof(T) == 4) {
+    float2 rest = __ffma2_rn(g, both(-kInvLn2), make_float2(-t.x, -t.y));
+    rest = __ffma2_rn(g, both(-kInvLn2Low), rest);
+    // past |t| = 128 e is 0 or held, and the remainder of an infinite g is NaN
+    rest.x = fabsf(t.x) < 128.f ? rest.x * kLn2 : 0.f;
+    rest.y = fabsf(t.y) < 128.f ? rest.y * kLn2 : 0.f;
+    e = __ffma2_rn(e, rest, e);
+  }
   const float2 d = __fadd2_rn(e, both(1.f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos.x) : "f"(d.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(pos.y) : "f"(d.y));
+  pos = make_float2(reciprocal(d.x), reciprocal(d.y));
+  if (CHAIN || sizeof(T) == 4)
+    pos = __ffma2_rn(pos, __ffma2_rn(make_float2(-d.x, -d.y), pos, both(1.f)), pos);
   neg = __fmul2_rn(e, pos);
 }
+template <class T, bool CHAIN = false>
+__device__ __forceinline__ void sigmoid_pair(float g, float& pos, float& neg) {
+  const float t = g * -kInvLn2;
+  float e = exp2_capped(t);
+  if (sizeof(T) == 4) {
+    const float rest = fmaf(g, -kInvLn2Low, fmaf(g, -kInvLn2, -t));
+    e = fmaf(e, fabsf(t) < 128.f ? rest * kLn2 : 0.f, e);
+  }
+  const float d = 1.f + e;
+  pos = reciprocal(d);
+  if (CHAIN || sizeof(T) == 4) pos = fmaf(pos, fmaf(-d, pos, 1.f), pos);
+  neg = e * pos;
+}
+
 template <class T>
 __device__ __forceinline__ float2 to_f32x2(const Pack<T, 2>& v) {
   return make_float2(to_f32(v.v[0]), to_f32(v.v[1]));

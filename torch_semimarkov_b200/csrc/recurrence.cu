@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(32 * kWarps) compose_kernel(const ScanArgs<T> 
 #pragma unroll
       for (int j = 0; j < L; ++j) {
         float n;
-        sigmoid_pair(to_f32(g[i].v[j]), f[i][j], n);
+        sigmoid_pair<T, true>(to_f32(g[i].v[j]), f[i][j], n);
         s[i][j] = BWD ? to_f32(v[i].v[j]) : n * to_f32(v[i].v[j]);
         if (!live) f[i][j] = 1.f, s[i][j] = 0.f;
       }
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) forward_kernel(const ScanArgs<
 #pragma unroll
       for (int j = 0; j < L; ++j) {
         float n;
-        sigmoid_pair(to_f32(g[i].v[j]), f[i][j], n);
+        sigmoid_pair<T, true>(to_f32(g[i].v[j]), f[i][j], n);
         s[i][j] = n * to_f32(x[i].v[j]);
         if (!live) f[i][j] = 1.f, s[i][j] = 0.f;
       }
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) backward_kernel(const ScanArgs
       const bool live = whole || t < at.len;
 #pragma unroll
       for (int j = 0; j < L; ++j) {
-        sigmoid_pair(to_f32(gq[i].v[j]), f[i][j], n[i][j]);
+        sigmoid_pair<T, true>(to_f32(gq[i].v[j]), f[i][j], n[i][j]);
         if (!live) f[i][j] = 1.f, n[i][j] = 0.f;
         x[i][j] = to_f32(xq[i].v[j]);
         dh[i][j] = to_f32(dq[i].v[j]);
@@ -431,7 +431,7 @@ __global__ void step_kernel(int64_t B, int64_t D, const T* __restrict__ x, int64
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float f, m;
-      sigmoid_pair(to_f32(gv.v[j]), f, m);
+      sigmoid_pair<T, true>(to_f32(gv.v[j]), f, m);
       o.v[j] = fmaf(f, s.v[j], m * to_f32(xv.v[j]));
       y.v[j] = from_f32<T>(o.v[j]);
     }
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
 #pragma unroll
       for (int j = 0; j < H; ++j) {
         float2 n;
-        sigmoid_pair2(g[j], u[i][j].P, n);
+        sigmoid_pair2<T, true>(g[j], u[i][j].P, n);
         u[i][j].S = __fmul2_rn(n, x[j]);
         if (kMasked && t0 + dir * i >= at.len) u[i][j] = Affine{both(1.f), both(0.f)};
       }
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
 #pragma unroll
       for (int j = 0; j < H; ++j) {
         float2 f, n;
-        sigmoid_pair2(g[j], f, n);
+        sigmoid_pair2<T, true>(g[j], f, n);
         q[j].P = __fmul2_rn(q[j].P, f);
         q[j].S = __fmul2_rn(f, __fadd2_rn(d[j], q[j].S));
       }
@@ -829,7 +829,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 2)
       tile_row<T>(dt, at.w, at.lane, i, a.reverse, d[i]);
 #pragma unroll
       for (int j = 0; j < H; ++j) {
-        sigmoid_pair2(g[j], f[i][j], n[i][j]);
+        sigmoid_pair2<T, true>(g[j], f[i][j], n[i][j]);
         if (off(i)) f[i][j] = both(1.f), n[i][j] = x[i][j] = d[i][j] = both(0.f);
       }
     }
