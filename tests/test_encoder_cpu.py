@@ -154,3 +154,16 @@ def test_reference_checkpoint_step():
     top = codes.abs().amax(-1)
     assert int(top.max()) <= 127 and int(top.min()) >= 63
     assert ((values - x).abs() <= 0.5 * torch.exp2(byte.double() - 127)).all()
+
+
+def test_encoder_arguments():
+    import torch_semimarkov_b200 as tsm
+
+    with pytest.raises(ValueError, match="num_layers"):
+        tsm.GatedRecurrentEncoder(4, 8, num_layers=0)
+    with pytest.raises(ValueError, match="dtype"):
+        tsm.GatedRecurrentEncoder(4, 8, dtype=torch.float64)
+    enc = tsm.GatedRecurrentEncoder(4, 8, num_layers=3)
+    assert len(enc.initial_states(2)) == 3 and enc.initial_states(2)[0].shape == (2, 8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        enc(torch.zeros(1, 3, 4))

@@ -10,7 +10,8 @@ fallback.
 Beside the head, the operators of a gated recurrent encoder in front of it:
 ``gated_linear_recurrence`` (and its one-position ``_step``),
 ``gated_residual_norm`` / ``rms_norm``, and 8-bit activation checkpoints
-(``pack_activation``, ``packed_linear``, ``packed_weight_grad``).
+(``pack_activation``, ``packed_linear``, ``packed_weight_grad``), and
+``GatedRecurrentEncoder``, the encoder made of them.
 """
 
 from .block_norm import gated_residual_norm, rms_norm
@@ -24,6 +25,7 @@ from .duration import (
     UniformDuration,
     create_duration_distribution,
 )
+from .encoder import GatedRecurrentEncoder
 from .helpers import Segment, ViterbiResult, score_gold_vectorized
 from .nn import SemiMarkovCRFHead
 from .packed import PackedActivation, pack_activation, packed_linear, packed_weight_grad
@@ -63,6 +65,7 @@ __all__ = [
     "NEG_INF",
     "UncertaintyMixin",
     "UncertaintySemiMarkovCRFHead",
+    "GatedRecurrentEncoder",
     "gated_linear_recurrence",
     "gated_linear_recurrence_step",
     "gated_residual_norm",
