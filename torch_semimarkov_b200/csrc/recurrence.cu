@@ -552,20 +552,19 @@ __global__ void __launch_bounds__(Column<T, 1, BULK>::kThreads, 2)
       if (col.ok[1]) h.y = p[col.channel(col.lane, 1)];
     }
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / STAGES) & 1);
-    const unsigned char *xt = ring.tile(slot, 0), *gt = ring.tile(slot, 1), *dt = ring.tile(slot, 2);
+    const unsigned char* xt = ring.tile(slot, 0);
+    const unsigned char *gt = xt + C::kBox, *dt = gt + C::kBox;
     // the factors and inputs of the run; masked positions have f = 1 and zeros
     float2 f[kRun], n[kRun], x[kRun], d[kRun];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      float2 v[1];
+      float2 g[1], xv[1], dv[1] = {both(0.f)};
       const int r = col.row(a, i);
-      col.load(gt, r, col.shift(a.g, r), v);
-      sigmoid_pair2<T, true>(v[0], f[i], n[i]);
-      col.load(xt, r, col.shift(a.x, r), v);
-      x[i] = v[0];
-      v[0] = both(0.f);
-      if (BULK || a.dh.p) col.load(dt, r, col.shift(a.dh, r), v);
-      d[i] = v[0];
+      col.load(gt, r, col.shift(a.g, r), g);
+      col.load(xt, r, col.shift(a.x, r), xv);
+      if (BULK || a.dh.p) col.load(dt, r, col.shift(a.dh, r), dv);
+      x[i] = xv[0], d[i] = dv[0];
+      sigmoid_pair2<T, true>(g[0], f[i], n[i]);
       if (off(i)) f[i] = both(1.f), n[i] = x[i] = d[i] = both(0.f);
     }
     ring.release(slot);
@@ -597,7 +596,7 @@ __global__ void __launch_bounds__(Column<T, 1, BULK>::kThreads, 2)
     const int64_t end = t0 + col.row(a, kRun - 1);
     T* xp = col.out(a.dx, end);
     T* gp = col.out(a.dg, end);
-    const int64_t xs = a.reverse ? a.dx.st : -a.dx.st, gs = a.reverse ? a.dg.st : -a.dg.st;
+    const int64_t dir = a.reverse ? -1 : 1;
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i) {
       const float2 lam = __fadd2_rn(d[i], mu);
@@ -608,8 +607,8 @@ __global__ void __launch_bounds__(Column<T, 1, BULK>::kThreads, 2)
         col.store(xp, dx);
         col.store(gp, dg);
       }
-      xp += xs;
-      gp += gs;
+      xp -= dir * a.dx.st;
+      gp -= dir * a.dg.st;
     }
     turn ^= 1;
     if (col.w == 0) enter[turn][col.lane] = mu;
@@ -660,31 +659,45 @@ __global__ void step_kernel(int64_t B, int64_t D, const T* __restrict__ x, int64
 
 int64_t chunks_of(int64_t T) { return (T + kChunk - 1) / kChunk; }
 
-// Chunks in the ring: what lets two CTAs share an SM's 228 KB (1 KB of each is
-// the system's) beside `fixed` bytes of their own, four at most.
-template <class C, int N>
-constexpr int stages_of(int fixed) {
-  return std::min(4, (114 * 1024 - 1024 - 128 - fixed) / (N * C::kBox));
-}
+// Chunks in the ring.  Two keep DRAM busy; a third and fourth, where two CTAs
+// still fit an SM, were slower (backward at batch 64 x 10^4 x 512: 646, 686 and
+// 748 us), since shared memory leaves that much less of the SM to L1.
+constexpr int kStages = 2;
+
 
 struct Cut {
   int tiles, segments;
   int64_t per;
 };
-// Segments: as many as fill the device's CTA slots once.
-Cut cut_of(int64_t B, int64_t T, int64_t D, int tile) {
-  Cut c;
-  c.tiles = (int)((D + tile - 1) / tile);
-  const int64_t columns = B * c.tiles, chunks = chunks_of(T), slots = 2 * device_sm_count();
-  const int64_t want = columns ? std::max<int64_t>(1, std::min(slots / columns, chunks)) : 1;
-  c.per = (chunks + want - 1) / want;
-  c.segments = c.per ? (int)((chunks + c.per - 1) / c.per) : 1;
-  return c;
+// Segments: one, or as many as fill the SMs with one CTA or with two, whichever
+// is the least by this measure: a CTA's chunks, 1.6 times as slow where two
+// share an SM, and with segments `compose` times the walk on top (0.7 forward,
+// 0.35 backward).  Measured at 16 bits, us for one / few / many segments:
+// forward of 128 columns of 4000 positions 99 / - / 136, of 64 columns of
+// 20000 495 / 406 / 315; backward of 64 columns of 40000 - / 733 / 524.
+Cut cut_of(int64_t B, int64_t T, int64_t D, int tile, float compose) {
+  Cut best{};
+  const int64_t tiles = (D + tile - 1) / tile, columns = B * tiles, chunks = chunks_of(T);
+  const int64_t sms = device_sm_count();
+  float least = 0.f;
+  for (const int64_t slots : {columns, sms, 2 * sms}) {
+    const int64_t want = std::max<int64_t>(1, std::min(slots / std::max<int64_t>(1, columns), chunks));
+    Cut c;
+    c.tiles = (int)tiles;
+    c.per = (chunks + want - 1) / want;
+    c.segments = c.per ? (int)((chunks + c.per - 1) / c.per) : 1;
+    const int64_t ctas = columns * c.segments;
+    const float cost = (float)c.per * (c.segments > 1 ? 1.f + compose : 1.f) *
+                       (ctas > sms ? 1.6f * (float)((ctas + 2 * sms - 1) / (2 * sms)) : 1.f);
+    if (best.segments == 0 || cost < least) best = c, least = cost;
+  }
+  return best;
 }
+constexpr float kComposeForward = 0.7f, kComposeBackward = 0.35f;
 
 template <class T>
-ScanArgs<T> scan_args(const semicrf_recurrence* p, int tile, void* workspace) {
-  const Cut c = cut_of(p->batch, p->T, p->D, tile);
+ScanArgs<T> scan_args(const semicrf_recurrence* p, int tile, float compose, void* workspace) {
+  const Cut c = cut_of(p->batch, p->T, p->D, tile, compose);
   ScanArgs<T> a{};
   a.B = p->batch;
   a.T_ = p->T;
@@ -743,7 +756,7 @@ bool allow_shared(K kernel, int bytes) {
 template <class T, int H, bool BULK>
 int launch_forward(const semicrf_recurrence* p, const ScanArgs<T>& a, cudaStream_t stream) {
   using C = Column<T, H, BULK>;
-  constexpr int S = stages_of<C, 2>(kWarps * 2 * C::kPairs * 16 + 64);
+  constexpr int S = kStages;
   using R = Ring<T, C, 2, S>;
   const auto walk = forward_kernel<T, H, BULK, S, false>;
   const auto compose = forward_kernel<T, H, BULK, S, true>;
@@ -762,12 +775,11 @@ template <class T, bool BULK>
 int launch_backward(const semicrf_recurrence* p, const semicrf_sequence& grad_h,
                     const ScanArgs<T>& a, cudaStream_t stream) {
   using C = Column<T, 1, BULK>;
-  constexpr int fixed = kWarps * 2 * C::kPairs * 24 + C::kPairs * 16 + 64;
-  constexpr int S = stages_of<C, 3>(fixed), SC = stages_of<C, 2>(fixed);
+  constexpr int S = kStages;
   using R = Ring<T, C, 3, S>;
-  using RC = Ring<T, C, 2, SC>;
+  using RC = Ring<T, C, 2, S>;
   const auto walk = backward_kernel<T, BULK, S>;
-  const auto compose = backward_compose_kernel<T, BULK, SC>;
+  const auto compose = backward_compose_kernel<T, BULK, S>;
   CUtensorMap xm{}, gm{}, dm{};
   if (!allow_shared(walk, R::kBytes) || !allow_shared(compose, RC::kBytes) ||
       (BULK && (!sequence_map<T>(&xm, p->x, a.B, a.T_, a.D, C::kTile) ||
@@ -788,7 +800,7 @@ int run_forward(const semicrf_recurrence* p, const semicrf_sequence& h, float* f
                 void* saved, void* workspace, cudaStream_t stream) {
   if (p->T == 0) return copy_state(p, p->initial_state, final_state, stream);
   const int H = sizeof(T) == 2 && p->D > 64 ? 2 : 1;
-  ScanArgs<T> a = scan_args<T>(p, 64 * H, workspace);
+  ScanArgs<T> a = scan_args<T>(p, 64 * H, kComposeForward, workspace);
   a.h = as_seq<T>(h);
   a.first = p->initial_state;
   a.last = final_state;
@@ -811,7 +823,7 @@ int run_backward(const semicrf_recurrence* p, const void* saved, const semicrf_s
                  const semicrf_sequence& grad_gate, float* grad_initial, void* workspace,
                  cudaStream_t stream) {
   if (p->T == 0) return copy_state(p, grad_state, grad_initial, stream);
-  ScanArgs<T> a = scan_args<T>(p, 64, workspace);
+  ScanArgs<T> a = scan_args<T>(p, 64, kComposeBackward, workspace);
   a.dh = as_seq<const T>(grad_h);
   a.dx = as_seq<T>(grad_x);
   a.dg = as_seq<T>(grad_gate);
@@ -856,8 +868,9 @@ size_t recurrence_saved_bytes(const semicrf_recurrence* p) {
   return sizeof(float) * p->batch * chunks_of(p->T) * p->D;
 }
 size_t recurrence_workspace_bytes(const semicrf_recurrence* p) {
-  const int segments = std::max(cut_of(p->batch, p->T, p->D, 64).segments,
-                                cut_of(p->batch, p->T, p->D, 128).segments);
+  const int segments = std::max({cut_of(p->batch, p->T, p->D, 64, kComposeForward).segments,
+                                 cut_of(p->batch, p->T, p->D, 128, kComposeForward).segments,
+                                 cut_of(p->batch, p->T, p->D, 64, kComposeBackward).segments});
   return sizeof(float2) * p->batch * segments * p->D;
 }
 
