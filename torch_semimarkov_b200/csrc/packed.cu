@@ -16,8 +16,20 @@ namespace {
 
 constexpr int kThreads = 256, kUnroll = 4;
 
-// FLAT: every position is valid and all lie at one distance (x.st).
-template <class T, int V, bool FLAT>
+// FLAT: every position is valid and all lie at one distance (x.st).  Without
+// ALIGNED a lane's values are loaded one by one: rows then start anywhere.
+template <class T, int V, bool ALIGNED>
+__device__ __forceinline__ void load_values(const T* p, int64_t left, Pack<T, V>& q) {
+  if (ALIGNED) {
+    q = *reinterpret_cast<const Pack<T, V>*>(p);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < left) q.v[k] = p[k];
+  }
+}
+
+template <class T, int V, bool FLAT, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, Places places, int64_t D,
                                                         int64_t G, Seq<const T> x,
                                                         const int64_t* __restrict__ lengths,
@@ -36,12 +48,11 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, Places pla
     for (int k = 0; k < V; ++k) q[u].v[k] = from_f32<T>(0.f);
     if (u < left && in) {
       if (FLAT) {
-        q[u] = *reinterpret_cast<const Pack<T, V>*>(src);
+        load_values<T, V, ALIGNED>(src, D - d, q[u]);
       } else {
         int64_t b, t;
         locate(places, first + u * deep, b, t);
-        if (!lengths || t < lengths[b])
-          q[u] = *reinterpret_cast<const Pack<T, V>*>(x.row(b, t) + d);
+        if (!lengths || t < lengths[b]) load_values<T, V, ALIGNED>(x.row(b, t) + d, D - d, q[u]);
       }
     }
     src += deep * x.st;
@@ -120,7 +131,7 @@ Grid grid_of(int64_t rows, int64_t G) {
               down <= 0x7fffffff && across <= 65535};
 }
 
-template <class T, int V>
+template <class T, int V, bool ALIGNED>
 int launch_pack(int64_t B, int64_t T_, int64_t D, const semicrf_sequence& x,
                 const int64_t* lengths, int8_t* codes, uint8_t* scales, cudaStream_t stream) {
   const int64_t G = pack_groups(D);
@@ -129,10 +140,10 @@ int launch_pack(int64_t B, int64_t T_, int64_t D, const semicrf_sequence& x,
   Seq<const T> xs = as_seq<const T>(x);
   if (!lengths && (B == 1 || T_ == 1 || x.batch_stride == T_ * x.time_stride)) {
     if (T_ == 1) xs.st = xs.sb;
-    pack_kernel<T, V, true><<<g.grid, g.block, 0, stream>>>(B * T_, Places{}, D, G, xs, nullptr,
+    pack_kernel<T, V, true, ALIGNED><<<g.grid, g.block, 0, stream>>>(B * T_, Places{}, D, G, xs, nullptr,
                                                             codes, scales);
   } else {
-    pack_kernel<T, V, false><<<g.grid, g.block, 0, stream>>>(B * T_, make_places(B, T_), D, G, xs,
+    pack_kernel<T, V, false, ALIGNED><<<g.grid, g.block, 0, stream>>>(B * T_, make_places(B, T_), D, G, xs,
                                                              lengths, codes, scales);
   }
   return launch_status();
@@ -143,8 +154,8 @@ int run_pack(int64_t B, int64_t T_, int64_t D, const semicrf_sequence& x, const 
              int8_t* codes, uint8_t* scales, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   if (D % V == 0 && seq_aligned(x, B, T_, sizeof(T), V))
-    return launch_pack<T, V>(B, T_, D, x, lengths, codes, scales, stream);
-  return launch_pack<T, 1>(B, T_, D, x, lengths, codes, scales, stream);
+    return launch_pack<T, V, true>(B, T_, D, x, lengths, codes, scales, stream);
+  return launch_pack<T, V, false>(B, T_, D, x, lengths, codes, scales, stream);
 }
 
 template <class T, int V>
