@@ -14,7 +14,7 @@ def _recurrence(**kw):
 
     base = dict(batch=0, T=10, D=4, dtype=0, reverse=0)
     base.update(kw)
-    return _lib.SemicrfRecurrence(**base)
+    return ctypes.byref(_lib.SemicrfRecurrence(**base))
 
 
 def _norm(**kw):
@@ -22,7 +22,7 @@ def _norm(**kw):
 
     base = dict(batch=0, T=10, D=4, dtype=1, eps=1e-6, next_weight=1)
     base.update(kw)
-    return _lib.SemicrfBlockNorm(**base)
+    return ctypes.byref(_lib.SemicrfBlockNorm(**base))
 
 
 def test_recurrence_validation_codes():
@@ -51,7 +51,7 @@ def test_block_norm_validation_codes():
     lib = _lib.load()
 
     def forward(p, codes=None):
-        seq = _lib.SemicrfSequence(1, 0, 0)
+        seq = ctypes.byref(_lib.SemicrfSequence(1, 0, 0))
         return lib.semicrf_block_norm_forward(p, seq, seq, None, codes, None, None)
 
     assert forward(_norm()) == _lib.SEMICRF_OK
@@ -71,7 +71,7 @@ def test_pack_validation_codes():
     from torch_semimarkov_b200 import _lib
 
     lib = _lib.load()
-    seq = _lib.SemicrfSequence(None, 0, 0)
+    seq = ctypes.byref(_lib.SemicrfSequence(None, 0, 0))
     assert lib.semicrf_pack(0, 5, 8, 1, seq, None, None, None, None) == _lib.SEMICRF_OK
     assert lib.semicrf_pack(2, 5, 8, 1, seq, None, None, None, None) == \
         _lib.SEMICRF_ERR_INVALID_ARGUMENT
@@ -120,6 +120,14 @@ def test_struct_mirrors_match_the_header():
     from torch_semimarkov_b200 import _lib
 
     assert ctypes.sizeof(_lib.SemicrfSequence) == 24
+    for mirror, packed in ((_lib.SemicrfSequence, _lib._SEQUENCE),
+                           (_lib.SemicrfRecurrence, _lib._RECURRENCE),
+                           (_lib.SemicrfBlockNorm, _lib._BLOCK_NORM)):
+        assert ctypes.sizeof(mirror) == packed.size
+    p = _lib.SemicrfBlockNorm(1, 2, 3, 1, 0.5, (4, 5, 6), (7, 8, 9), (10, 11, 12), 13, 14, 15, 16)
+    assert bytes(p) == _lib._BLOCK_NORM.pack(1, 2, 3, 1, 0.5, *range(4, 17))
+    p = _lib.SemicrfRecurrence(1, 2, 3, 2, 1, (4, 5, 6), (7, 8, 9), 10, 11)
+    assert bytes(p) == _lib._RECURRENCE.pack(1, 2, 3, 2, 1, *range(4, 12))
     assert ctypes.sizeof(_lib.SemicrfRecurrence) == 3 * 8 + 8 + 2 * 24 + 16
     assert ctypes.sizeof(_lib.SemicrfBlockNorm) == 3 * 8 + 8 + 3 * 24 + 4 * 8
 

@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 from typing import Optional
 
 import torch
@@ -233,31 +234,32 @@ def load():
     lib.semicrf_edge_scan_backward.restype = ci
     lib.semicrf_edge_scan_backward.argtypes = [i64, i64, i64, i64, vp, vp, ci, vp, vp, vp, vp,
                                                sz, vp]
-    R, N, Q = (ctypes.POINTER(c) for c in (SemicrfRecurrence, SemicrfBlockNorm, SemicrfSequence))
-    for name, arg in (("semicrf_recurrence_saved_size", R),
-                      ("semicrf_recurrence_workspace_size", R),
-                      ("semicrf_block_norm_workspace_size", N)):
+    # The encoder operators' descriptions (semicrf_recurrence, semicrf_block_norm,
+    # semicrf_sequence) are passed as addresses: of a mirror structure (byref) or
+    # of its packed bytes, which take a fraction of the time to make.
+    for name in ("semicrf_recurrence_saved_size", "semicrf_recurrence_workspace_size",
+                 "semicrf_block_norm_workspace_size"):
         f = getattr(lib, name)
         f.restype = sz
-        f.argtypes = [arg]
+        f.argtypes = [vp]
     lib.semicrf_recurrence_forward.restype = ci
-    lib.semicrf_recurrence_forward.argtypes = [R, Q, vp, vp, vp, sz, vp]
+    lib.semicrf_recurrence_forward.argtypes = [vp, vp, vp, vp, vp, sz, vp]
     lib.semicrf_recurrence_backward.restype = ci
-    lib.semicrf_recurrence_backward.argtypes = [R, vp, Q, vp, Q, Q, vp, vp, sz, vp]
+    lib.semicrf_recurrence_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.semicrf_recurrence_step.restype = ci
     lib.semicrf_recurrence_step.argtypes = [i64, i64, ci, vp, i64, vp, i64, vp, vp, vp, vp, vp]
     lib.semicrf_block_norm_forward.restype = ci
-    lib.semicrf_block_norm_forward.argtypes = [N, Q, Q, vp, vp, vp, vp]
+    lib.semicrf_block_norm_forward.argtypes = [vp, vp, vp, vp, vp, vp, vp]
     lib.semicrf_block_norm_backward.restype = ci
-    lib.semicrf_block_norm_backward.argtypes = [N, vp, Q, Q, Q, Q, Q, vp, vp, sz, vp]
+    lib.semicrf_block_norm_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.semicrf_pack.restype = ci
-    lib.semicrf_pack.argtypes = [i64, i64, i64, ci, Q, vp, vp, vp, vp]
+    lib.semicrf_pack.argtypes = [i64, i64, i64, ci, vp, vp, vp, vp, vp]
     lib.semicrf_unpack.restype = ci
     lib.semicrf_unpack.argtypes = [i64, i64, ci, vp, vp, vp, vp]
     lib.semicrf_packed_weight_grad_workspace_size.restype = sz
     lib.semicrf_packed_weight_grad_workspace_size.argtypes = [i64, i64, i64, i64, ci]
     lib.semicrf_packed_weight_grad.restype = ci
-    lib.semicrf_packed_weight_grad.argtypes = [i64, i64, i64, i64, ci, Q, vp, vp, vp, ci, vp, vp,
+    lib.semicrf_packed_weight_grad.argtypes = [i64, i64, i64, i64, ci, vp, vp, vp, vp, ci, vp, vp,
                                                sz, vp]
     _lib = lib
     return lib
@@ -594,14 +596,22 @@ def _raw_stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _sequence(t: Optional[torch.Tensor]) -> SemicrfSequence:
+# struct semicrf_sequence, semicrf_recurrence and semicrf_block_norm
+_SEQUENCE = struct.Struct("Pqq")
+_RECURRENCE = struct.Struct("qqqiiPqqPqqPP")
+_BLOCK_NORM = struct.Struct("qqqifPqqPqqPqqPPPP")
+_NO_SEQUENCE = _SEQUENCE.pack(0, 0, 0)
+
+
+def _sequence(t: Optional[torch.Tensor]) -> bytes:
     if t is None:
-        return SemicrfSequence(None, 0, 0)
-    return SemicrfSequence(t.data_ptr(), t.stride(0), t.stride(1))
+        return _NO_SEQUENCE
+    sb, st, _ = t.stride()
+    return _SEQUENCE.pack(t.data_ptr(), sb, st)
 
 
-def _addr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 class _SameDevice:
@@ -635,25 +645,31 @@ def first_order(backward):
     return choose
 
 
-def _recurrence(x, gate, initial_state, lengths, reverse) -> SemicrfRecurrence:
+def _recurrence(x, gate, initial_state, lengths, reverse) -> bytes:
     B, T, D = x.shape
-    return SemicrfRecurrence(B, T, D, ACTIVATION_DTYPES[x.dtype], int(bool(reverse)),
-                             _sequence(x), _sequence(gate), _addr(lengths), _addr(initial_state))
+    xb, xt, _ = x.stride()
+    gb, gt, _ = gate.stride()
+    return _RECURRENCE.pack(B, T, D, ACTIVATION_DTYPES[x.dtype], bool(reverse), x.data_ptr(), xb,
+                            xt, gate.data_ptr(), gb, gt, _addr(lengths), _addr(initial_state))
 
 
 def recurrence_forward(x, gate, initial_state, lengths, reverse, want_saved):
     """semicrf_recurrence_forward.  Returns (h, final_state, saved or None)."""
     lib = load()
-    B, T, D = x.shape
+    B, _, D = x.shape
     dev = x.device
     p = _recurrence(x, gate, initial_state, lengths, reverse)
     with _on(dev):
         h = torch.empty_like(x)
-        state = torch.empty((B, D), dtype=torch.float32, device=dev)
-        saved = _scratch(lib.semicrf_recurrence_saved_size(p), dev) if want_saved else None
-        ws = _scratch(lib.semicrf_recurrence_workspace_size(p), dev)
+        state = x.new_empty((B, D), dtype=torch.float32)
+        need = lib.semicrf_recurrence_workspace_size(p)
+        saved = None
+        if want_saved:
+            saved = _scratch(lib.semicrf_recurrence_saved_size(p), dev)
+        ws = _scratch(need, dev)
         st = lib.semicrf_recurrence_forward(p, _sequence(h), state.data_ptr(), _addr(saved),
-                                            ws.data_ptr(), ws.numel(), _raw_stream(dev))
+                                            ws.data_ptr(), need, _raw_stream(dev))
+    if st:
         check(st, "semicrf_recurrence_forward")
     return h, state, saved
 
@@ -661,16 +677,17 @@ def recurrence_forward(x, gate, initial_state, lengths, reverse, want_saved):
 def recurrence_backward(x, gate, lengths, reverse, saved, grad_h, grad_state, want_initial):
     """semicrf_recurrence_backward.  Returns (grad_x, grad_gate, grad_initial or None)."""
     lib = load()
-    B, T, D = x.shape
     dev = x.device
     p = _recurrence(x, gate, None, lengths, reverse)
     with _on(dev):
         gx, gg = torch.empty_like(x), torch.empty_like(gate)
-        gi = torch.empty((B, D), dtype=torch.float32, device=dev) if want_initial else None
-        ws = _scratch(lib.semicrf_recurrence_workspace_size(p), dev)
+        gi = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if want_initial else None
+        need = lib.semicrf_recurrence_workspace_size(p)
+        ws = _scratch(need, dev)
         st = lib.semicrf_recurrence_backward(p, saved.data_ptr(), _sequence(grad_h),
                                              _addr(grad_state), _sequence(gx), _sequence(gg),
-                                             _addr(gi), ws.data_ptr(), ws.numel(), _raw_stream(dev))
+                                             _addr(gi), ws.data_ptr(), need, _raw_stream(dev))
+    if st:
         check(st, "semicrf_recurrence_backward")
     return gx, gg, gi
 
@@ -688,17 +705,24 @@ def recurrence_step(x, gate, state, active, state_out):
                                          x.stride(0), gate.data_ptr(), gate.stride(0),
                                          _addr(active), state.data_ptr(), state_out.data_ptr(),
                                          h.data_ptr(), _raw_stream(dev))
+    if st:
         check(st, "semicrf_recurrence_step")
     return h, state_out
 
 
 def _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
-                eps) -> SemicrfBlockNorm:
+                eps) -> bytes:
     B, T, D = residual.shape
-    return SemicrfBlockNorm(B, T, D, ACTIVATION_DTYPES[residual.dtype], float(eps),
-                            _sequence(residual), _sequence(branch), _sequence(gate),
-                            _addr(branch_weight), _addr(residual_scale), _addr(next_weight),
-                            _addr(lengths))
+    rb, rt, _ = residual.stride()
+    if branch is None:
+        rows = (0, 0, 0, 0, 0, 0)
+    else:
+        bb, bt, _ = branch.stride()
+        gb, gt, _ = gate.stride()
+        rows = (branch.data_ptr(), bb, bt, gate.data_ptr(), gb, gt)
+    return _BLOCK_NORM.pack(B, T, D, ACTIVATION_DTYPES[residual.dtype], eps, residual.data_ptr(),
+                            rb, rt, *rows, _addr(branch_weight), _addr(residual_scale),
+                            next_weight.data_ptr(), _addr(lengths))
 
 
 def packed_buffers(B: int, T: int, D: int, device):
@@ -720,11 +744,11 @@ def block_norm_forward(residual, branch, gate, branch_weight, residual_scale, ne
     with _on(dev):
         out = None if branch is None else torch.empty_like(residual)
         normed = torch.empty_like(residual)
-        stats = (torch.empty((B, T, 2), dtype=torch.float32, device=dev) if want_statistics
-                 else None)
+        stats = residual.new_empty((B, T, 2), dtype=torch.float32) if want_statistics else None
         codes, scales = packed_buffers(B, T, D, dev) if pack else (None, None)
         st = lib.semicrf_block_norm_forward(p, _sequence(out), _sequence(normed), _addr(stats),
                                             _addr(codes), _addr(scales), _raw_stream(dev))
+    if st:
         check(st, "semicrf_block_norm_forward")
     return out, normed, stats, codes, scales
 
@@ -743,12 +767,13 @@ def block_norm_backward(residual, branch, gate, branch_weight, residual_scale, n
         gb = gg = None
         if branch is not None:
             gb, gg = torch.empty_like(branch), torch.empty_like(gate)
-        gw = torch.empty((3, D), dtype=torch.float32, device=dev)
+        gw = residual.new_empty((3, D), dtype=torch.float32)
         ws = _scratch(lib.semicrf_block_norm_workspace_size(p), dev)
         st = lib.semicrf_block_norm_backward(p, stats.data_ptr(), _sequence(grad_out),
                                              _sequence(grad_normed), _sequence(gr), _sequence(gb),
                                              _sequence(gg), gw.data_ptr(), ws.data_ptr(),
                                              ws.numel(), _raw_stream(dev))
+    if st:
         check(st, "semicrf_block_norm_backward")
     return gr, gb, gg, gw
 
@@ -762,6 +787,7 @@ def pack(x, lengths):
         codes, scales = packed_buffers(B, T, D, dev)
         st = lib.semicrf_pack(B, T, D, ACTIVATION_DTYPES[x.dtype], _sequence(x), _addr(lengths),
                               codes.data_ptr(), scales.data_ptr(), _raw_stream(dev))
+    if st:
         check(st, "semicrf_pack")
     return codes, scales
 
@@ -775,6 +801,7 @@ def unpack(codes, scales, D: int, dtype):
         out = torch.empty((B, T, D), dtype=dtype, device=dev)
         st = lib.semicrf_unpack(B * T, D, ACTIVATION_DTYPES[dtype], codes.data_ptr(),
                                 scales.data_ptr(), out.data_ptr(), _raw_stream(dev))
+    if st:
         check(st, "semicrf_unpack")
     return out
 
@@ -792,5 +819,6 @@ def packed_weight_grad(grad_output, codes, scales, D: int, lengths, out_dtype):
                                             codes.data_ptr(), scales.data_ptr(), _addr(lengths),
                                             ACTIVATION_DTYPES[out_dtype], out.data_ptr(),
                                             ws.data_ptr(), ws.numel(), _raw_stream(dev))
+    if st:
         check(st, "semicrf_packed_weight_grad")
     return out

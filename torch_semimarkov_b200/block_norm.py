@@ -23,10 +23,9 @@ class _BlockNorm(torch.autograd.Function):
     inputs and two statistics a position; the backward recomputes r."""
 
     @staticmethod
-    def forward(ctx, residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
-                eps, pack):
-        weights = [None if w is None else w.to(torch.float32).contiguous()
-                   for w in (branch_weight, residual_scale, next_weight)]
+    def forward(ctx, residual, branch, gate, branch_weight, residual_scale, next_weight, weights,
+                lengths, eps, pack):
+        # weights: the three as contiguous float32, what the kernels read
         out, normed, stats, codes, scales = _lib.block_norm_forward(
             residual, branch, gate, *weights, lengths, eps, want_statistics=True, pack=pack)
         ctx.save_for_backward(residual, branch, gate, *weights, lengths, stats)
@@ -48,8 +47,9 @@ class _BlockNorm(torch.autograd.Function):
             grad_normed = _lib.activation(grad_normed, "grad_normed", like=residual)
         gr, gb, gg, gw = _lib.block_norm_backward(residual, branch, gate, w1, scale, w2, lengths,
                                                   ctx.eps, stats, grad_out, grad_normed)
-        grads = [None if dt is None else gw[i].to(dt) for i, dt in enumerate(ctx.weight_dtypes)]
-        return gr, gb, gg, *grads, None, None, None
+        grads = [None if dt is None else g if dt == torch.float32 else g.to(dt)
+                 for g, dt in zip(gw.unbind(0), ctx.weight_dtypes)]
+        return gr, gb, gg, *grads, None, None, None, None
 
 
 def _call(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths, eps, pack):
@@ -71,7 +71,8 @@ def _call(residual, branch, gate, branch_weight, residual_scale, next_weight, le
     lengths = _lib.valid_lengths(lengths, B, T, dev)
     given = (residual, branch, gate, branch_weight, residual_scale, next_weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
-        out, normed, codes, scales = _BlockNorm.apply(*given, lengths, eps, bool(pack))
+        out, normed, codes, scales = _BlockNorm.apply(*given, (w1, scale, w2), lengths, eps,
+                                                       bool(pack))
     else:
         out, normed, _, codes, scales = _lib.block_norm_forward(
             residual, branch, gate, w1, scale, w2, lengths, eps, want_statistics=False, pack=pack)

@@ -22,9 +22,10 @@ class _GatedLinearRecurrence(torch.autograd.Function):
     positions; the backward recomputes the states inside a run from those."""
 
     @staticmethod
-    def forward(ctx, x, gate, initial_state, lengths, reverse):
-        s0 = None if initial_state is None else initial_state.to(torch.float32).contiguous()
-        h, state, saved = _lib.recurrence_forward(x, gate, s0, lengths, reverse, want_saved=True)
+    def forward(ctx, x, gate, initial_state, start, lengths, reverse):
+        # start holds initial_state as contiguous float32, what the kernels read
+        h, state, saved = _lib.recurrence_forward(x, gate, start[0], lengths, reverse,
+                                                  want_saved=True)
         ctx.save_for_backward(x, gate, lengths, saved)
         ctx.reverse = reverse
         ctx.initial_dtype = None if initial_state is None else initial_state.dtype
@@ -42,9 +43,9 @@ class _GatedLinearRecurrence(torch.autograd.Function):
         want = ctx.initial_dtype is not None and ctx.needs_input_grad[2]
         gx, gg, gi = _lib.recurrence_backward(x, gate, lengths, ctx.reverse, saved, grad_h,
                                               grad_state, want)
-        if gi is not None:
+        if want and ctx.initial_dtype != torch.float32:
             gi = gi.to(ctx.initial_dtype)
-        return gx, gg, gi, None, None
+        return gx, gg, gi, None, None, None
 
 
 def gated_linear_recurrence(
@@ -77,12 +78,12 @@ def gated_linear_recurrence(
     needs_grad = torch.is_grad_enabled() and (
         x.requires_grad or gate.requires_grad
         or (initial_state is not None and initial_state.requires_grad))
+    s0 = None
     if initial_state is not None:
         s0 = _lib.float_vector(initial_state, "initial_state", (B, D), x.device)
     if needs_grad:
-        return _GatedLinearRecurrence.apply(x, gate, initial_state, lengths, bool(reverse))
-    h, state, _ = _lib.recurrence_forward(x, gate, None if initial_state is None else s0, lengths,
-                                          reverse, want_saved=False)
+        return _GatedLinearRecurrence.apply(x, gate, initial_state, (s0,), lengths, bool(reverse))
+    h, state, _ = _lib.recurrence_forward(x, gate, s0, lengths, reverse, want_saved=False)
     return h, state
 
 
