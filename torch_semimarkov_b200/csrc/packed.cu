@@ -5,6 +5,10 @@
 // lanes of a group of 32 channels are neighbours and its maximum is a few
 // shuffles.  A thread keeps its columns and takes kUnroll rows, all requested
 // before the first is used.
+//
+// Rows that do not start on 16-byte boundaries are taken by the same lanes,
+// value by value: the vectors' lines are in L1 after the first load.  Lanes of
+// one value each, which need no alignment, do eight times the work a value.
 
 #include <algorithm>
 #include <type_traits>
@@ -16,8 +20,7 @@ namespace {
 
 constexpr int kThreads = 256, kUnroll = 4;
 
-// FLAT: every position is valid and all lie at one distance (x.st).  Without
-// ALIGNED a lane's values are loaded one by one: rows then start anywhere.
+// A lane's values, the first `left` of them where rows are not ALIGNED.
 template <class T, int V, bool ALIGNED>
 __device__ __forceinline__ void load_values(const T* p, int64_t left, Pack<T, V>& q) {
   if (ALIGNED) {
@@ -29,6 +32,7 @@ __device__ __forceinline__ void load_values(const T* p, int64_t left, Pack<T, V>
   }
 }
 
+// FLAT: every position is valid and all lie at one distance (x.st).
 template <class T, int V, bool FLAT, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, Places places, int64_t D,
                                                         int64_t G, Seq<const T> x,
@@ -140,11 +144,11 @@ int launch_pack(int64_t B, int64_t T_, int64_t D, const semicrf_sequence& x,
   Seq<const T> xs = as_seq<const T>(x);
   if (!lengths && (B == 1 || T_ == 1 || x.batch_stride == T_ * x.time_stride)) {
     if (T_ == 1) xs.st = xs.sb;
-    pack_kernel<T, V, true, ALIGNED><<<g.grid, g.block, 0, stream>>>(B * T_, Places{}, D, G, xs, nullptr,
-                                                            codes, scales);
+    pack_kernel<T, V, true, ALIGNED>
+        <<<g.grid, g.block, 0, stream>>>(B * T_, Places{}, D, G, xs, nullptr, codes, scales);
   } else {
-    pack_kernel<T, V, false, ALIGNED><<<g.grid, g.block, 0, stream>>>(B * T_, make_places(B, T_), D, G, xs,
-                                                             lengths, codes, scales);
+    pack_kernel<T, V, false, ALIGNED><<<g.grid, g.block, 0, stream>>>(
+        B * T_, make_places(B, T_), D, G, xs, lengths, codes, scales);
   }
   return launch_status();
 }
@@ -164,8 +168,8 @@ int launch_unpack(int64_t rows, int64_t D, const int8_t* codes, const uint8_t* s
   const int64_t G = pack_groups(D);
   const Grid g = grid_of<V>(rows, G);
   if (!g.ok) return SEMICRF_ERR_UNSUPPORTED;
-  unpack_kernel<T, V><<<g.grid, g.block, 0, stream>>>(rows, D, G, codes, scales,
-                                                      static_cast<T*>(out));
+  unpack_kernel<T, V>
+      <<<g.grid, g.block, 0, stream>>>(rows, D, G, codes, scales, static_cast<T*>(out));
   return launch_status();
 }
 
