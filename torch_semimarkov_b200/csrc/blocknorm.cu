@@ -50,13 +50,14 @@ struct NormArgs {
 
 // Sums over the row's lanes; every lane gets the result.  `red` alternates
 // between two slots, so one barrier per sum is enough.
-template <int WR>
+template <class L>
 struct RowSum {
+  static constexpr int WR = L::WR;
   float (*red)[WR];
   int slot, w, lane, barrier;
   __device__ __forceinline__ float operator()(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    for (int o = 16 / L::SPLIT; o > 0; o >>= 1) v += __shfl_xor_sync(L::peers(), v, o);
     if (WR > 1) {
       slot ^= 1;
       if (lane == 0) red[slot][w] = v;
@@ -69,19 +70,29 @@ struct RowSum {
   }
 };
 
-// PER channels to a lane in vectors of V, WR warps to a row.
-template <class T, int V_, int WR_, int PER_>
+// PER channels to a lane in vectors of V, WR warps to a row or SPLIT rows to a warp.
+template <class T, int V_, int WR_, int PER_, int SPLIT_ = 1>
 struct Layout {
-  static constexpr int V = V_, WR = WR_, PER = PER_;
+  static constexpr int V = V_, WR = WR_, PER = PER_, SPLIT = SPLIT_;
   static constexpr int J = PER / V;                   // vectors of a lane
   static constexpr int H = PER / 2;                   // pairs of a lane
-  static constexpr int NL = 32 * WR;                  // lanes of a row
-  static constexpr int kRows = WR >= 4 ? 1 : 4 / WR;  // rows that a CTA works on at once
+  static constexpr int NL = 32 * WR / SPLIT;          // lanes of a row
+  static constexpr int kRows = SPLIT * (WR >= 4 ? 1 : 4 / WR);  // rows that a CTA works on at once
+  static_assert(SPLIT == 1 || NL * V >= kPackGroup, "a row's lanes hold its groups' codes");
   static constexpr int kThreads = NL * kRows;
-  // CTAs of the backward on an SM: 12 warps of 16 channels a lane (168 registers),
-  // 16 of 8 (128), 24 of 4 (80)
-  static constexpr int kWarpsPerSm = PER == 16 ? 12 : PER == 8 ? 16 : 24;
+  // CTAs of the backward on an SM: 8 warps of 24 channels a lane (255 registers),
+  // 12 of 16 (168), 16 of 8 (128), 24 of 4 (80)
+  static constexpr int kWarpsPerSm = PER == 24 ? 8 : PER == 16 ? 12 : PER == 8 ? 16 : 24;
   static constexpr int kPerSm = NL * kRows < 32 * kWarpsPerSm ? 32 * kWarpsPerSm / kThreads : 1;
+  // shared memory of a CTA beside a ring, and what a CTA may take if n of them are to lie on an SM
+  static constexpr bool kSharedWeights = H * NL <= 2048;
+  static constexpr int kFixedBytes =
+      (kSharedWeights ? 16 * H * NL : 16) + (kRows > 1 ? 8 * H * NL : 8) + 8 * kRows * WR + 2048;
+  static constexpr int share(int n) { return 228 * 1024 / n - kFixedBytes; }
+  // the lanes of a warp that work on this lane's row; others may be elsewhere
+  __device__ static __forceinline__ unsigned peers() {
+    return SPLIT == 1 ? ~0u : ((1u << (32 / SPLIT)) - 1) << (threadIdx.x & 31 & ~(32 / SPLIT - 1));
+  }
   // channel of vector j of lane l
   __device__ static __forceinline__ int channel(int j, int l) { return (j * NL + l) * V; }
   // channel of half k of pair i of lane l
@@ -126,7 +137,7 @@ struct Held {
 // shared memory, or in the widest layout (64 KB of them) from global memory.
 template <class L, bool BRANCH>
 struct Weights {
-  static constexpr bool kShared = L::H * L::NL <= 2048;
+  static constexpr bool kShared = L::kSharedWeights;
   static constexpr int kSize = kShared ? L::H * L::NL : 1;
   float2 *sw_, *w2_;
   const float *s, *w1, *w2g;
@@ -173,7 +184,9 @@ struct PlainRows {
 template <class T, class L, int N>
 struct RingRows {
   static constexpr int kSlotBytes = N * L::J * L::kThreads * 16;
-  static constexpr int kSlots = 3 * kSlotBytes <= 96 * 1024 ? 3 : 2 * kSlotBytes <= 200 * 1024 ? 2 : 0;
+  static constexpr int kCtas = N == 5 ? L::kPerSm : 1;  // that have to fit an SM
+  static constexpr int kRoom = L::share(kCtas) / kSlotBytes;
+  static constexpr int kSlots = kRoom >= 3 && 3 * kSlotBytes <= 96 * 1024 ? 3 : kRoom >= 2 ? 2 : 0;
   unsigned char* at;  // this thread's part of the present slot
   __device__ __forceinline__ float2 pair(int k, int i) const {
     const int j = 2 * i / L::V;
@@ -227,7 +240,7 @@ __device__ __forceinline__ void put_codes(const NormArgs<T>& a, int64_t row, int
 #pragma unroll
       for (int k = 0; k < L::V; ++k) v.v[k] = from_f32<T>(0.f);
     Pack<int8_t, L::V> c;
-    const uint8_t byte = pack_encode(v, c);
+    const uint8_t byte = pack_encode(v, c, L::peers());
     if (d < G * kPackGroup) {
       *reinterpret_cast<Pack<int8_t, L::V>*>(a.codes + row * G * kPackGroup + d) = c;
       if (d % kPackGroup == 0) a.scales[row * G + d / kPackGroup] = byte;
@@ -244,7 +257,7 @@ __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArg
   __shared__ float red[L::kRows][2][L::WR];
   __shared__ float2 sw_at[BRANCH ? Weights<L, BRANCH>::kSize : 1], w2_at[Weights<L, BRANCH>::kSize];
   const int group = threadIdx.x / NL, l = threadIdx.x % NL;
-  RowSum<L::WR> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
+  RowSum<L> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
   bool ok[L::J];
 #pragma unroll
   for (int j = 0; j < L::J; ++j) ok[j] = L::channel(j, l) < a.D;
@@ -332,10 +345,10 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_backward_kernel(c
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float red[L::kRows][2][L::WR];
   __shared__ float2 sw_at[BRANCH ? Weights<L, BRANCH>::kSize : 1], w2_at[Weights<L, BRANCH>::kSize];
-  __shared__ float2 sums[L::kRows > 1 ? H * NL : 1];
+  __shared__ float2 sums[L::kRows > L::SPLIT ? H * NL : 1];
   const Weights<L, BRANCH> weight(a, sw_at, w2_at);
   const int group = threadIdx.x / NL, l = threadIdx.x % NL;
-  RowSum<L::WR> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
+  RowSum<L> row_sum{red[group], 0, l >> 5, l & 31, 1 + group};
   bool ok[L::J];
 #pragma unroll
   for (int j = 0; j < L::J; ++j) ok[j] = L::channel(j, l) < a.D;
@@ -439,18 +452,27 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_backward_kernel(c
   }
   if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
 
-  // the CTA's sums, its row groups added in order
+  // the CTA's sums: over the rows of a warp, then its row groups in order
+  constexpr int kGroups = L::kRows / L::SPLIT;
+  const int mine = group / L::SPLIT;
 #pragma unroll
   for (int m = BRANCH ? 0 : 1; m < 2; ++m) {
-    if (L::kRows > 1) {
+#pragma unroll
+    for (int o = NL; o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        acc[m][i].x += __shfl_xor_sync(~0u, acc[m][i].x, o);
+        acc[m][i].y += __shfl_xor_sync(~0u, acc[m][i].y, o);
+      }
+    if (kGroups > 1) {
 #pragma unroll 1
-      for (int turn = L::kRows - 1; turn > 0; --turn) {
+      for (int turn = kGroups - 1; turn > 0; --turn) {
         __syncthreads();
-        if (group == turn)
+        if (group == turn * L::SPLIT)
 #pragma unroll
           for (int i = 0; i < H; ++i) sums[i * NL + l] = acc[m][i];
         __syncthreads();
-        if (group == turn - 1)
+        if (mine == turn - 1)
 #pragma unroll
           for (int i = 0; i < H; ++i) acc[m][i] = __fadd2_rn(acc[m][i], sums[i * NL + l]);
       }
@@ -524,11 +546,11 @@ template <class T, class L, bool BRANCH>
 int launch(const NormArgs<T>& a, bool backward, float* grad_weights, cudaStream_t stream) {
   if (!backward) {
     const int64_t all = (a.rows + L::kRows - 1) / L::kRows;
-    const int64_t most = (int64_t)std::max(1, 1024 / L::kThreads) * device_sm_count();
-    const unsigned grid = (unsigned)std::min<int64_t>(all, most);
     constexpr bool kRing = BRANCH && L::V * sizeof(T) == 16 && RingRows<T, L, 3>::kSlots > 0;
     const auto kernel = norm_forward_kernel<T, L, BRANCH, kRing>;
     constexpr int bytes = kRing ? RingRows<T, L, 3>::kSlots * RingRows<T, L, 3>::kSlotBytes : 0;
+    const int64_t most = (int64_t)std::max(1, 1024 / L::kThreads) * device_sm_count();
+    const unsigned grid = (unsigned)std::min<int64_t>(all, most);
     if (bytes && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       bytes) != cudaSuccess)
       return SEMICRF_ERR_CUDA;
@@ -550,19 +572,27 @@ int launch(const NormArgs<T>& a, bool backward, float* grad_weights, cudaStream_
   return launch_status();
 }
 
-// The fewest warps whose registers hold a row: 16 channels a lane where 16-bit
-// values lie packed, 8 else (16 above 4096, where 8 would want 32 warps).
+// The fewest lanes whose registers hold a row: 16 or 24 channels a lane where
+// 16-bit values lie packed, 8 else (16 above 4096, where 8 would want 32 warps);
+// narrow rows share a warp.
 template <class T, int V, bool BRANCH>
 int launch_width(const NormArgs<T>& a, bool backward, float* gw, cudaStream_t s) {
-  constexpr int W = V < 4 ? V : 4;
-  if (a.D <= 128) return launch<T, Layout<T, W, 1, 4>, BRANCH>(a, backward, gw, s);
-  if (a.D <= 256) return launch<T, Layout<T, V, 1, 8>, BRANCH>(a, backward, gw, s);
+  constexpr int N = V > 1 ? V : 4;  // channels of a lane of a narrow row
+  if constexpr (V >= 4) {
+    if (V == 8 && a.D <= 4 * N)
+      return launch<T, Layout<T, V, 1, N, V>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 8 * N) return launch<T, Layout<T, V, 1, N, 4>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 16 * N) return launch<T, Layout<T, V, 1, N, 2>, BRANCH>(a, backward, gw, s);
+  }
+  if (a.D <= 32 * N) return launch<T, Layout<T, V, 1, N>, BRANCH>(a, backward, gw, s);
+  if constexpr (N < 8)
+    if (a.D <= 256) return launch<T, Layout<T, V, 1, 8>, BRANCH>(a, backward, gw, s);
   if (a.D > 4096) return launch<T, Layout<T, V, 16, 16>, BRANCH>(a, backward, gw, s);
   if constexpr (V * sizeof(T) == 16 && sizeof(T) == 2) {
     if (a.D <= 512) return launch<T, Layout<T, V, 1, 16>, BRANCH>(a, backward, gw, s);
-    if (a.D <= 768) return launch<T, Layout<T, V, 3, 8>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 768) return launch<T, Layout<T, V, 1, 24>, BRANCH>(a, backward, gw, s);
     if (a.D <= 1024) return launch<T, Layout<T, V, 2, 16>, BRANCH>(a, backward, gw, s);
-    if (a.D <= 1536) return launch<T, Layout<T, V, 3, 16>, BRANCH>(a, backward, gw, s);
+    if (a.D <= 1536) return launch<T, Layout<T, V, 2, 24>, BRANCH>(a, backward, gw, s);
     if (a.D <= 2048) return launch<T, Layout<T, V, 4, 16>, BRANCH>(a, backward, gw, s);
     return launch<T, Layout<T, V, 8, 16>, BRANCH>(a, backward, gw, s);
   } else {

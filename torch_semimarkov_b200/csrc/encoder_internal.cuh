@@ -213,7 +213,7 @@ __device__ __forceinline__ float pack_scale(uint8_t byte) {  // 255 (inf) times 
 
 // The largest magnitude of a lane's values, as the bits of a float.
 template <class T, int V>
-__device__ __forceinline__ unsigned pack_top(const Pack<T, V>& v) {
+__device__ __forceinline__ unsigned pack_top(const Pack<T, V>& v, unsigned lanes) {
   unsigned top = 0;
   if constexpr (sizeof(T) == 2 && V % 2 == 0) {
     // 16-bit types order by their bits without the sign: two at a time
@@ -221,24 +221,25 @@ __device__ __forceinline__ unsigned pack_top(const Pack<T, V>& v) {
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
 #pragma unroll
-    for (int o = 1; o < kPackGroup / V; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(~0u, top, o));
+    for (int o = 1; o < kPackGroup / V; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(lanes, top, o));
     const unsigned short one = (unsigned short)max(top & 0xffffu, top >> 16);
     return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&one)));
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(to_f32(v.v[j])) & 0x7fffffffu);
 #pragma unroll
-    for (int o = 1; o < kPackGroup / V; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+    for (int o = 1; o < kPackGroup / V; o <<= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
     return top;
   }
 }
 
 // Codes of a group whose values lie V to a lane in 32 / V neighbouring lanes
-// (all lanes of the warp call this); returns the scale byte.
+// (all of `lanes` call this together); returns the scale byte.
 template <class T, int V>
-__device__ __forceinline__ uint8_t pack_encode(const Pack<T, V>& v, Pack<int8_t, V>& q) {
+__device__ __forceinline__ uint8_t pack_encode(const Pack<T, V>& v, Pack<int8_t, V>& q,
+                                               unsigned lanes = ~0u) {
   // top = m 2^p, 1/2 <= m < 1, exponent field p + 126: e is p - 7 where m <= 127/128, else p - 6
-  const unsigned top = pack_top(v);
+  const unsigned top = pack_top(v, lanes);
   const int field = (int)(top >> 23);
   int byte = max(1, field - 6 + ((top & 0x7fffffu) > 0x7e0000u));
   if (top == 0) byte = 0;
