@@ -17,6 +17,13 @@
 // tile takes a run of positions; the runs' partial results are summed in
 // order by a second kernel.
 //
+// Bound by the tensor cores with wide products, by decoding with narrow ones.
+// Measured, 131,072 positions, M 1,536, D 512: bfloat16 by bulk copies 175 us,
+// 1,180 TFLOP/s, 0.71 of the library product's measured rate (the decoding
+// warps' fences and the hand-over of a stage leave the tensor pipe idle for the
+// rest); float16 and odd strides through registers 450 to 590 us; float32 with
+// M 768 620 to 670 us (three products each).  The runs' sum is 10 us more.
+//
 // The tensor cores truncate their float32 sums (measured: 1.8e-8 of the result
 // for each 16 positions), which is nothing beside 16-bit dy.  For float32 the
 // leading piece is summed apart from the others and, every 512 positions,
