@@ -310,13 +310,15 @@ int semicrf_unpack(int64_t rows, int64_t D, int dtype, const int8_t* codes,
                    const uint8_t* scales, void* out, void* stream);
 /* Gradient of a linear layer's weight from its input's checkpoint:
  * out (M, D) = sum over valid positions of grad_output^T x, grad_output
- * (B, T, M) of type dtype, out of type out_dtype. */
+ * (B, T, M) of type dtype, the checkpoint made of a tensor of type
+ * packed_dtype, out of type out_dtype. */
 size_t semicrf_packed_weight_grad_workspace_size(int64_t B, int64_t T, int64_t D, int64_t M,
                                                  int dtype);
 int semicrf_packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
                                const semicrf_sequence* grad_output, const int8_t* codes,
-                               const uint8_t* scales, const int64_t* lengths, int out_dtype,
-                               void* out, void* workspace, size_t workspace_bytes, void* stream);
+                               const uint8_t* scales, int packed_dtype, const int64_t* lengths,
+                               int out_dtype, void* out, void* workspace, size_t workspace_bytes,
+                               void* stream);
 
 const char* semicrf_strerror(int status);
 int semicrf_abi_version(void);

@@ -81,7 +81,7 @@ def test_pack_validation_codes():
     assert lib.semicrf_unpack(3, 8, 1, None, None, None, None) == \
         _lib.SEMICRF_ERR_INVALID_ARGUMENT
     assert lib.semicrf_packed_weight_grad_workspace_size(2, 5, 8, 0, 1) == 0
-    assert lib.semicrf_packed_weight_grad(2, 5, 8, 3, 1, seq, None, None, None, 0, None, None, 0,
+    assert lib.semicrf_packed_weight_grad(2, 5, 8, 3, 1, seq, None, None, 1, None, 0, None, None, 0,
                                           None) == _lib.SEMICRF_ERR_INVALID_ARGUMENT
 
 

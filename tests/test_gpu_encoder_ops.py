@@ -657,6 +657,31 @@ def test_weight_grad_of_many_positions(dtype):
     _check_weight_grad(_normal(g, B, T, D, dtype=dtype), _normal(g, B, T, M, dtype=dtype), n)
 
 
+@pytest.mark.parametrize("D,M", [(64, 72), (160, 264)])
+def test_weight_grad_of_float16_from_end_to_end(D, M):
+    """Groups of the smallest subnormal numbers, of the largest and of zeros,
+    and gradients that are subnormal themselves."""
+    g = _gen(D)
+    B, T = 2, 333
+    x, dy = (_normal(g, B, T, n, dtype=torch.float16) for n in (D, M))
+    x[:, ::5] = x[:, ::5] * 2.0 ** -22
+    x[:, 1::5, :32] = 65504.0
+    x[:, 2::5, 32:] = 0.0
+    x[:, 3::5] = x[:, 3::5] * 2.0 ** -12
+    dy[:, ::3] = dy[:, ::3] * 2.0 ** -20
+    n = torch.tensor([333, 100])
+    _check_weight_grad(x, dy, None, torch.float32)
+    _check_weight_grad(x, dy, n, torch.float32)
+
+
+def test_weight_grad_of_float16_over_a_wider_checkpoint():
+    """A checkpoint of bfloat16 values holds what float16 does not."""
+    g = _gen(3)
+    x = _normal(g, 2, 100, 64, dtype=torch.bfloat16) * 1e20
+    x[:, ::2] *= 1e-30
+    _check_weight_grad(x, _normal(g, 2, 100, 64, dtype=torch.float16), None, torch.float32)
+
+
 def test_weight_grad_strides_and_scales():
     """grad_output as a slice (aligned and not) and transposed; scales far apart."""
     g = _gen(9)

@@ -259,8 +259,8 @@ def load():
     lib.semicrf_packed_weight_grad_workspace_size.restype = sz
     lib.semicrf_packed_weight_grad_workspace_size.argtypes = [i64, i64, i64, i64, ci]
     lib.semicrf_packed_weight_grad.restype = ci
-    lib.semicrf_packed_weight_grad.argtypes = [i64, i64, i64, i64, ci, vp, vp, vp, vp, ci, vp, vp,
-                                               sz, vp]
+    lib.semicrf_packed_weight_grad.argtypes = [i64, i64, i64, i64, ci, vp, vp, vp, ci, vp, ci, vp,
+                                               vp, sz, vp]
     _lib = lib
     return lib
 
@@ -806,7 +806,7 @@ def unpack(codes, scales, D: int, dtype):
     return out
 
 
-def packed_weight_grad(grad_output, codes, scales, D: int, lengths, out_dtype):
+def packed_weight_grad(grad_output, codes, scales, D: int, packed_dtype, lengths, out_dtype):
     """semicrf_packed_weight_grad.  Returns the (M, D) gradient."""
     lib = load()
     B, T, M = grad_output.shape
@@ -816,7 +816,8 @@ def packed_weight_grad(grad_output, codes, scales, D: int, lengths, out_dtype):
         out = torch.empty((M, D), dtype=out_dtype, device=dev)
         ws = _scratch(lib.semicrf_packed_weight_grad_workspace_size(B, T, D, M, dt), dev)
         st = lib.semicrf_packed_weight_grad(B, T, D, M, dt, _sequence(grad_output),
-                                            codes.data_ptr(), scales.data_ptr(), _addr(lengths),
+                                            codes.data_ptr(), scales.data_ptr(),
+                                            ACTIVATION_DTYPES[packed_dtype], _addr(lengths),
                                             ACTIVATION_DTYPES[out_dtype], out.data_ptr(),
                                             ws.data_ptr(), ws.numel(), _raw_stream(dev))
     if st:

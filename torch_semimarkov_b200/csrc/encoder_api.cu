@@ -181,18 +181,18 @@ size_t semicrf_packed_weight_grad_workspace_size(int64_t B, int64_t T, int64_t D
 
 int semicrf_packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
                                const semicrf_sequence* grad_output, const int8_t* codes,
-                               const uint8_t* scales, const int64_t* lengths, int out_dtype,
-                               void* out, void* workspace, size_t workspace_bytes, void* stream) {
+                               const uint8_t* scales, int packed_dtype, const int64_t* lengths,
+                               int out_dtype, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   int st = check_sizes(B, T, D, dtype);
   if (st == SEMICRF_OK) st = M < 1 ? SEMICRF_ERR_INVALID_ARGUMENT : check_sizes(B, T, M, dtype);
   if (st != SEMICRF_OK) return st;
-  if (!known_type(out_dtype) || !out) return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!known_type(out_dtype) || !known_type(packed_dtype) || !out) return SEMICRF_ERR_INVALID_ARGUMENT;
   if (!grad_output || (B && T && (!grad_output->data || !codes || !scales)))
     return SEMICRF_ERR_INVALID_ARGUMENT;
   const size_t need = packed_weight_grad_workspace_bytes(B, T, D, M, dtype);
   if (workspace_bytes < need || !workspace) return SEMICRF_ERR_WORKSPACE;
-  return packed_weight_grad(B, T, D, M, dtype, *grad_output, codes, scales, lengths, out_dtype,
-                            out, workspace, as_stream(stream));
+  return packed_weight_grad(B, T, D, M, dtype, packed_dtype, *grad_output, codes, scales, lengths,
+                            out_dtype, out, workspace, as_stream(stream));
 }
 
 }  // extern "C"

@@ -291,6 +291,30 @@ __device__ __forceinline__ uint4 pack_decode(uint2 q, uint8_t byte) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// The same for the checkpoint of a float16 activation, whose decoded values are
+// all float16: code byte q + 128 below 0x64 is 1024 + q + 128.  The scale may lie
+// below float16's range and is then multiplied in two steps; the first is exact,
+// since 2^-14 is the smallest normal number, and the second ends on a float16.
+__device__ __forceinline__ uint4 pack_decode_half(uint2 q, uint8_t byte) {
+  const bool low = byte < 127 - 14;
+  const __half2 unit = __half2half2(__float2half_rn(low ? 6.103515625e-5f : pack_scale(byte)));
+  const __half2 rest = __half2half2(__float2half_rn(low ? pack_scale(byte + 14) : 1.f));
+  const __half2 zero_at = __half2half2(__float2half_rn(1152.f));
+  unsigned o[4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned w = (k ? q.y : q.x) ^ 0x80808080u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned a = __byte_perm(w, 0x64646464u, h ? 0x4342u : 0x4140u);
+      const __half2 v = __hmul2(
+          __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&a), zero_at), unit), rest);
+      o[2 * k + h] = *reinterpret_cast<const unsigned*>(&v);
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 inline int launch_status() {
   return cudaGetLastError() == cudaSuccess ? SEMICRF_OK : SEMICRF_ERR_CUDA;
 }
@@ -327,7 +351,7 @@ int unpack_rows(int64_t rows, int64_t D, int dtype, const int8_t* codes, const u
 
 // packgrad.cu
 size_t packed_weight_grad_workspace_bytes(int64_t B, int64_t T, int64_t D, int64_t M, int dtype);
-int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
+int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype, int packed_dtype,
                        const semicrf_sequence& grad_output, const int8_t* codes,
                        const uint8_t* scales, const int64_t* lengths, int out_dtype, void* out,
                        void* workspace, cudaStream_t stream);

@@ -6,10 +6,12 @@
 // operands lie in memory with their channels contiguous, so both are
 // MN-major; a position is one row of the shared-memory tile.
 //
-// x: a code times a power of two has 7 bits, so its bfloat16 value is exact.
-// dy: bfloat16 as it is; float16 and float32 are cut into 2 and 3 bfloat16
-// pieces of 8 bits each (exact: 11 and 24 bits), one product each.  So every
-// product is exact and only the float32 sums round.
+// x: a code times a power of two has 7 bits, so its bfloat16 value is exact,
+// and its float16 value too where the checkpoint is of a float16 tensor.
+// dy: bfloat16 as it is, and float16 as it is over a float16 checkpoint; else
+// float16 and float32 are cut into 2 and 3 bfloat16 pieces of 8 bits each
+// (exact: 11 and 24 bits), one product each.  So every product is exact and
+// only the float32 sums round.
 //
 // Tiles: 256 x 256 outputs to a pair of CTAs (cta_group::2: a CTA brings 128
 // channels of either operand, so each code is decoded for 256 outputs), or
@@ -18,11 +20,12 @@
 // order by a second kernel.
 //
 // Bound by the tensor cores with wide products, by decoding with narrow ones.
-// Measured, 131,072 positions, M 1,536, D 512: bfloat16 by bulk copies 175 us,
-// 1,180 TFLOP/s, 0.71 of the library product's measured rate (the decoding
+// Measured, 131,072 positions, M 1,536, D 512, 16-bit types by bulk copies: 175
+// us, 1,180 TFLOP/s, 0.71 of the library product's measured rate (the decoding
 // warps' fences and the hand-over of a stage leave the tensor pipe idle for the
-// rest); float16 and odd strides through registers 450 to 590 us; float32 with
-// M 768 620 to 670 us (three products each).  The runs' sum is 10 us more.
+// rest).  Through registers (odd strides) bfloat16 370 us and float16, in two
+// pieces, 450 to 590; float32 with M 768 620 to 670 us.  The runs' sum is 10 us
+// more.
 //
 // The tensor cores truncate their float32 sums (measured: 1.8e-8 of the result
 // for each 16 positions), which is nothing beside 16-bit dy.  For float32 the
@@ -118,10 +121,11 @@ __device__ __forceinline__ void commit_to(uint64_t* b) {
         "h"((uint16_t)3)
         : "memory");
 }
-template <int CG>
+template <int CG, class T>
 __device__ __forceinline__ void product(unsigned d, uint64_t a, uint64_t b, bool add) {
-  // float32 accumulator, bfloat16 operands, both MN-major, 128 CG x 128 CG
-  constexpr unsigned kind = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
+  // float32 accumulator, both operands of type T and MN-major, 128 CG x 128 CG
+  constexpr unsigned type = std::is_same<T, __half>::value ? 0 : 1;
+  constexpr unsigned kind = (1u << 4) | (type << 7) | (type << 10) | (1u << 15) | (1u << 16) |
                             ((unsigned)(kTile * CG >> 3) << 17) |
                             ((unsigned)(kTile * CG >> 4) << 24);
   if (CG == 1)
@@ -399,10 +403,10 @@ __global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kerne
         for (int j = 0; j < NP; ++j) {
           const uint64_t ad = operand(at + j * S::kOperand + k * 2048, S::kAtom);
           if (kApart)
-            product<CG>(tmem + (j ? 2 * kCols : buffer * kCols), ad, bd,
+            product<CG, __nv_bfloat16>(tmem + (j ? 2 * kCols : buffer * kCols), ad, bd,
                         j ? it > 0 || k > 0 || j > 1 : !opens || k > 0);
           else
-            product<CG>(tmem, ad, bd, it > 0 || k > 0 || j > 0);
+            product<CG, __nv_bfloat16>(tmem, ad, bd, it > 0 || k > 0 || j > 0);
         }
       }
       commit_to<CG>(&empty[slot]);
@@ -467,7 +471,9 @@ __global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kerne
 }
 
 // ---------------------------------------------------------------------------
-// bfloat16 dy whose positions are evenly spaced: the bulk-copy form.  One
+// bfloat16 dy, or float16 with a checkpoint of float16 values (both operands
+// float16 then: one product for the two of the pieces), whose positions are
+// evenly spaced: the bulk-copy form.  One
 // thread fetches codes and one dy (into the operand tile, swizzled) by TMA.
 // The decoding warps read their scales from global memory right after they
 // publish a stage, for the stage they take next, so that their fence before a
@@ -487,7 +493,7 @@ constexpr int kCodes = kStep * kTile;        // bytes of a stage's codes
 constexpr int kBulkBytes = kGroups * 2 * kOperand + kCodeSlots * kCodes + 1024;
 constexpr int kBulkThreads = 32 * (kDecoders + 4);
 
-template <int CG>
+template <class T, int CG>
 __global__ void __launch_bounds__(kBulkThreads, 1)
     weight_grad_bulk_kernel(const GradArgs a, const __grid_constant__ CUtensorMap dy_map,
                             const __grid_constant__ CUtensorMap code_map) {
@@ -591,8 +597,9 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
       for (int p = 0; p < kPasses; ++p) {
         const uint2 q = *reinterpret_cast<const uint2*>(codes + p * kRows * kTile);
         const unsigned bytes = __shfl_sync(~0u, scale, (row0 & 1) + 2 * p);
+        const uint8_t byte = (uint8_t)(bytes >> (col >> 2) * 8);
         *reinterpret_cast<uint4*>(base + kOperand + p * kRows * 128) =
-            pack_decode(q, (uint8_t)(bytes >> (col >> 2) * 8));
+            std::is_same<T, __half>::value ? pack_decode_half(q, byte) : pack_decode(q, byte);
       }
       __syncwarp();
       if (lane == 0) barrier_arrive<1>(&code_free[cs]);
@@ -620,7 +627,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
         const uint64_t ad = operand(at, kAtom), bd = operand(at + kOperand, kAtom);
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k)  // 16 positions are 2048 bytes
-          product<CG>(tmem, ad + k * (2048 >> 4), bd + k * (2048 >> 4), it > 0 || k > 0);
+          product<CG, T>(tmem, ad + k * (2048 >> 4), bd + k * (2048 >> 4), it > 0 || k > 0);
         commit_to<CG>(&empty[slot]);
         if (it == steps - 1) commit_to<CG>(&ready);
       }
@@ -772,7 +779,7 @@ int launch(const GradArgs& a, int runs, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? SEMICRF_OK : SEMICRF_ERR_CUDA;
 }
 
-// (width, rows) bytes or bfloat16 values, in boxes of one stage's positions
+// (width, rows) bytes or 16-bit values, in boxes of one stage's positions
 bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t width,
               int64_t rows, int64_t row_bytes, int box, CUtensorMapSwizzle swizzle) {
   const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
@@ -781,15 +788,18 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int6
   return make_tensor_map(map, type, 2, base, dims, strides, boxes, swizzle);
 }
 
-template <int CG>
+template <class T, int CG>
 int launch_bulk(const GradArgs& a, int runs, cudaStream_t stream) {
-  const auto kernel = weight_grad_bulk_kernel<CG>;
+  const auto kernel = weight_grad_bulk_kernel<T, CG>;
   CUtensorMap dy, codes;
   // the runtime's call comes first: it gives a thread that has none yet the
   // device's context, which encoding a map needs
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkBytes) !=
           cudaSuccess ||
-      !make_map(&dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.dy, a.M, a.N, a.st * 2, 64,
+      !make_map(&dy,
+                std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                a.dy, a.M, a.N, a.st * 2, 64,
                 CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_map(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, a.Dp, a.N, a.Dp, kTile,
                 CU_TENSOR_MAP_SWIZZLE_NONE))
@@ -810,6 +820,10 @@ int launch_bulk(const GradArgs& a, int runs, cudaStream_t stream) {
 }
 
 template <class T>
+int launch_bulk_group(const GradArgs& a, const Plan& p, cudaStream_t stream) {
+  return p.group == 2 ? launch_bulk<T, 2>(a, p.runs, stream) : launch_bulk<T, 1>(a, p.runs, stream);
+}
+template <class T>
 int launch_group(const GradArgs& a, const Plan& p, cudaStream_t stream) {
   return p.group == 2 ? launch<T, 2>(a, p.runs, stream) : launch<T, 1>(a, p.runs, stream);
 }
@@ -822,7 +836,7 @@ size_t packed_weight_grad_workspace_bytes(int64_t B, int64_t T, int64_t D, int64
   return sizeof(float) * p.runs * p.tiles_m * kTile * p.tiles_d * p.group * kTile;
 }
 
-int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
+int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype, int packed_dtype,
                        const semicrf_sequence& dy, const int8_t* codes, const uint8_t* scales,
                        const int64_t* lengths, int out_dtype, void* out, void* workspace,
                        cudaStream_t stream) {
@@ -848,20 +862,19 @@ int packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
   a.tiles_d = p.tiles_d;
   a.partial = static_cast<float*>(workspace);
   if (a.flat) a.st = T > 1 ? a.st : B > 1 ? a.sb : (M + 7) / 8 * 8;
+  // bulk copies want aligned rows at one distance, and a row index in 31 bits
+  const bool bulk = a.vec && a.N && a.N < (1ll << 31) - kStep &&
+                    reinterpret_cast<uintptr_t>(codes) % 16 == 0 && a.flat && a.st >= M &&
+                    a.st < (1ll << 36);
   int st;
-  switch (dtype) {
-    case SEMICRF_F32: st = launch<float, 1>(a, p.runs, stream); break;
-    case SEMICRF_BF16:
-      // bulk copies want aligned rows at one distance, and a row index in 31 bits
-      if (a.vec && a.N && a.N < (1ll << 31) - kStep && reinterpret_cast<uintptr_t>(codes) % 16 == 0 &&
-          a.flat && a.st >= M && a.st < (1ll << 36)) {
-        st = p.group == 2 ? launch_bulk<2>(a, p.runs, stream) : launch_bulk<1>(a, p.runs, stream);
-      } else {
-        st = launch_group<__nv_bfloat16>(a, p, stream);
-      }
-      break;
-    default: st = launch_group<__half>(a, p, stream);
-  }
+  if (dtype == SEMICRF_F32)
+    st = launch<float, 1>(a, p.runs, stream);
+  else if (dtype == SEMICRF_BF16)
+    st = bulk ? launch_bulk_group<__nv_bfloat16>(a, p, stream)
+              : launch_group<__nv_bfloat16>(a, p, stream);
+  else
+    st = bulk && packed_dtype == SEMICRF_F16 ? launch_bulk_group<__half>(a, p, stream)
+                                             : launch_group<__half>(a, p, stream);
   if (st != SEMICRF_OK) return st;
   const dim3 grid((unsigned)((M + 31) / 32), (unsigned)((D + 31) / 32));
   const int64_t cols = (int64_t)p.tiles_d * p.group * kTile;

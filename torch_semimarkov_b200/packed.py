@@ -84,17 +84,18 @@ def packed_weight_grad(grad_output: torch.Tensor, packed: PackedActivation,
         raise ValueError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     lengths = _lib.valid_lengths(lengths, B, T, grad_output.device)
     return _lib.packed_weight_grad(grad_output, packed.codes, packed.scales, packed.channels,
-                                   lengths, dtype)
+                                   packed.dtype, lengths, dtype)
 
 
 class _PackedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, codes, scales, lengths):
+    def forward(ctx, x, weight, bias, packed, lengths):
         w = weight.to(x.dtype)
         y = torch.matmul(x, w.t())
         if bias is not None:
             y += bias.to(x.dtype)
-        ctx.save_for_backward(weight, codes, scales, lengths)
+        ctx.save_for_backward(weight, packed.codes, packed.scales, lengths)
+        ctx.packed_dtype = packed.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
@@ -107,15 +108,15 @@ class _PackedLinear(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             gx = torch.matmul(grad, weight.to(grad.dtype))
         if ctx.needs_input_grad[1]:
-            gw = _lib.packed_weight_grad(grad, codes, scales, weight.shape[1], lengths,
-                                         weight.dtype)
+            gw = _lib.packed_weight_grad(grad, codes, scales, weight.shape[1], ctx.packed_dtype,
+                                         lengths, weight.dtype)
         if ctx.needs_input_grad[2]:
             if lengths is not None:
                 T = grad.shape[1]
                 live = torch.arange(T, device=grad.device) < lengths[:, None]
                 grad = grad.masked_fill(~live[..., None], 0.0)
             gb = grad.sum((0, 1), dtype=torch.float32).to(ctx.bias_dtype)
-        return gx, gw, gb, None, None, None
+        return gx, gw, gb, None, None
 
 
 def packed_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -149,4 +150,4 @@ def packed_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         _check(packed)
         if packed.shape != x.shape or packed.codes.device != x.device:
             raise ValueError(f"packed holds {tuple(packed.shape)}, x is {tuple(x.shape)}")
-    return _PackedLinear.apply(x, weight, bias, packed.codes, packed.scales, lengths)
+    return _PackedLinear.apply(x, weight, bias, packed, lengths)
