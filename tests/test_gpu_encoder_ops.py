@@ -435,6 +435,23 @@ def test_norm_rows_that_share_a_warp(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("D", [2, 29, 37, 61, 65, 100])
+def test_norm_narrow_rows_without_alignment(dtype, D):
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(D + 11)
+    B, T = 5, 37
+    n = torch.tensor([37, 0, 18, 1, 36], device=_dev())
+    t, w = _norm_inputs(g, B, T, D, dtype, n)
+    dr = _spoil(_normal(g, B, T, D, dtype=dtype), n, float("nan"))
+    dn = _spoil(_normal(g, B, T, D, dtype=dtype), n, float("inf"))
+    _check_norm(t, w, n, dr, dn)
+    _, y, p = tsm.gated_residual_norm(*t.values(), *w.values(), lengths=n, pack=True)
+    q = tsm.pack_activation(y)
+    assert torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("B,T", [(1, 1), (1, 5), (2, 1500), (40, 60)])
 def test_norm_row_counts(dtype, B, T):
     g = _gen(B * T)

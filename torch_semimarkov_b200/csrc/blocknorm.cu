@@ -26,7 +26,7 @@
 // to 1.5 times their bytes' time at the copy rate, up to 4,096; wider rows have
 // one CTA an SM, and of 16-bit types a ring beside which the weights find no
 // room: 8,192 takes 2.8 and 4.1 times it.  Rows without 16-byte alignment go
-// value by value: 203 channels 1.7 times.
+// value by value: 1.0 to 1.7 times for float32, 1.5 to 3 for 16-bit types.
 
 #include <algorithm>
 #include <type_traits>
@@ -86,7 +86,8 @@ struct Layout {
   static constexpr int H = PER / 2;                   // pairs of a lane
   static constexpr int NL = 32 * WR / SPLIT;          // lanes of a row
   static constexpr int kRows = SPLIT * (WR >= 4 ? 1 : 4 / WR);  // rows that a CTA works on at once
-  static_assert(SPLIT == 1 || NL * V >= kPackGroup, "a row's lanes hold its groups' codes");
+  // whether the lanes that share a group of the checkpoint share a row
+  static constexpr bool kCodes = NL * V >= kPackGroup;
   static constexpr int kThreads = NL * kRows;
   // CTAs of the backward on an SM: 8 warps of 24 channels a lane (255 registers),
   // 12 of 16 (168), 16 of 8 (128), 24 of 4 (80)
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArg
       for (int i = 0; i < H; ++i) out.set(i, both(0.f));
       if (BRANCH) out.put(a.r.row(b, t), l, ok);
       out.put(a.n.row(b, t), l, ok);
-      if (a.codes) put_codes<T, L>(a, row, l, ok, out);
+      if (L::kCodes && a.codes) put_codes<T, L>(a, row, l, ok, out);
       continue;
     }
     if constexpr (!RING) {
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArg
 #pragma unroll
     for (int i = 0; i < H; ++i) out.set(i, __fmul2_rn(__fmul2_rn(r[i], both(rr)), weight.w2(i)));
     out.put(a.n.row(b, t), l, ok);
-    if (a.codes) put_codes<T, L>(a, row, l, ok, out);
+    if (L::kCodes && a.codes) put_codes<T, L>(a, row, l, ok, out);
   }
   if (RING) asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -580,11 +581,12 @@ int launch(const NormArgs<T>& a, bool backward, float* grad_weights, cudaStream_
   return launch_status();
 }
 
-// The first of the layouts whose lanes hold a row.
+// The first of the layouts whose lanes hold a row, and its codes where wanted.
 template <class T, bool BRANCH, class L, class... Wider>
 int launch_first(const NormArgs<T>& a, bool backward, float* gw, cudaStream_t s) {
   if constexpr (sizeof...(Wider) > 0)
-    if (a.D > L::NL * L::PER) return launch_first<T, BRANCH, Wider...>(a, backward, gw, s);
+    if (a.D > L::NL * L::PER || (a.codes && !L::kCodes))
+      return launch_first<T, BRANCH, Wider...>(a, backward, gw, s);
   return launch<T, L, BRANCH>(a, backward, gw, s);
 }
 
@@ -592,7 +594,9 @@ int launch_first(const NormArgs<T>& a, bool backward, float* gw, cudaStream_t s)
 // 16 or 24 channels a lane, few idle ones at any width, since the more a lane
 // holds the more of its arithmetic overlaps (eight, one row to a warp: width
 // 256 backward 236 us for the 218 of sixteen and two rows; width 64 in a whole
-// warp 618 us for 232).  Else 8, at most 16 warps.
+// warp 618 us for 232).  Else 4 or 8, at most 16 warps; narrow rows share a
+// warp there too, unless their codes are wanted (37 channels without alignment,
+// backward, 1036 us in a whole warp and 538 in half of one).
 template <class T, int V, bool BRANCH>
 int launch_width(const NormArgs<T>& a, bool backward, float* gw, cudaStream_t s) {
   if constexpr (V == 8)
@@ -608,7 +612,8 @@ int launch_width(const NormArgs<T>& a, bool backward, float* gw, cudaStream_t s)
                         Layout<T, V, 4, 8>, Layout<T, V, 8, 8>, Layout<T, V, 16, 8>,
                         Layout<T, V, 16, 16>>(a, backward, gw, s);
   else
-    return launch_first<T, BRANCH, Layout<T, V, 1, 4>, Layout<T, V, 1, 8>, Layout<T, V, 2, 8>,
+    return launch_first<T, BRANCH, Layout<T, V, 1, 4, 4>, Layout<T, V, 1, 4, 2>,
+                        Layout<T, V, 1, 4>, Layout<T, V, 1, 8>, Layout<T, V, 2, 8>,
                         Layout<T, V, 4, 8>, Layout<T, V, 8, 8>, Layout<T, V, 16, 8>,
                         Layout<T, V, 16, 16>>(a, backward, gw, s);
 }
