@@ -3,7 +3,7 @@
 // Both directions are one pass, bound by memory: 2 + 1 + 1/32 bytes an
 // element for 16-bit activations.  A lane takes 16 bytes of a row, so the
 // lanes of a group of 32 channels are neighbours and its maximum is a few
-// shuffles.  A thread keeps its columns and takes kUnroll rows, all requested
+// shuffles.  A thread keeps its columns and takes 4 rows, all requested
 // before the first is used.
 //
 // Measured, bfloat16, 10^6 x 512: storing 278 us, reading back 265 us, 3.03
@@ -12,7 +12,8 @@
 // Rows that do not start on 16-byte boundaries are packed by the same lanes,
 // which load value by value (64 x 5,000 x 203: 65 us; lanes of one value each,
 // 182 us).  Reading back, such rows are written by lanes of one value, whose
-// neighbours' stores join (88 us; by the wide lanes 186 us).
+// neighbours' stores join, 8 rows to a thread (74 us; with 4 rows 88 us; by the
+// wide lanes 186 us).
 
 #include <algorithm>
 #include <type_traits>
@@ -22,7 +23,11 @@
 namespace semicrf {
 namespace {
 
-constexpr int kThreads = 256, kUnroll = 4;
+constexpr int kThreads = 256;
+// rows of a thread: more where its values are single ones (2, 8 and 16 rows of
+// vectors or 4 and 16 of single values are slower)
+template <int V>
+constexpr int kUnroll = V == 1 ? 8 : 4;
 
 // A lane's values, the first `left` of them where rows are not ALIGNED.
 template <class T, int V, bool ALIGNED>
@@ -43,15 +48,16 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, Places pla
                                                         const int64_t* __restrict__ lengths,
                                                         int8_t* __restrict__ codes,
                                                         uint8_t* __restrict__ scales) {
-  const int64_t first = ((int64_t)blockIdx.x * kUnroll) * blockDim.y + threadIdx.y;
+  constexpr int kRows = kUnroll<V>;
+  const int64_t first = ((int64_t)blockIdx.x * kRows) * blockDim.y + threadIdx.y;
   const int64_t d = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
   const int deep = blockDim.y;
-  const int left = (int)min((rows - first + deep - 1) / deep, (int64_t)kUnroll);  // rows here
+  const int left = (int)min((rows - first + deep - 1) / deep, (int64_t)kRows);  // rows here
   const bool in = d < D;
-  Pack<T, V> q[kUnroll];
+  Pack<T, V> q[kRows];
   const T* src = x.p + first * x.st + d;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kRows; ++u) {
 #pragma unroll
     for (int k = 0; k < V; ++k) q[u].v[k] = from_f32<T>(0.f);
     if (u < left && in) {
@@ -69,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, Places pla
   codes += first * G * kPackGroup + d;
   scales += first * G + d / kPackGroup;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kRows; ++u) {
     Pack<int8_t, V> c;
     const uint8_t byte = pack_encode(q[u], c);  // lanes past the end hold zeros
     if (u < left && stored) {
@@ -86,17 +92,18 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(int64_t rows, int64_t 
                                                           const int8_t* __restrict__ codes,
                                                           const uint8_t* __restrict__ scales,
                                                           T* __restrict__ out) {
-  const int64_t first = ((int64_t)blockIdx.x * kUnroll) * blockDim.y + threadIdx.y;
+  constexpr int kRows = kUnroll<V>;
+  const int64_t first = ((int64_t)blockIdx.x * kRows) * blockDim.y + threadIdx.y;
   const int64_t d = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
   const int deep = blockDim.y;
-  const int left = (int)min((rows - first + deep - 1) / deep, (int64_t)kUnroll);  // rows here
+  const int left = (int)min((rows - first + deep - 1) / deep, (int64_t)kRows);  // rows here
   if (d >= D) return;
-  Pack<int8_t, V> c[kUnroll];
-  uint8_t byte[kUnroll];
+  Pack<int8_t, V> c[kRows];
+  uint8_t byte[kRows];
   codes += first * G * kPackGroup + d;
   scales += first * G + d / kPackGroup;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kRows; ++u) {
     if (u < left) {
       byte[u] = *scales;
       c[u] = *reinterpret_cast<const Pack<int8_t, V>*>(codes);
@@ -106,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(int64_t rows, int64_t 
   }
   out += first * D + d;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kRows; ++u) {
     if (u < left) {
       Pack<T, V> q;
       if constexpr (V == 8 && std::is_same<T, __nv_bfloat16>::value) {
@@ -134,7 +141,7 @@ Grid grid_of(int64_t rows, int64_t G) {
   const int64_t per = G * (kPackGroup / V);
   const unsigned wide = (unsigned)std::min<int64_t>(per, kThreads), deep = kThreads / wide;
   const int64_t across = (per + wide - 1) / wide;
-  const int64_t down = (rows + (int64_t)deep * kUnroll - 1) / ((int64_t)deep * kUnroll);
+  const int64_t down = (rows + (int64_t)deep * kUnroll<V> - 1) / ((int64_t)deep * kUnroll<V>);
   return Grid{dim3((unsigned)down, (unsigned)across), dim3(wide, deep),
               down <= 0x7fffffff && across <= 65535};
 }
