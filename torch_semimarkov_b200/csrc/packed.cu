@@ -24,7 +24,7 @@ namespace semicrf {
 namespace {
 
 constexpr int kThreads = 256;
-// rows of a thread: more where its values are single ones (2, 8 and 16 rows of
+// rows of a thread: more where its values are single ones (2 and 8 rows of
 // vectors or 4 and 16 of single values are slower)
 template <int V>
 constexpr int kUnroll = V == 1 ? 8 : 4;
