@@ -1,0 +1,123 @@
+"""The encoder operators where their rules meet their limits: long sums,
+tensors whose rows overlap, gates and states at the ends of their types.
+
+Bounds follow from the operation count, as in encoder_reference."""
+
+import pytest
+import torch
+
+import encoder_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["fp32", "bf16", "fp16"]
+
+
+def _dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return torch.device("cuda:0")
+
+
+def _gen(seed):
+    return torch.Generator(device=_dev()).manual_seed(seed)
+
+
+def _normal(gen, *shape, dtype=torch.float32, scale=1.0, shift=0.0):
+    v = torch.randn(*shape, generator=gen, device=_dev()) * scale + shift
+    return v.to(dtype)
+
+
+def _offset(t):
+    """The same values in rows that do not start on 16-byte boundaries."""
+    wide = torch.empty(*t.shape[:-1], t.shape[-1] + 1, dtype=t.dtype, device=t.device)
+    wide[..., 1:] = t
+    return wide[..., 1:]
+
+
+# ---------------------------------------------------------------------------
+# weight gradient: sums of many positions
+# ---------------------------------------------------------------------------
+# Forms: rows of 16-bit types on 16-byte boundaries (bulk copies), others,
+# float16 over a checkpoint of another type (two pieces), float32 (three).
+FORMS = [("bf16", torch.bfloat16, True), ("bf16 unaligned", torch.bfloat16, False),
+         ("fp16", torch.float16, True), ("fp16 unaligned", torch.float16, False),
+         ("fp32", torch.float32, True), ("fp32 unaligned", torch.float32, False)]
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("M,D", [(2000, 1000), (1000, 500), (120, 96)])
+@pytest.mark.parametrize("form", FORMS, ids=[f[0] for f in FORMS])
+def test_weight_grad_sums_every_position_once(form, M, D, ragged):
+    """Values whose sums float32 holds exactly, in any order: not one position
+    may be missing or counted twice.  Runs of several thousand positions pass
+    through every slot and both halves of tensor memory several times.
+
+    16 bits: integers, at most 15,000 * 3 * 4 < 2^24.  float32: multiples of
+    2^-15 that need all three pieces (leading, 2^-7 and 2^-15), summed over
+    every 32nd channel value, so that sums stay below 2^9."""
+    import torch_semimarkov_b200 as tsm
+
+    _, dtype, aligned = form
+    g = _gen(M + ragged)
+    B, T = 3, 5000
+    sign = 1 - 2 * torch.randint(0, 2, (B, T, D), generator=g, device=_dev()).float()
+    if dtype == torch.float32:
+        some = torch.randint(0, 32, (B, T, D), generator=g, device=_dev()) == 0
+        x = sign * some
+        a, b, c = (torch.randint(lo, hi, (B, T, M), generator=g, device=_dev()).float()
+                   for lo, hi in ((1, 4), (0, 2), (0, 2)))
+        dy = a + b * 2.0 ** -7 + c * 2.0 ** -15
+    else:
+        x = sign * 2.0 ** torch.randint(0, 3, (B, T, D), generator=g, device=_dev())
+        dy = torch.randint(-3, 4, (B, T, M), generator=g, device=_dev()).float()
+    x, dy = x.to(dtype), dy.to(dtype)
+    n = torch.tensor([T, 4111, 0], device=_dev()) if ragged else None
+    p = tsm.pack_activation(x, n)
+    assert n is not None or torch.equal(p.unpack(), x)
+    got = tsm.packed_weight_grad(dy if aligned else _offset(dy), p, n, torch.float32)
+    live = torch.ones(B, T, 1, device=_dev()) if n is None else \
+        (torch.arange(T, device=_dev()) < n[:, None]).float()[..., None]
+    want = torch.matmul((dy.double() * live).view(-1, M).t(), x.double().view(-1, D))
+    if dtype == torch.float32:
+        assert float(want.abs().max()) < 2.0 ** 8  # and every part of a sum below 2^9
+    assert torch.equal(got.double(), want)
+
+
+LONG = [("bf16", torch.bfloat16, torch.bfloat16, True),
+        ("bf16 unaligned", torch.bfloat16, torch.bfloat16, False),
+        ("fp16", torch.float16, torch.float16, True),
+        ("fp16 over bf16", torch.float16, torch.bfloat16, True),
+        ("fp32", torch.float32, torch.float32, True)]
+
+
+@pytest.mark.parametrize("form", LONG, ids=[f[0] for f in LONG])
+def test_weight_grad_of_one_sign_does_not_shrink(form):
+    """131,072 positions of positive values in one run: the tensor cores' sums
+    truncate, always downwards, so the error may only be that of a segment.
+
+    Bound, of the result: a sum of 2,048 positions (512 for float32) grows
+    evenly through 128 (32) truncations for each piece, each at most 2^-23 of
+    what has been summed, half the final on average; the segments' sum rounds
+    as often as there are segments, at most 2^-24 of half the final on average.
+    A tenth is added for sums that do not grow quite evenly."""
+    import torch_semimarkov_b200 as tsm
+
+    _, dtype, stored, aligned = form
+    g = _gen(7)
+    N, D, M = 131072, 1024, 2560
+    x = torch.rand(1, N, D, generator=g, device=_dev()).add_(0.5).to(stored)
+    dy = torch.rand(1, N, M, generator=g, device=_dev()).add_(0.5).to(dtype)
+    if dtype == torch.float32:
+        dy = dy.bfloat16().float()  # the leading piece alone: its sums are the long ones
+    p = tsm.pack_activation(x)
+    got = tsm.packed_weight_grad(dy if aligned else _offset(dy), p, dtype=torch.float32)
+    rows, cols = torch.arange(0, M, 37, device=_dev()), torch.arange(0, D, 13, device=_dev())
+    v = p.unpack(torch.float32)[0][:, cols].double()
+    want = dy[0][:, rows].double().t() @ v
+    pieces = 2 if dtype != stored or (dtype == torch.float16 and not aligned) else 1
+    segment = 512 if dtype == torch.float32 else 2048
+    tol = 1.1 * (pieces * (segment / 16 + 1) / 2 * 2.0 ** -23
+                 + (N / segment + 1) / 2 * 2.0 ** -24)
+    err = ((got[rows][:, cols].double() - want) / want).abs().max()
+    assert err <= tol, (float(err), tol)

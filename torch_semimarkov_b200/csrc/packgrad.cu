@@ -20,17 +20,23 @@
 // order by a second kernel.
 //
 // Bound by the tensor cores with wide products, by decoding with narrow ones.
-// Measured, 131,072 positions, M 1,536, D 512, 16-bit types by bulk copies: 175
-// us, 1,180 TFLOP/s, 0.71 of the library product's measured rate (the decoding
-// warps' fences and the hand-over of a stage leave the tensor pipe idle for the
-// rest).  Through registers (odd strides) bfloat16 370 us and float16, in two
-// pieces, 450 to 590; float32 with M 768 620 to 670 us.  The runs' sum is 10 us
-// more.
+// Measured, 131,072 positions, M 1,536, D 512, the runs' sum (10 us) included,
+// 16-bit types by bulk copies: 187 us, 1,160 TFLOP/s in the product, 0.7 of the
+// library product's measured rate (the decoding warps' fences and the hand-over of
+// a stage leave the tensor pipe idle for the rest).  Through registers (odd strides)
+// bfloat16 351 us and float16, in two pieces, 433, over a bfloat16 checkpoint 600;
+// float32 with M 768 630 us.
 //
-// The tensor cores truncate their float32 sums (measured: 1.8e-8 of the result
-// for each 16 positions), which is nothing beside 16-bit dy.  For float32 the
-// leading piece is summed apart from the others and, every 512 positions,
-// moved from tensor memory to registers that round to nearest.
+// The tensor cores truncate their float32 sums, always towards zero, so a long
+// chain of them shrinks the result: values of one sign summed in one run of 131,072
+// positions lost 6.3e-4, of 640,000 4.0e-3 (two pieces 6.0e-3).  No chain is longer
+// than a segment: every kSums positions tensor memory is emptied into float32 sums
+// that round to nearest.  For 16-bit dy those are the partial result itself, to which
+// four warps of their own add one buffer of tensor memory while the next one fills.
+// For float32 they are registers, the segments shorter and the leading piece summed
+// apart from the others.  Errors then, at either length: 0.9e-6 for one piece, 5.2e-6
+// for two, 2e-7 for float32 (random signs 0.5e-6, 2.1e-6, 3e-7).  Segments of 1,024
+// positions would make them 0.4e-6 and 1.4e-6 and take 5% longer.
 
 #include <algorithm>
 #include <type_traits>
@@ -47,24 +53,36 @@ constexpr int kTile = 128;      // channels of dy, and of x, that a CTA brings
 constexpr int kStep = 64;       // positions of a stage
 constexpr int kAtom = kStep * 128;  // bytes of 64 channels of a stage: 64 rows of 128
 constexpr int kOperand = 2 * kAtom; // bytes of an operand of a stage
-constexpr int kReaders = 16;    // bulk form: warps that read tensor memory
+constexpr int kReaders = 16;    // 16-bit dy: warps that read the last segment's sums
+constexpr int kAdders = 4;      // 16-bit dy: warps that add the others', one a quarter of the rows
 constexpr int kGroupWarps = 4;  // warps that produce a stage together
+constexpr int kSums = 2048;     // 16-bit dy: positions of a segment
 
 template <class T>
 struct Form;  // pieces of a value; positions of a stage; warps that produce, that read tensor
-              // memory, and both (one more issues)
+              // memory at the end of a segment or of all, and both; warps after those: one
+              // issues, and the last kAdders add where others > 1
 template <>
 struct Form<__nv_bfloat16> {
   static constexpr int pieces = 1, step = 32, producers = 16, readers = 16, warps = 16;
+  static constexpr int others = 4 + kAdders;
 };
 template <>
 struct Form<__half> {
   static constexpr int pieces = 2, step = 32, producers = 16, readers = 16, warps = 16;
+  static constexpr int others = 4 + kAdders;
 };
 template <>
 struct Form<float> {
-  static constexpr int pieces = 3, step = 32, producers = 8, readers = 8, warps = 16;
+  static constexpr int pieces = 3, step = 32, producers = 8, readers = 8, warps = 16, others = 1;
 };
+
+// Registers a thread of the 16-bit forms: what the launch gives all of them, and
+// what the producing and the other warpgroups make of it.  With the same for all,
+// the rows on their way would spill (131,072 x 512 x 1,536 bfloat16: 495 us for
+// 351).  What is taken has to be what is given, or the warps that take would wait.
+constexpr int kLaunchRegs = 80, kProducerRegs = 96, kOtherRegs = 48;
+static_assert(16 * kProducerRegs + 8 * kOtherRegs == 24 * kLaunchRegs, "of 16 and 8 warps");
 
 template <class T>
 struct Shape {
@@ -163,6 +181,81 @@ __device__ __forceinline__ void read_columns(unsigned at, float (&f)[16]) {
 #pragma unroll
   for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(v[k]);
 }
+// Adds N columns of this warp's rows of tensor memory to a tile of the partial
+// result, a lane's row at `out` and its columns kTile apart; the first segment's
+// are stored as they are.  The sums are formed in L2, by additions that no one
+// waits for: read here and written back they took half as long again (2,048
+// positions of 147 tiles are 19 MB).  One CTA adds to an address, a segment
+// after the other, so the order is fixed.  L2 rounds to nearest and takes
+// subnormal numbers for zeros.
+template <int N>
+__device__ __forceinline__ void add_columns(unsigned at, float* out, bool first) {
+  float v[16];
+#pragma unroll 2
+  for (int c = 0; c < N; c += 16) {
+    float* p = out + (int64_t)c * kTile;
+    read_columns(at + c, v);
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (first)
+        __stcg(p + k * kTile, v[k]);
+      else
+        asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(p + k * kTile), "f"(v[k])
+                     : "memory");
+  }
+}
+// This lane's row of a quarter of a tile's rows, column 0.
+__device__ __forceinline__ float* partial_row(const GradArgs& a, int tm, int td, int cols,
+                                              int quarter) {
+  return a.partial +
+         (((int64_t)blockIdx.y * a.tiles_m + tm) * a.tiles_d + td) * cols * kTile + quarter * 32 +
+         (threadIdx.x & 31);
+}
+// Every segment's sums but the last one's, by one warp a quarter of the rows.
+// A buffer is `ready` when its segment's products are done, and `taken` when
+// all of these warps (of both CTAs) have read it, which the issuing thread
+// waits for; so no wait is more than one phase ahead of its barrier.
+template <int CG>
+__device__ __forceinline__ void add_segments(const GradArgs& a, int tm, int td, unsigned tmem,
+                                             int segments, uint64_t* ready, uint64_t* taken,
+                                             int* lost) {
+  constexpr int kCols = kTile * CG;
+  const int quarter = (int)(threadIdx.x >> 5) & 3;
+  float* const out = partial_row(a, tm, td, kCols, quarter);
+  for (int g = 0; g + 1 < segments; ++g) {
+    const int buffer = g & 1;
+    if (!__all_sync(~0u, barrier_wait(&ready[buffer], (unsigned)(g / 2) & 1))) {
+      *lost = 1;
+      return;
+    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    add_columns<kCols>(tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(buffer * kCols), out,
+                       g == 0);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) barrier_arrive<CG>(&taken[buffer]);
+  }
+}
+// The last segment's, by kReaders warps, after a barrier of the CTA.
+template <int CG>
+__device__ __forceinline__ void add_last_segment(const GradArgs& a, int tm, int td, unsigned tmem,
+                                                 int segments, uint64_t* ready, bool lost) {
+  constexpr int kCols = kTile * CG, kShare = kCols / (kReaders / 4);
+  const int warp = threadIdx.x >> 5, quarter = warp & 3, c0 = (warp >> 2) * kShare;
+  const int last = segments - 1, buffer = last & 1;
+  float* const out = partial_row(a, tm, td, kCols, quarter) + (int64_t)c0 * kTile;
+  const bool good = !lost && (!segments || __all_sync(~0u, barrier_wait(&ready[buffer],
+                                                                        (unsigned)(last / 2) & 1)));
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (segments && good) {
+    add_columns<kShare>(
+        tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(buffer * kCols + c0), out, last == 0);
+  } else {  // no positions: zeros; a wait that ran out shows as NaN
+#pragma unroll 16
+    for (int k = 0; k < kShare; ++k) out[k * kTile] = good ? 0.f : __uint_as_float(0x7fc00000u);
+  }
+}
+
 // Shared-memory operand, MN-major, 128-byte swizzle: 64 channels are one row
 // of 128 bytes, 8 positions 1024 bytes, the next 64 channels `atom` further.
 __device__ __forceinline__ uint64_t operand(unsigned addr, int atom) {
@@ -213,21 +306,23 @@ __device__ __forceinline__ void cut(const Pack<T, 8>& v, uint4 (&piece)[NP]) {
 // are no more groups than slots, so that wait is never more than one phase
 // ahead of its barrier.
 template <class T, int CG>
-__global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kernel(const GradArgs a) {
+__global__ void __launch_bounds__(32 * (Form<T>::warps + Form<T>::others), 1)
+    weight_grad_kernel(const GradArgs a) {
   using F = Form<T>;
   using S = Shape<T>;
   constexpr int NP = F::pieces, NS = S::kStages, STEP = F::step, W = F::warps;
   constexpr int kGroups = F::producers / kGroupWarps, kPart = 32 * kGroupWarps;
   constexpr int kPasses = STEP / 8;     // 16 threads a row, 8 rows at once
-  constexpr int kSegment = 512 / STEP;  // float32: stages that tensor memory sums
-  constexpr bool kApart = NP == 3;      // float32: segments, lower pieces apart
+  constexpr bool kApart = NP == 3;      // float32: lower pieces apart, sums in registers
+  constexpr int kSegment = (kApart ? 512 : kSums) / STEP;  // stages that tensor memory sums
   constexpr int kCols = kTile * CG;     // columns of the accumulator
-  constexpr int kTmem = kApart ? 512 : kCols;
+  constexpr int kTmem = kApart ? 512 : 2 * kCols;
   static_assert(!kApart || CG == 1, "tensor memory holds two segments and the lower pieces");
   static_assert(kGroups <= NS, "see above");
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[NS], empty[NS], ready[2], taken[2];
   __shared__ unsigned tmem_at;
+  __shared__ int lost;
   unsigned char* ring = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -238,15 +333,17 @@ __global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kerne
   const int64_t left = a.N - first;
   const int count = (int)(left < a.run ? (left < 0 ? 0 : left) : a.run);
   const int steps = (count + STEP - 1) / STEP;
+  const int segments = (steps + kSegment - 1) / kSegment;
 
   if (tid == 0) {
+    lost = 0;
     for (int s = 0; s < NS; ++s) {
       barrier_init(&full[s], kGroupWarps * CG);
       barrier_init(&empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       barrier_init(&ready[s], 1);
-      barrier_init(&taken[s], F::readers);
+      barrier_init(&taken[s], kApart ? F::readers : kAdders * CG);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -272,6 +369,13 @@ __global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kerne
   const unsigned tmem = tmem_at;
 
   bool ok = true;
+  if constexpr (!kApart) {
+    static_assert(F::producers == 16 && W + F::others == 24, "see kLaunchRegs");
+    if (warp < F::producers)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  }
   if (warp < F::producers) {
     // this thread's 8 channels of dy and of x, and its first row of a stage
     const int group = tid / kPart, col = tid & 15, row0 = tid % kPart >> 4;
@@ -387,38 +491,47 @@ __global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kerne
     else
       produce(std::false_type());
   } else if (warp == W && lane == 0 && rank == 0) {
-    for (int it = 0; it < steps; ++it) {
-      const int slot = it % NS, segment = it / kSegment, buffer = kApart ? segment & 1 : 0;
-      const bool opens = kApart ? it % kSegment == 0 : it == 0;
-      if (kApart && opens && segment >= 2)
-        ok = barrier_wait(&taken[buffer], (unsigned)(segment / 2 - 1) & 1);
-      ok = ok && barrier_wait(&full[slot], (unsigned)(it / NS) & 1);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const unsigned at = smem_addr(ring + slot * S::kStage);
+    int slot = 0;
+    unsigned parity = 0;
+    for (int segment = 0; segment < segments && ok; ++segment) {
+      const int buffer = segment & 1, n = min(steps - segment * kSegment, kSegment);
+      const unsigned sums = tmem + buffer * kCols;
+      if (segment >= 2) ok = barrier_wait(&taken[buffer], (unsigned)(segment / 2 - 1) & 1);
+      for (int i = 0; i < n; ++i) {
+        ok = ok && barrier_wait(&full[slot], parity);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const unsigned at = smem_addr(ring + slot * S::kStage);
 #pragma unroll
-      for (int k = 0; k < STEP / 16; ++k) {
-        const uint64_t bd = operand(at + NP * S::kOperand + k * 2048, S::kAtom);
+        for (int k = 0; k < STEP / 16; ++k) {
+          const uint64_t bd = operand(at + NP * S::kOperand + k * 2048, S::kAtom);
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          const uint64_t ad = operand(at + j * S::kOperand + k * 2048, S::kAtom);
-          if (kApart)
-            product<CG, __nv_bfloat16>(tmem + (j ? 2 * kCols : buffer * kCols), ad, bd,
-                        j ? it > 0 || k > 0 || j > 1 : !opens || k > 0);
-          else
-            product<CG, __nv_bfloat16>(tmem, ad, bd, it > 0 || k > 0 || j > 0);
+          for (int j = 0; j < NP; ++j) {
+            const uint64_t ad = operand(at + j * S::kOperand + k * 2048, S::kAtom);
+            if (kApart && j)
+              product<CG, __nv_bfloat16>(tmem + 2 * kCols, ad, bd,
+                                         segment > 0 || i > 0 || k > 0 || j > 1);
+            else
+              product<CG, __nv_bfloat16>(sums, ad, bd, i > 0 || k > 0 || j > 0);
+          }
         }
+        commit_to<CG>(&empty[slot]);
+        if (++slot == NS) slot = 0, parity ^= 1;
       }
-      commit_to<CG>(&empty[slot]);
-      if (it == steps - 1 || (kApart && it % kSegment == kSegment - 1))
-        commit_to<CG>(&ready[buffer]);
+      if (ok) commit_to<CG>(&ready[buffer]);
     }
+  } else if (!kApart && warp >= W + F::others - kAdders) {
+    add_segments<CG>(a, tm, td, tmem, segments, ready, taken, &lost);
   }
   __syncwarp();
 
   // Tensor memory to the partial result: a warp reads its 32 lanes (rows of
   // the tile) and a share of the columns; a column's rows are contiguous.
-  if (warp >= W - F::readers && warp < W) {
+  if constexpr (!kApart) {
+    static_assert(F::readers == kReaders, "the warps that read the last segment");
+    __syncthreads();
+    if (warp < kReaders) add_last_segment<CG>(a, tm, td, tmem, segments, ready, lost != 0);
+  } else if (warp >= W - F::readers && warp < W) {
     constexpr int kShare = kCols / (F::readers / 4);
     static_assert(kShare % 16 == 0, "a warp reads 16 columns at once");
     const int quarter = warp & 3, c0 = (warp - (W - F::readers)) / 4 * kShare;
@@ -426,7 +539,6 @@ __global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kerne
     float sum[kShare];
 #pragma unroll
     for (int k = 0; k < kShare; ++k) sum[k] = 0.f;
-    const int segments = !steps ? 0 : kApart ? (steps + kSegment - 1) / kSegment : 1;
     bool good = true;
     for (int g = 0; g < segments && good; ++g) {
       const int buffer = g & 1;
@@ -439,21 +551,17 @@ __global__ void __launch_bounds__(32 * Form<T>::warps + 32, 1) weight_grad_kerne
         read_columns(at + buffer * kCols + c, v);
 #pragma unroll
         for (int k = 0; k < 16; ++k) sum[c + k] += v[k];
-        if (kApart && g == segments - 1) {
+        if (g == segments - 1) {
           read_columns(at + 2 * kCols + c, v);
 #pragma unroll
           for (int k = 0; k < 16; ++k) sum[c + k] += v[k];
         }
       }
-      if (kApart) {
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) barrier_arrive<1>(&taken[buffer]);
-      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) barrier_arrive<1>(&taken[buffer]);
     }
-    float* out = a.partial +
-                 ((((int64_t)blockIdx.y * a.tiles_m + tm) * a.tiles_d + td) * kCols + c0) * kTile +
-                 quarter * 32 + lane;
+    float* out = partial_row(a, tm, td, kCols, quarter) + (int64_t)c0 * kTile;
 #pragma unroll
     for (int k = 0; k < kShare; ++k)  // a wait that ran out shows as NaN
       out[(int64_t)k * kTile] = good ? sum[k] : __uint_as_float(0x7fc00000u);
@@ -491,16 +599,19 @@ constexpr int kDecoders = kGroups * kGroupWarps;
 constexpr int kCodeSlots = 7;
 constexpr int kCodes = kStep * kTile;        // bytes of a stage's codes
 constexpr int kBulkBytes = kGroups * 2 * kOperand + kCodeSlots * kCodes + 1024;
-constexpr int kBulkThreads = 32 * (kDecoders + 4);
+constexpr int kBulkThreads = 32 * (kDecoders + 4 + kAdders);
 
 template <class T, int CG>
 __global__ void __launch_bounds__(kBulkThreads, 1)
     weight_grad_bulk_kernel(const GradArgs a, const __grid_constant__ CUtensorMap dy_map,
                             const __grid_constant__ CUtensorMap code_map) {
-  constexpr int NS = kGroups, NC = kCodeSlots, kCols = kTile * CG;
+  constexpr int NS = kGroups, NC = kCodeSlots, kCols = kTile * CG, kTmem = 2 * kCols;
+  constexpr int kSegment = kSums / kStep;  // stages that tensor memory sums
   extern __shared__ unsigned char raw[];
-  __shared__ uint64_t code_landed[NC], code_free[NC], dy_landed[NS], full[NS], empty[NS], ready;
+  __shared__ uint64_t code_landed[NC], code_free[NC], dy_landed[NS], full[NS], empty[NS];
+  __shared__ uint64_t ready[2], taken[2];
   __shared__ unsigned tmem_at;
+  __shared__ int lost;
   unsigned char* ring = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   unsigned char* code_ring = ring + NS * 2 * kOperand;
@@ -512,8 +623,10 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
   const int64_t left = a.N - first;
   const int count = (int)(left < a.run ? (left < 0 ? 0 : left) : a.run);
   const int steps = (count + kStep - 1) / kStep;
+  const int segments = (steps + kSegment - 1) / kSegment;
 
   if (tid == 0) {
+    lost = 0;
     for (int s = 0; s < NC; ++s) {
       barrier_init(&code_landed[s], 1);
       barrier_init(&code_free[s], kGroupWarps);
@@ -523,20 +636,23 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
       barrier_init(&full[s], (kGroupWarps + 1) * CG);  // each CTA's group, and its dy
       barrier_init(&empty[s], 1);
     }
-    barrier_init(&ready, 1);
+    for (int s = 0; s < 2; ++s) {
+      barrier_init(&ready[s], 1);
+      barrier_init(&taken[s], kAdders * CG);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kDecoders) {
     if (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                        smem_addr(&tmem_at)),
-                   "n"(kCols)
+                   "n"(kTmem)
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                        smem_addr(&tmem_at)),
-                   "n"(kCols)
+                   "n"(kTmem)
                    : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
@@ -617,20 +733,28 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
       request(it + kGroups);
     }
   } else if (warp == kDecoders) {
-    if (lane == 0 && rank == 0)
-      for (int it = 0; it < steps; ++it) {
-        const int slot = it % NS;
-        ok = barrier_wait(&full[slot], (unsigned)(it / NS) & 1);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const unsigned at = smem_addr(ring + slot * 2 * kOperand);
-        const uint64_t ad = operand(at, kAtom), bd = operand(at + kOperand, kAtom);
+    if (lane == 0 && rank == 0) {
+      int slot = 0;
+      unsigned parity = 0;
+      for (int segment = 0; segment < segments && ok; ++segment) {
+        const int buffer = segment & 1, n = min(steps - segment * kSegment, kSegment);
+        const unsigned sums = tmem + buffer * kCols;
+        if (segment >= 2) ok = barrier_wait(&taken[buffer], (unsigned)(segment / 2 - 1) & 1);
+        for (int i = 0; i < n; ++i) {
+          ok = ok && barrier_wait(&full[slot], parity);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const unsigned at = smem_addr(ring + slot * 2 * kOperand);
+          const uint64_t ad = operand(at, kAtom), bd = operand(at + kOperand, kAtom);
 #pragma unroll
-        for (int k = 0; k < kStep / 16; ++k)  // 16 positions are 2048 bytes
-          product<CG, T>(tmem, ad + k * (2048 >> 4), bd + k * (2048 >> 4), it > 0 || k > 0);
-        commit_to<CG>(&empty[slot]);
-        if (it == steps - 1) commit_to<CG>(&ready);
+          for (int k = 0; k < kStep / 16; ++k)  // 16 positions are 2048 bytes
+            product<CG, T>(sums, ad + k * (2048 >> 4), bd + k * (2048 >> 4), i > 0 || k > 0);
+          commit_to<CG>(&empty[slot]);
+          if (++slot == NS) slot = 0, parity ^= 1;
+        }
+        if (ok) commit_to<CG>(&ready[buffer]);
       }
+    }
   } else if (warp == kDecoders + 1) {
     if (lane == 0) {
       const int m0 = tm * kTile;
@@ -668,6 +792,8 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
       for (int k = it > NC ? it - NC : 0; k < it; ++k)
         barrier_wait(&code_landed[k % NC], (unsigned)(k / NC) & 1);
     }
+  } else if (warp > kDecoders + 3) {
+    add_segments<CG>(a, tm, td, tmem, segments, ready, taken, &lost);
   } else {
     if (lane == 0)
       for (int it = 0; it < steps; ++it) {
@@ -679,37 +805,17 @@ __global__ void __launch_bounds__(kBulkThreads, 1)
   }
   __syncwarp();
 
-  if (warp < kReaders) {
-    constexpr int kShare = kCols / (kReaders / 4);
-    const int quarter = warp & 3, c0 = (warp >> 2) * kShare;
-    const unsigned at = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c0;
-    const bool good = !steps || __all_sync(~0u, barrier_wait(&ready, 0));
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    float* out = a.partial +
-                 ((((int64_t)blockIdx.y * a.tiles_m + tm) * a.tiles_d + td) * kCols + c0) * kTile +
-                 quarter * 32 + lane;
-#pragma unroll
-    for (int c = 0; c < kShare; c += 16) {
-      float v[16];
-      if (steps && good) {
-        read_columns(at + c, v);
-      } else {  // no positions: zeros; a wait that ran out shows as NaN
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = good ? 0.f : __uint_as_float(0x7fc00000u);
-      }
-#pragma unroll
-      for (int k = 0; k < 16; ++k) out[(int64_t)(c + k) * kTile] = v[k];
-    }
-  }
+  __syncthreads();
+  if (warp < kReaders) add_last_segment<CG>(a, tm, td, tmem, segments, ready, lost != 0);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (CG > 1) sync_all<CG>();
   if (warp == kDecoders) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (CG == 1)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols));
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem));
     else
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols));
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem));
   }
 }
 
@@ -765,9 +871,14 @@ int launch(const GradArgs& a, int runs, cudaStream_t stream) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
       cudaSuccess)
     return SEMICRF_ERR_CUDA;
+  if (sizeof(T) == 2) {  // no launch with other registers than its warpgroups count on
+    cudaFuncAttributes at{};
+    if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess || at.numRegs != kLaunchRegs)
+      return SEMICRF_ERR_CUDA;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.tiles_m * a.tiles_d), (unsigned)runs);
-  cfg.blockDim = dim3(32 * Form<T>::warps + 32);
+  cfg.blockDim = dim3(32 * (Form<T>::warps + Form<T>::others));
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
