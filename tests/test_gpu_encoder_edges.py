@@ -121,3 +121,52 @@ def test_weight_grad_of_one_sign_does_not_shrink(form):
                  + (N / segment + 1) / 2 * 2.0 ** -24)
     err = ((got[rows][:, cols].double() - want) / want).abs().max()
     assert err <= tol, (float(err), tol)
+
+
+# ---------------------------------------------------------------------------
+# rows that overlap or are one and the same
+# ---------------------------------------------------------------------------
+def _overlapping(g, B, T, D, dtype):
+    """Windows of a signal (fewer and more positions than channels, by the
+    caller), rows a step of four apart, one sequence or one position for all."""
+    signal = _normal(g, B, T + D, dtype=dtype)
+    yield "windows", signal.unfold(1, D, 1)[:, :T]
+    yield "steps", _normal(g, B, 4 * T + D, dtype=dtype).unfold(1, D, 4)[:, :T]
+    yield "batch", _normal(g, 1, T, D, dtype=dtype).expand(B, T, D)
+    yield "time", _normal(g, B, 1, D, dtype=dtype).expand(B, T, D)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("B,T,D", [(3, 4, 10), (2, 70, 16), (2, 9, 64)])
+def test_overlapping_rows_equal_their_copies(dtype, B, T, D):
+    """Forward and backward of the recurrence and the norms on inputs whose rows
+    overlap: what contiguous copies of them give (rows that are loaded in other
+    units sum in another order: a few roundings)."""
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(T)
+    w = [_normal(g, D, scale=0.2, shift=1.0) for _ in range(3)]
+    dh, dn = _normal(g, B, T, D, dtype=dtype), _normal(g, B, T, D, dtype=dtype)
+    u = ref.UNIT[dtype]
+
+    def every(x):
+        leaves = [x.detach().requires_grad_(True) for _ in range(2)]
+        h, s = tsm.gated_linear_recurrence(*leaves)
+        out = [h, s, *torch.autograd.grad((h, s), leaves, (dh, s.detach()))]
+        leaves = [x.detach().requires_grad_(True) for _ in range(3)]
+        r, n = tsm.gated_residual_norm(*leaves, *w)
+        out += [r, n, *torch.autograd.grad((r, n), leaves, (dh, dn))]
+        leaf = x.detach().requires_grad_(True)
+        n = tsm.rms_norm(leaf, w[0])
+        out += [n, *torch.autograd.grad(n, leaf, dn)]
+        p = tsm.pack_activation(x)
+        return out + [p.codes, p.scales, tsm.packed_weight_grad(x, p)]
+
+    for how, x in _overlapping(g, B, T, D, dtype):
+        for a, b in zip(every(x), every(x.contiguous())):
+            if a.dtype in (torch.int8, torch.uint8):
+                assert torch.equal(a, b), how
+                continue
+            a, b = a.detach().double(), b.detach().double()
+            tol = 2 * u * b.abs() + 512 * ref.U32 * float(b.abs().max())
+            assert ((a - b).abs() <= tol).all(), (how, float((a - b).abs().max()))

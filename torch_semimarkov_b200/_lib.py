@@ -560,6 +560,17 @@ def activation(t, name: str, shape=None, like: Optional[torch.Tensor] = None) ->
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+def rows_like(t: torch.Tensor) -> torch.Tensor:
+    """A new tensor of t's shape and type whose channels are contiguous, as the
+    kernels write them.  Its other strides are in t's order where t's rows lie
+    apart; for rows that overlap (windows of a signal), empty_like makes strides
+    up, and may put other dimensions inside the channels."""
+    out = torch.empty_like(t)
+    if out.stride(2) != 1 and out.shape[2] != 1:
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return out
+
+
 def float_vector(t, name: str, shape, device) -> torch.Tensor:
     """A checked float32 copy (or the tensor itself) of a parameter or state."""
     if not isinstance(t, torch.Tensor) or not t.is_floating_point():
@@ -660,7 +671,7 @@ def recurrence_forward(x, gate, initial_state, lengths, reverse, want_saved):
     dev = x.device
     p = _recurrence(x, gate, initial_state, lengths, reverse)
     with _on(dev):
-        h = torch.empty_like(x)
+        h = rows_like(x)
         state = x.new_empty((B, D), dtype=torch.float32)
         need = lib.semicrf_recurrence_workspace_size(p)
         saved = None
@@ -680,7 +691,7 @@ def recurrence_backward(x, gate, lengths, reverse, saved, grad_h, grad_state, wa
     dev = x.device
     p = _recurrence(x, gate, None, lengths, reverse)
     with _on(dev):
-        gx, gg = torch.empty_like(x), torch.empty_like(gate)
+        gx, gg = rows_like(x), rows_like(gate)
         gi = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if want_initial else None
         need = lib.semicrf_recurrence_workspace_size(p)
         ws = _scratch(need, dev)
@@ -742,8 +753,8 @@ def block_norm_forward(residual, branch, gate, branch_weight, residual_scale, ne
     p = _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
                     eps)
     with _on(dev):
-        out = None if branch is None else torch.empty_like(residual)
-        normed = torch.empty_like(residual)
+        out = None if branch is None else rows_like(residual)
+        normed = rows_like(residual)
         stats = residual.new_empty((B, T, 2), dtype=torch.float32) if want_statistics else None
         codes, scales = packed_buffers(B, T, D, dev) if pack else (None, None)
         st = lib.semicrf_block_norm_forward(p, _sequence(out), _sequence(normed), _addr(stats),
@@ -763,10 +774,10 @@ def block_norm_backward(residual, branch, gate, branch_weight, residual_scale, n
     p = _block_norm(residual, branch, gate, branch_weight, residual_scale, next_weight, lengths,
                     eps)
     with _on(dev):
-        gr = torch.empty_like(residual)
+        gr = rows_like(residual)
         gb = gg = None
         if branch is not None:
-            gb, gg = torch.empty_like(branch), torch.empty_like(gate)
+            gb, gg = rows_like(branch), rows_like(gate)
         gw = residual.new_empty((3, D), dtype=torch.float32)
         ws = _scratch(lib.semicrf_block_norm_workspace_size(p), dev)
         st = lib.semicrf_block_norm_backward(p, stats.data_ptr(), _sequence(grad_out),
