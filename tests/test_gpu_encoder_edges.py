@@ -170,3 +170,30 @@ def test_overlapping_rows_equal_their_copies(dtype, B, T, D):
             a, b = a.detach().double(), b.detach().double()
             tol = 2 * u * b.abs() + 512 * ref.U32 * float(b.abs().max())
             assert ((a - b).abs() <= tol).all(), (how, float((a - b).abs().max()))
+
+
+# ---------------------------------------------------------------------------
+# padding of the encoder's features
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_encoder_padding_reaches_no_gradient(dtype, packed):
+    """NaN and infinities past each length: outputs and every parameter's
+    gradient are, bit for bit, those of zero padding."""
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(50)
+    B, T, n = 3, 40, torch.tensor([40, 13, 0])
+    live = ref.live_mask(n, B, T).to(_dev())[..., None]
+    x, target = _normal(g, B, T, 7), _normal(g, B, T, 24)
+    results = []
+    for how in (0.0, float("nan"), float("inf")):
+        torch.manual_seed(51)
+        enc = tsm.GatedRecurrentEncoder(7, 24, checkpoint_8bit=packed, dtype=dtype).to(_dev())
+        features = torch.where(live, x, torch.full_like(x, how)).requires_grad_(True)
+        y = enc(features, n)
+        (y.float() * target).sum().backward()
+        results.append([y.detach(), features.grad, *(p.grad for p in enc.parameters())])
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.isfinite(b).all() and torch.equal(a, b)
