@@ -197,3 +197,39 @@ def test_encoder_padding_reaches_no_gradient(dtype, packed):
     for other in results[1:]:
         for a, b in zip(results[0], other):
             assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# gates at the ends of their types
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("D", [37, 64, 512, 4100])
+def test_norm_gates_at_their_limits(dtype, D):
+    """silu is 0 at the lowest values of a type, as a masked gate has them, and
+    far into saturation; its slope too.  Bounds as for any other gate."""
+    from test_gpu_encoder_ops import _check_norm, _norm_inputs
+
+    g = _gen(D)
+    B, T = 2, 6
+    t, w = _norm_inputs(g, B, T, D, dtype)
+    low = torch.finfo(dtype).min
+    values = torch.tensor([low, low / 2, low / 1e4, -2e4, -200.0, -128.0, -100.0, -88.0, -80.0, 0.0,
+                           60.0, 200.0], device=_dev())
+    pick = torch.randint(0, len(values), (B, T, D), generator=g, device=_dev())
+    t["gate"] = values[pick].to(dtype)
+    dr, dn = _normal(g, B, T, D, dtype=dtype), _normal(g, B, T, D, dtype=dtype)
+    _check_norm(t, w, None, dr, dn)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_norm_gate_of_minus_infinity_closes_the_branch(dtype):
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(60)
+    x, z = (_normal(g, 2, 5, 72, dtype=dtype) for _ in range(2))
+    w = [torch.ones(72, device=_dev()) for _ in range(3)]
+    leaves = [v.requires_grad_(True) for v in (x, z, torch.full_like(x, float("-inf")))]
+    r, n = tsm.gated_residual_norm(*leaves, *w)
+    assert torch.equal(r, x) and torch.equal(n, tsm.rms_norm(x, w[2]))
+    _, gz, gg = torch.autograd.grad((r, n), leaves, (x.detach(), z.detach()))
+    assert float(gz.abs().max()) <= 1e-30 and float(gg.abs().max()) <= 1e-30

@@ -257,6 +257,14 @@ __device__ __forceinline__ void put_codes(const NormArgs<T>& a, int64_t row, int
   }
 }
 
+// A gate as the rows use it: below -128 its sigmoid is held to 2^-126, which times
+// a gate near the type's lowest value would not be silu's 0 any more (-4 at bfloat16's).
+__device__ __forceinline__ float2 held_gate(float2 g) {
+  asm("max.NaN.f32 %0, %0, 0fC3000000;" : "+f"(g.x));
+  asm("max.NaN.f32 %0, %0, 0fC3000000;" : "+f"(g.y));
+  return g;
+}
+
 template <class T, class L, bool BRANCH, bool RING>
 __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArgs<T> a) {
   constexpr int H = L::H, NL = L::NL;
@@ -321,7 +329,7 @@ __global__ void __launch_bounds__(L::kThreads) norm_forward_kernel(const NormArg
       r[i] = in.pair(kX, i);
       if (BRANCH) {
         float2 sig, neg;
-        const float2 g = in.pair(kG, i);
+        const float2 g = held_gate(in.pair(kG, i));
         sigmoid_pair2<T>(g, sig, neg);
         const float2 u = __fmul2_rn(__fmul2_rn(g, sig), weight.sw(i));
         r[i] = __ffma2_rn(u, __fmul2_rn(in.pair(kZ, i), both(rz)), r[i]);
@@ -419,7 +427,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_backward_kernel(c
       rh[i] = in.pair(kX, i);
       if (BRANCH) {
         float2 neg;
-        const float2 g = in.pair(kG, i);
+        const float2 g = held_gate(in.pair(kG, i));
         sigmoid_pair2<T>(g, sig[i], neg);
         rh[i] = __ffma2_rn(__fmul2_rn(__fmul2_rn(g, sig[i]), weight.sw(i)),
                            __fmul2_rn(in.pair(kZ, i), rz), rh[i]);
@@ -438,7 +446,8 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_backward_kernel(c
       const float2 d = __ffma2_rn(rr, __ffma2_rn(rh[i], c2, p), in.pair(kDr, i));
       out.set(i, d);
       if (BRANCH) {
-        const float2 zh = __fmul2_rn(in.pair(kZ, i), rz), g = in.pair(kG, i);
+        const float2 zh = __fmul2_rn(in.pair(kZ, i), rz),
+                     g = held_gate(in.pair(kG, i));
         const float2 du = __fmul2_rn(d, __fmul2_rn(g, sig[i]));
         acc[0][i] = __ffma2_rn(du, zh, acc[0][i]);
         // silu'(g) = sig (1 + g (1 - sig))
