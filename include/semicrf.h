@@ -302,7 +302,9 @@ int semicrf_block_norm_backward(const semicrf_block_norm* p, const float* statis
  * the byte e + 127 and its values as int8 codes rint(x / 2^e), no code past
  * the type's largest finite value.  A group of zeros has byte 0; one with a
  * value that is not finite has byte 255 and reads back as NaN.
- * codes (B*T, 32 * ceil(D/32)), zero beyond D; scales (B*T, ceil(D/32)). */
+ * codes (B*T, 32 * ceil(D/32)), zero beyond D, on a multiple of 8 bytes (any
+ * other address is refused, here and wherever codes are taken); scales
+ * (B*T, ceil(D/32)). */
 int semicrf_pack(int64_t B, int64_t T, int64_t D, int dtype, const semicrf_sequence* x,
                  const int64_t* lengths, int8_t* codes, uint8_t* scales, void* stream);
 /* out (rows, D), contiguous, of type dtype. */

@@ -34,3 +34,38 @@ def test_outputs_have_contiguous_channels_whatever_the_inputs_rows_do(B, T, D):
         assert max(seen) < out.untyped_storage().nbytes() // 4
     # an order of its own is kept
     assert _lib.rows_like(dense.transpose(0, 1)).stride() == dense.transpose(0, 1).stride()
+
+
+def test_misaligned_addresses_are_refused_before_any_launch():
+    """Codes are read 8 at a time, activations by their elements; an address
+    between them is an error code, not a launch."""
+    import ctypes
+
+    from torch_semimarkov_b200 import _lib
+
+    lib, bad = _lib.load(), _lib.SEMICRF_ERR_INVALID_ARGUMENT
+    good = ctypes.byref(_lib.SemicrfSequence(64, 40, 8))
+    odd = ctypes.byref(_lib.SemicrfSequence(65, 40, 8))
+    for at in (1025, 1026, 1028):
+        assert lib.semicrf_pack(2, 5, 8, 1, good, None, at, 4096, None) == bad
+        assert lib.semicrf_unpack(3, 8, 1, at, 4096, 8192, None) == bad
+        assert lib.semicrf_packed_weight_grad(2, 5, 8, 3, 1, good, at, 4096, 1, None, 0, 8192, 4096,
+                                              1 << 30, None) == bad
+        p = ctypes.byref(_lib.SemicrfBlockNorm(2, 5, 8, 1, 0.0, (64, 40, 8), (0, 0, 0), (0, 0, 0),
+                                               None, None, 64, None))
+        none = ctypes.byref(_lib.SemicrfSequence(None, 0, 0))
+        assert lib.semicrf_block_norm_forward(p, none, good, None, at, 4096, None) == bad
+    assert lib.semicrf_pack(2, 5, 8, 1, odd, None, 1024, 4096, None) == bad
+    p = ctypes.byref(_lib.SemicrfRecurrence(2, 5, 8, 1, 0, (65, 40, 8), (64, 40, 8), None, None))
+    assert lib.semicrf_recurrence_forward(p, good, 64, None, 64, 1 << 30, None) == bad
+
+
+def test_codes_at_an_odd_place_of_a_buffer_are_copied():
+    from torch_semimarkov_b200 import _lib
+
+    buffer = torch.arange(1 + 64, dtype=torch.int8)
+    codes = buffer[1:].view(1, 2, 32)
+    assert codes.data_ptr() % 8 != 0 and codes.is_contiguous()
+    kept = _lib.aligned_codes(codes)
+    assert kept.data_ptr() % 8 == 0 and torch.equal(kept, codes)
+    assert _lib.aligned_codes(kept) is kept

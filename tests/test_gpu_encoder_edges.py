@@ -233,3 +233,25 @@ def test_norm_gate_of_minus_infinity_closes_the_branch(dtype):
     assert torch.equal(r, x) and torch.equal(n, tsm.rms_norm(x, w[2]))
     _, gz, gg = torch.autograd.grad((r, n), leaves, (x.detach(), z.detach()))
     assert float(gz.abs().max()) <= 1e-30 and float(gg.abs().max()) <= 1e-30
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("at", [1, 3, 4, 8])
+def test_checkpoints_at_any_place_of_a_buffer(dtype, at):
+    """Codes and scales as slices of one byte buffer, as a file would hold them."""
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(70)
+    x, dy = _normal(g, 2, 30, 72, dtype=dtype), _normal(g, 2, 30, 48, dtype=dtype)
+    p = tsm.pack_activation(x)
+    n = p.codes.numel()
+    buffer = torch.zeros(at + n + p.scales.numel(), dtype=torch.uint8, device=_dev())
+    codes = buffer[at:at + n].view(torch.int8).view(p.codes.shape)
+    scales = buffer[at + n:].view(p.scales.shape)
+    codes.copy_(p.codes), scales.copy_(p.scales)
+    q = tsm.PackedActivation(codes, scales, p.channels, p.dtype)
+    assert torch.equal(p.unpack(), q.unpack())
+    assert torch.equal(tsm.packed_weight_grad(dy, p), tsm.packed_weight_grad(dy, q))
+    w = _normal(g, 48, 72).requires_grad_(True)
+    a, b = (torch.autograd.grad(tsm.packed_linear(x, w, packed=k), w, dy)[0] for k in (p, q))
+    assert torch.equal(a, b)

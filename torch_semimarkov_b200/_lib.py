@@ -743,6 +743,12 @@ def packed_buffers(B: int, T: int, D: int, device):
             torch.empty((B, T, G), dtype=torch.uint8, device=device))
 
 
+def aligned_codes(codes: torch.Tensor) -> torch.Tensor:
+    """The codes where the kernels can read them: on a multiple of 8 bytes (copied
+    where they are a slice of a buffer at another place)."""
+    return codes if codes.data_ptr() % 8 == 0 else codes.clone()
+
+
 def block_norm_forward(residual, branch, gate, branch_weight, residual_scale, next_weight,
                        lengths, eps, want_statistics, pack):
     """semicrf_block_norm_forward.  Returns (residual_out or None without a
@@ -806,6 +812,7 @@ def pack(x, lengths):
 def unpack(codes, scales, D: int, dtype):
     """semicrf_unpack.  Returns the (B, T, D) values."""
     lib = load()
+    codes = aligned_codes(codes)
     B, T = codes.shape[:2]
     dev = codes.device
     with _on(dev):
@@ -820,6 +827,7 @@ def unpack(codes, scales, D: int, dtype):
 def packed_weight_grad(grad_output, codes, scales, D: int, packed_dtype, lengths, out_dtype):
     """semicrf_packed_weight_grad.  Returns the (M, D) gradient."""
     lib = load()
+    codes = aligned_codes(codes)
     B, T, M = grad_output.shape
     dev = grad_output.device
     dt = ACTIVATION_DTYPES[grad_output.dtype]

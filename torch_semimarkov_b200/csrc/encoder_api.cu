@@ -2,6 +2,8 @@
 // (include/semicrf.h).  Each validates its arguments before any CUDA call and
 // enqueues kernels on the given stream; nothing allocates or synchronises.
 
+#include <initializer_list>
+
 #include "encoder_internal.cuh"
 
 using namespace semicrf;
@@ -52,6 +54,16 @@ int check_norm_inputs(const semicrf_block_norm* p) {
   return SEMICRF_OK;
 }
 
+// What the kernels read and write codes by: half a group's 16 bytes or less.
+bool codes_aligned(const int8_t* codes) { return reinterpret_cast<uintptr_t>(codes) % 8 == 0; }
+
+// Whether every tensor starts on a multiple of its element's size.
+bool elements_aligned(int dtype, std::initializer_list<const semicrf_sequence*> list) {
+  for (const semicrf_sequence* s : list)
+    if (reinterpret_cast<uintptr_t>(s->data) % (dtype == SEMICRF_F32 ? 4 : 2)) return false;
+  return true;
+}
+
 cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 
 }  // namespace
@@ -74,6 +86,7 @@ int semicrf_recurrence_forward(const semicrf_recurrence* p, const semicrf_sequen
   if (p->batch == 0) return SEMICRF_OK;
   if (!h || !final_state) return SEMICRF_ERR_INVALID_ARGUMENT;
   if (p->T && (!p->x.data || !p->gate.data || !h->data)) return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!elements_aligned(p->dtype, {&p->x, &p->gate, h})) return SEMICRF_ERR_INVALID_ARGUMENT;
   const size_t need = recurrence_workspace_bytes(p);
   if (workspace_bytes < need || (need && !workspace)) return SEMICRF_ERR_WORKSPACE;
   return recurrence_forward(p, *h, final_state, saved, workspace, as_stream(stream));
@@ -89,6 +102,8 @@ int semicrf_recurrence_backward(const semicrf_recurrence* p, const void* saved,
   if (p->batch == 0) return SEMICRF_OK;
   if (!grad_h || !grad_x || !grad_gate) return SEMICRF_ERR_INVALID_ARGUMENT;
   if (p->T && (!p->x.data || !p->gate.data || !grad_x->data || !grad_gate->data || !saved))
+    return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!elements_aligned(p->dtype, {&p->x, &p->gate, grad_h, grad_x, grad_gate}))
     return SEMICRF_ERR_INVALID_ARGUMENT;
   const size_t need = recurrence_workspace_bytes(p);
   if (workspace_bytes < need || (need && !workspace)) return SEMICRF_ERR_WORKSPACE;
@@ -118,6 +133,9 @@ int semicrf_block_norm_forward(const semicrf_block_norm* p, const semicrf_sequen
   if (!residual_out || !normed || !normed->data || (p->branch.data && !residual_out->data) ||
       !codes != !scales)
     return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!codes_aligned(codes) ||
+      !elements_aligned(p->dtype, {&p->residual, &p->branch, &p->gate, residual_out, normed}))
+    return SEMICRF_ERR_INVALID_ARGUMENT;
   return block_norm_forward(p, *residual_out, *normed, statistics, codes, scales,
                             as_stream(stream));
 }
@@ -143,6 +161,9 @@ int semicrf_block_norm_backward(const semicrf_block_norm* p, const float* statis
       (!statistics || !grad_residual->data ||
        (p->branch.data && (!grad_branch->data || !grad_gate->data))))
     return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!elements_aligned(p->dtype, {&p->residual, &p->branch, &p->gate, grad_residual_out, grad_normed,
+                                   grad_residual, grad_branch, grad_gate}))
+    return SEMICRF_ERR_INVALID_ARGUMENT;
   if (p->batch == 0 || p->T == 0)
     return cudaMemsetAsync(grad_weights, 0, sizeof(float) * 3 * p->D, as_stream(stream)) ==
                    cudaSuccess
@@ -161,6 +182,7 @@ int semicrf_pack(int64_t B, int64_t T, int64_t D, int dtype, const semicrf_seque
   if (st != SEMICRF_OK) return st;
   if (B == 0 || T == 0) return SEMICRF_OK;
   if (!x || !x->data || !codes || !scales) return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!codes_aligned(codes) || !elements_aligned(dtype, {x})) return SEMICRF_ERR_INVALID_ARGUMENT;
   return pack_rows(B, T, D, dtype, *x, lengths, codes, scales, as_stream(stream));
 }
 
@@ -169,7 +191,7 @@ int semicrf_unpack(int64_t rows, int64_t D, int dtype, const int8_t* codes,
   const int st = check_sizes(1, rows, D, dtype);
   if (st != SEMICRF_OK) return st;
   if (rows == 0) return SEMICRF_OK;
-  if (!codes || !scales || !out) return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!codes || !scales || !out || !codes_aligned(codes)) return SEMICRF_ERR_INVALID_ARGUMENT;
   return unpack_rows(rows, D, dtype, codes, scales, out, as_stream(stream));
 }
 
@@ -182,12 +204,15 @@ size_t semicrf_packed_weight_grad_workspace_size(int64_t B, int64_t T, int64_t D
 int semicrf_packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,
                                const semicrf_sequence* grad_output, const int8_t* codes,
                                const uint8_t* scales, int packed_dtype, const int64_t* lengths,
-                               int out_dtype, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+                               int out_dtype, void* out, void* workspace, size_t workspace_bytes,
+                               void* stream) {
   int st = check_sizes(B, T, D, dtype);
   if (st == SEMICRF_OK) st = M < 1 ? SEMICRF_ERR_INVALID_ARGUMENT : check_sizes(B, T, M, dtype);
   if (st != SEMICRF_OK) return st;
   if (!known_type(out_dtype) || !known_type(packed_dtype) || !out) return SEMICRF_ERR_INVALID_ARGUMENT;
   if (!grad_output || (B && T && (!grad_output->data || !codes || !scales)))
+    return SEMICRF_ERR_INVALID_ARGUMENT;
+  if (!codes_aligned(codes) || !elements_aligned(dtype, {grad_output}))
     return SEMICRF_ERR_INVALID_ARGUMENT;
   const size_t need = packed_weight_grad_workspace_bytes(B, T, D, M, dtype);
   if (workspace_bytes < need || !workspace) return SEMICRF_ERR_WORKSPACE;
