@@ -744,9 +744,10 @@ def packed_buffers(B: int, T: int, D: int, device):
 
 
 def aligned_codes(codes: torch.Tensor) -> torch.Tensor:
-    """The codes where the kernels can read them: on a multiple of 8 bytes (copied
-    where they are a slice of a buffer at another place)."""
-    return codes if codes.data_ptr() % 8 == 0 else codes.clone()
+    """The codes on a multiple of 16 bytes, copied where they are a slice of a
+    buffer at another place: the kernels read them 8 at a time, and by bulk copies
+    from such addresses only (a result must not depend on where codes lie)."""
+    return codes if codes.data_ptr() % 16 == 0 else codes.clone()
 
 
 def block_norm_forward(residual, branch, gate, branch_weight, residual_scale, next_weight,
