@@ -255,3 +255,41 @@ def test_checkpoints_at_any_place_of_a_buffer(dtype, at):
     w = _normal(g, 48, 72).requires_grad_(True)
     a, b = (torch.autograd.grad(tsm.packed_linear(x, w, packed=k), w, dy)[0] for k in (p, q))
     assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# infinite states
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("shift", [1.0, -30.0], ids=["gates near 0", "gates near -30"])
+@pytest.mark.parametrize("B,T,D", [(1, 9000, 4), (64, 150, 512)],
+                         ids=["segments", "one segment"])
+def test_recurrence_infinities_pass_every_position(B, T, D, shift, reverse):
+    """An infinite initial state, value or gradient stays infinite over any
+    number of positions, however small the product of their gates, and however
+    the positions are shared out: the formula's infinities, at its places."""
+    from test_gpu_encoder_ops import _lam_max, _recurrence_bounds
+
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(T + D)
+    inf = float("inf")
+    gate = _normal(g, B, T, D, shift=shift)
+    for what in ("state", "x", "grad"):
+        x, s0, dh, ds = (_normal(g, B, T, D), _normal(g, B, D), _normal(g, B, T, D),
+                         _normal(g, B, D))
+        scale = [t.clone() for t in (x, s0, dh, ds)]
+        if what == "state":
+            s0[:, 0], s0[:, 1] = inf, -inf
+        elif what == "x":
+            x[:, T // 3, 0], x[:, T // 2, 1] = inf, -inf
+        else:
+            ds[:, 0], dh[:, T // 2, 1] = inf, -inf
+        leaves = [t.requires_grad_(True) for t in (x, gate.clone(), s0)]
+        h, s = tsm.gated_linear_recurrence(*leaves[:2], s0, reverse=reverse)
+        got = (h, s, *torch.autograd.grad((h, s), leaves, (dh, ds)))
+        want = ref.recurrence(x, gate, s0, None, reverse, dh, ds)
+        tol = _recurrence_bounds(want, scale[0], scale[1], torch.float32, T,
+                                 _lam_max(x, gate, None, reverse, scale[2], scale[3]))
+        for v, k in zip(got, ("h", "state", "grad_x", "grad_gate", "grad_initial")):
+            ref.assert_within(v, want[k], torch.nan_to_num(tol[k], posinf=0.0), f"{what}: {k}")

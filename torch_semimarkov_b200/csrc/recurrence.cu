@@ -86,6 +86,16 @@ __device__ __forceinline__ Affine then(const Affine& a, const Affine& b) {  // b
   return Affine{__fmul2_rn(b.P, a.P), __ffma2_rn(b.P, a.S, b.S)};
 }
 
+// The product of a run as it is handed on: one too small for float32 stays above 0,
+// as every f is, so that an infinite state passes it as it passes the single steps
+// (0 times infinity would be NaN, and where runs end depends on the launch).  A
+// finite state is off by less than 5e-7 at 3e38.
+__device__ __forceinline__ float2 held_product(float2 P) {
+  asm("max.NaN.f32 %0, %0, 0f00000001;" : "+f"(P.x));
+  asm("max.NaN.f32 %0, %0, 0f00000001;" : "+f"(P.y));
+  return P;
+}
+
 // Where a CTA works, and how its rows lie in shared memory.  Pair lane + 32 j
 // is lane's j-th.  BULK: a lane's channels are neighbours, else 32 apart.
 template <class T, int H, bool BULK>
@@ -314,7 +324,8 @@ __device__ __forceinline__ float2 enter_segment(const ScanArgs<T>& a, const C& c
 }
 template <class T, class C>
 __device__ __forceinline__ void put_composed(const ScanArgs<T>& a, const C& col, const Affine& own) {
-  const float2 v[2] = {make_float2(own.P.x, own.S.x), make_float2(own.P.y, own.S.y)};
+  const float2 P = held_product(own.P);
+  const float2 v[2] = {make_float2(P.x, own.S.x), make_float2(P.y, own.S.y)};
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t d = col.channel(threadIdx.x, h);
@@ -400,6 +411,7 @@ __global__ void __launch_bounds__(Column<T, H, BULK>::kThreads, 2)
         Affine q = u[0][j];
 #pragma unroll
         for (int i = 1; i < kRun; ++i) q = then(q, u[i][j]);
+        q.P = held_product(q.P);
         part[turn][col.w][col.lane + 32 * j] = q;
       }
     compute_barrier();
@@ -506,6 +518,7 @@ __global__ void __launch_bounds__(Column<T, 1, BULK>::kThreads, 2)
       q.S = __fmul2_rn(f, __fadd2_rn(d[0], q.S));
     }
     ring.release(slot);
+    q.P = held_product(q.P);
     part[turn][col.w][col.lane] = q;
     compute_barrier();
     if (tid < PAIRS)
@@ -585,6 +598,7 @@ __global__ void __launch_bounds__(Column<T, 1, BULK>::kThreads, 2)
       float2 m = both(0.f);
 #pragma unroll
       for (int i = kRun - 1; i >= 0; --i) m = __fmul2_rn(f[i], __fadd2_rn(d[i], m));
+      q.P = held_product(q.P);
       part[turn][col.w][col.lane] = q;
       mpart[turn][col.w][col.lane] = m;
     }
