@@ -69,3 +69,69 @@ def test_codes_at_an_odd_place_of_a_buffer_are_copied():
     kept = _lib.aligned_codes(codes)
     assert kept.data_ptr() % 8 == 0 and torch.equal(kept, codes)
     assert _lib.aligned_codes(kept) is kept
+
+
+def _walk_with_marks(marked_f, marked_d):
+    """The recurrence's chunk as its computing warps walk it (8 warps of 8
+    positions, compositions handed on between them) for 4 channels, on inputs that
+    look valid, with the marks of a chunk that never came."""
+    g = torch.Generator().manual_seed(0)
+    warps, run, C = 8, 8, 4
+    f, x, d = (torch.rand(warps, run, C, generator=g) for _ in range(3))
+    n = 1 - f
+    nan = float("nan")
+    f[:, 0, marked_f] = nan
+    d[:, run - 1, marked_d] = nan
+    P, S, M = torch.ones(warps, C), torch.zeros(warps, C), torch.zeros(warps, C)
+    for i in range(run):
+        P, S = f[:, i] * P, f[:, i] * S + n[:, i] * x[:, i]
+    for i in reversed(range(run)):
+        M = f[:, i] * (d[:, i] + M)
+    h, dx, dg = (torch.empty(warps, run, C) for _ in range(3))
+    for w in range(warps):
+        state, mu = torch.ones(C), torch.ones(C)
+        for k in range(w):
+            state = P[k] * state + S[k]
+        for k in reversed(range(w + 1, warps)):
+            mu = P[k] * mu + M[k]
+        before = torch.empty(run, C)
+        for i in range(run):
+            before[i] = state
+            state = f[w, i] * state + n[w, i] * x[w, i]
+            h[w, i] = state
+        for i in reversed(range(run)):
+            lam = d[w, i] + mu
+            mu = f[w, i] * lam
+            dx[w, i] = lam * n[w, i]
+            dg[w, i] = mu * n[w, i] * (before[i] - x[w, i])
+    return h, dx, dg
+
+
+def test_marks_of_a_lost_chunk_reach_every_value():
+    """All channels of a lane have to be marked, and in the backward both ends of
+    a run; then no state and no gradient of the chunk is a number."""
+    every, none, one = slice(None), slice(0, 0), slice(0, 1)
+    h, dx, dg = _walk_with_marks(every, every)
+    assert torch.isnan(h).all() and torch.isnan(dx).all() and torch.isnan(dg).all()
+    h, dx, dg = _walk_with_marks(one, none)  # a mark on one channel leaves the others
+    assert not torch.isnan(h[..., 1:]).any() and not torch.isnan(dx).all()
+    h, dx, dg = _walk_with_marks(every, none)  # the state's marks alone miss dx
+    assert torch.isnan(h).all() and not torch.isnan(dx).all()
+
+
+def test_every_wait_for_a_chunk_marks_all_channels():
+    """In the recurrence's kernels: whatever waits for a chunk marks what comes
+    of it with mark_lost, and nothing marks half a pair."""
+    import os
+    import re
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    with open(os.path.join(here, "..", "torch_semimarkov_b200", "csrc", "recurrence.cu")) as file:
+        source = file.read()
+    waits = [m.start() for m in re.finditer(r"if \(ok\) ok = barrier_wait\(&full", source)]
+    assert len(waits) == 3
+    for at, end in zip(waits, waits[1:] + [len(source)]):
+        failed = source[source.index("if (!ok)", at, end):end]
+        assert "mark_lost(" in failed[:120]
+    assert not re.search(r"\.[xy] = __uint_as_float\(0x7fc00000u\)", source)
+    assert "mark_lost(f[0]), mark_lost(d[kRun - 1])" in source

@@ -96,6 +96,12 @@ __device__ __forceinline__ float2 held_product(float2 P) {
   return P;
 }
 
+// What becomes of values whose chunk never came: NaN in every channel of the lane.
+// Marked are the product of a run's first step, from which NaN reaches every later
+// state (and the run's composition, so every later run), and in the backward also
+// the gradient at the run's last position, from which it reaches every earlier one.
+__device__ __forceinline__ void mark_lost(float2& v) { v = both(__uint_as_float(0x7fc00000u)); }
+
 // Where a CTA works, and how its rows lie in shared memory.  Pair lane + 32 j
 // is lane's j-th.  BULK: a lane's channels are neighbours, else 32 apart.
 template <class T, int H, bool BULK>
@@ -404,7 +410,9 @@ __global__ void __launch_bounds__(Column<T, H, BULK>::kThreads, 2)
       }
     }
     ring.release(slot);
-    if (!ok) u[0][0].P.x = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+    if (!ok)
+#pragma unroll
+      for (int j = 0; j < H; ++j) mark_lost(u[0][j].P);
     if (COMPOSE || col.w < kParts)
 #pragma unroll
       for (int j = 0; j < H; ++j) {
@@ -505,7 +513,8 @@ __global__ void __launch_bounds__(Column<T, 1, BULK>::kThreads, 2)
     const int64_t t0 = col.chunk_time(a, c);
     if (ok) ok = barrier_wait(&full[slot], (unsigned)(it / STAGES) & 1);
     const unsigned char *dt = ring.tile(slot, 0), *gt = ring.tile(slot, 1);
-    Affine q{both(ok ? 1.f : __uint_as_float(0x7fc00000u)), both(0.f)};
+    Affine q{both(1.f), both(0.f)};
+    if (!ok) mark_lost(q.P);
 #pragma unroll
     for (int i = kRun - 1; i >= 0; --i) {
       const int r = col.row(a, i);
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(Column<T, 1, BULK>::kThreads, 2)
       if (off(i)) f[i] = both(1.f), n[i] = x[i] = d[i] = both(0.f);
     }
     ring.release(slot);
-    if (!ok) f[0].x = __uint_as_float(0x7fc00000u);  // a copy that never came shows as NaN
+    if (!ok) mark_lost(f[0]), mark_lost(d[kRun - 1]);
     {
       Affine q{f[0], __fmul2_rn(n[0], x[0])};
 #pragma unroll
