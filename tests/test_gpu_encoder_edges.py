@@ -293,3 +293,47 @@ def test_recurrence_infinities_pass_every_position(B, T, D, shift, reverse):
                                  _lam_max(x, gate, None, reverse, scale[2], scale[3]))
         for v, k in zip(got, ("h", "state", "grad_x", "grad_gate", "grad_initial")):
             ref.assert_within(v, want[k], torch.nan_to_num(tol[k], posinf=0.0), f"{what}: {k}")
+
+
+# ---------------------------------------------------------------------------
+# forward-mode differentiation
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_tangents_are_refused_not_lost(grad_mode):
+    """The operators have no forward-mode derivative; an input with a tangent is
+    an error wherever it stands, whether or not it requires a gradient.  The plain
+    product of packed_linear has one and keeps it."""
+    import torch.autograd.forward_ad as fw
+
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(80)
+    x, dy = _normal(g, 2, 9, 16), _normal(g, 2, 9, 16)
+    w, s, wm = _normal(g, 16), _normal(g, 2, 16), _normal(g, 8, 16)
+    p = tsm.pack_activation(x)
+    with torch.set_grad_enabled(grad_mode), fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t.clone(), torch.ones_like(t))
+
+        calls = [lambda: tsm.gated_linear_recurrence(dual(x), x),
+                 lambda: tsm.gated_linear_recurrence(x, dual(x)),
+                 lambda: tsm.gated_linear_recurrence(x, x, dual(s)),
+                 lambda: tsm.gated_linear_recurrence_step(dual(x[:, 0]), x[:, 0], s),
+                 lambda: tsm.gated_linear_recurrence_step(x[:, 0], x[:, 0], dual(s)),
+                 lambda: tsm.rms_norm(dual(x), w), lambda: tsm.rms_norm(x, dual(w)),
+                 lambda: tsm.pack_activation(dual(x)),
+                 lambda: tsm.packed_weight_grad(dual(dy), p)]
+        for k in range(6):
+            v = [x, x, x, w, w, w]
+            v[k] = dual(v[k])
+            calls.append(lambda v=tuple(v): tsm.gated_residual_norm(*v))
+        for k, call in enumerate(calls):
+            with pytest.raises(NotImplementedError):
+                call()
+        y = tsm.packed_linear(dual(x), wm)
+        torch.testing.assert_close(fw.unpack_dual(y).tangent, torch.ones_like(x) @ wm.t())
+        # without a tangent the calls are what they are outside
+        h, _ = tsm.gated_linear_recurrence(x, x)
+        n = tsm.rms_norm(x, w)
+    assert torch.equal(h, tsm.gated_linear_recurrence(x, x)[0])
+    assert torch.equal(n, tsm.rms_norm(x, w))

@@ -16,6 +16,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsemicrf.so")
@@ -642,6 +643,28 @@ def _on(device):
     if device.index is None or device.index == torch.cuda.current_device():
         return _SAME_DEVICE
     return torch.cuda.device(device)
+
+
+def has_tangent(tensors) -> bool:
+    """Whether forward-mode differentiation is under way and one of the tensors
+    (None among them) carries a tangent."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def recorded(*tensors) -> bool:
+    """Whether a call on these tensors has to go through its autograd function:
+    one requires a gradient, or carries a forward-mode tangent, which the function
+    refuses and a plain launch would lose."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return has_tangent(tensors)
+
+
+def refuse_tangents(name: str, *tensors):
+    """For what has no derivative: an error in place of a tangent lost."""
+    if has_tangent(tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def first_order(backward):

@@ -70,7 +70,7 @@ def _call(residual, branch, gate, branch_weight, residual_scale, next_weight, le
                            dev)
     lengths = _lib.valid_lengths(lengths, B, T, dev)
     given = (residual, branch, gate, branch_weight, residual_scale, next_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+    if _lib.recorded(*given):
         out, normed, codes, scales = _BlockNorm.apply(*given, (w1, scale, w2), lengths, eps,
                                                        bool(pack))
     else:

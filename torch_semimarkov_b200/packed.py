@@ -60,8 +60,10 @@ def _check(p: PackedActivation):
 
 def pack_activation(x: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> PackedActivation:
     """Store x (batch, T, channels) in 8 bits.  Positions past a sequence's
-    length are stored as zeros, whatever they hold."""
+    length are stored as zeros, whatever they hold.  No gradient passes through a
+    checkpoint: what is read back stands apart from x."""
     x = _lib.activation(x, "x")
+    _lib.refuse_tangents("pack_activation", x)
     lengths = _lib.valid_lengths(lengths, x.shape[0], x.shape[1], x.device)
     codes, scales = _lib.pack(x, lengths)
     return PackedActivation(codes, scales, x.shape[2], x.dtype)
@@ -72,9 +74,11 @@ def packed_weight_grad(grad_output: torch.Tensor, packed: PackedActivation,
                        dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Weight gradient of y = x W^T from x's checkpoint: the (M, channels) sum
     over valid positions of grad_output (batch, T, M)^T x, summed in float32
-    and returned as ``dtype`` (grad_output's type if None)."""
+    and returned as ``dtype`` (grad_output's type if None).  The result is not
+    differentiable."""
     _check(packed)
     grad_output = _lib.activation(grad_output, "grad_output")
+    _lib.refuse_tangents("packed_weight_grad", grad_output)
     B, T, _ = grad_output.shape
     if packed.codes.shape[:2] != (B, T) or packed.codes.device != grad_output.device:
         raise ValueError(f"packed holds {tuple(packed.shape)} on {packed.codes.device}, "

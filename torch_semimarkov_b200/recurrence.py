@@ -75,13 +75,10 @@ def gated_linear_recurrence(
     gate = _lib.activation(gate, "gate", like=x)
     B, T, D = x.shape
     lengths = _lib.valid_lengths(lengths, B, T, x.device)
-    needs_grad = torch.is_grad_enabled() and (
-        x.requires_grad or gate.requires_grad
-        or (initial_state is not None and initial_state.requires_grad))
     s0 = None
     if initial_state is not None:
         s0 = _lib.float_vector(initial_state, "initial_state", (B, D), x.device)
-    if needs_grad:
+    if _lib.recorded(x, gate, initial_state):
         return _GatedLinearRecurrence.apply(x, gate, initial_state, (s0,), lengths, bool(reverse))
     h, state, _ = _lib.recurrence_forward(x, gate, s0, lengths, reverse, want_saved=False)
     return h, state
@@ -132,4 +129,5 @@ def gated_linear_recurrence_step(
         x = x.contiguous()
     if gate.stride(1) != 1:
         gate = gate.contiguous()
+    _lib.refuse_tangents("gated_linear_recurrence_step", x, gate, state)
     return _lib.recurrence_step(x, gate, state, active, out_state)
