@@ -337,3 +337,42 @@ def test_forward_mode_tangents_are_refused_not_lost(grad_mode):
         n = tsm.rms_norm(x, w)
     assert torch.equal(h, tsm.gated_linear_recurrence(x, x)[0])
     assert torch.equal(n, tsm.rms_norm(x, w))
+
+
+# ---------------------------------------------------------------------------
+# packed_linear
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("trained", [True, False])
+@pytest.mark.parametrize("how", ["rows", "slices", "time first"])
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+def test_packed_linear_rounds_once(dtype, how, trained):
+    """Product and bias are rounded together: at most half a unit of the result
+    (and 64 float32 steps of what is summed), not half a unit of the product more."""
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(90)
+    B, T, D, M = 2, 200, 64, 96
+    x = _normal(g, B, T, 3 * D, dtype=dtype)[..., D:2 * D]
+    x = {"rows": x.contiguous(), "slices": x, "time first": x.transpose(0, 1).contiguous()
+         .transpose(0, 1)}[how]
+    w = _normal(g, M, D, scale=D ** -0.5, dtype=dtype).requires_grad_(trained)
+    b = _normal(g, M, dtype=dtype).requires_grad_(trained)
+    y = tsm.packed_linear(x, w, b).detach().double()
+    assert y.shape == (B, T, M)
+    xd, wd, bd = (t.detach().double() for t in (x, w, b))
+    want = xd @ wd.t() + bd
+    tol = ref.UNIT[dtype] * want.abs() + (D + 1) * ref.U32 * (xd.abs() @ wd.abs().t() + bd.abs())
+    assert ((y - want).abs() <= tol + ref.TINY[dtype]).all()
+
+
+def test_packed_linear_without_positions():
+    import torch_semimarkov_b200 as tsm
+
+    w = torch.ones(3, 8, device=_dev(), requires_grad=True)
+    b = torch.ones(3, device=_dev(), requires_grad=True)
+    for shape in ((0, 5, 8), (2, 0, 8)):
+        x = torch.empty(shape, device=_dev(), requires_grad=True)
+        y = tsm.packed_linear(x, w, b)
+        assert y.shape == (*shape[:2], 3)
+        for v in torch.autograd.grad(y.sum(), (x, w, b)):
+            assert not v.any()

@@ -91,13 +91,20 @@ def packed_weight_grad(grad_output: torch.Tensor, packed: PackedActivation,
                                    packed.dtype, lengths, dtype)
 
 
+def _linear(x, weight, bias):
+    """x weight^T + bias in x's type: one product whose sums take the bias before
+    they are rounded."""
+    w = weight.to(x.dtype)
+    if bias is None:
+        return torch.matmul(x, w.t())
+    B, T, D = x.shape
+    return torch.addmm(bias.to(x.dtype), x.reshape(B * T, D), w.t()).view(B, T, w.shape[0])
+
+
 class _PackedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, packed, lengths):
-        w = weight.to(x.dtype)
-        y = torch.matmul(x, w.t())
-        if bias is not None:
-            y += bias.to(x.dtype)
+        y = _linear(x, weight, bias)
         ctx.save_for_backward(weight, packed.codes, packed.scales, lengths)
         ctx.packed_dtype = packed.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
@@ -146,8 +153,7 @@ def packed_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     needs = torch.is_grad_enabled() and (weight.requires_grad or x.requires_grad
                                          or (bias is not None and bias.requires_grad))
     if not needs:
-        y = torch.matmul(x, weight.to(x.dtype).t())
-        return y if bias is None else y + bias.to(x.dtype)
+        return _linear(x, weight, bias)
     if packed is None:
         packed = pack_activation(x, lengths)
     else:
