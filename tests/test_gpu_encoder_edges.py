@@ -199,6 +199,22 @@ def test_encoder_padding_reaches_no_gradient(dtype, packed):
             assert torch.isfinite(b).all() and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_encoder_padding_reaches_no_output_of_inference(dtype):
+    import torch_semimarkov_b200 as tsm
+
+    g = _gen(52)
+    B, T, n = 3, 40, torch.tensor([40, 13, 0])
+    live = ref.live_mask(n, B, T).to(_dev())[..., None]
+    x = _normal(g, B, T, 7)
+    enc = tsm.GatedRecurrentEncoder(7, 24, dtype=dtype).to(_dev())
+    trained = enc(x, n).detach()
+    with torch.no_grad():
+        for how in (0.0, float("nan"), float("-inf")):
+            y = enc(torch.where(live, x, torch.full_like(x, how)), n)
+            assert torch.equal(y, trained) and not y[~live[..., 0]].any()
+
+
 # ---------------------------------------------------------------------------
 # gates at the ends of their types
 # ---------------------------------------------------------------------------

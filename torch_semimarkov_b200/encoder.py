@@ -92,10 +92,11 @@ class GatedRecurrentEncoder(nn.Module):
         if lengths is not None:
             B, T = x.shape[:2]
             lengths = _lib.valid_lengths(lengths, B, T, x.device)
-            # the embedding's weight gradient is a product over all positions, and
-            # a zero gradient times what padding may hold need not be zero
-            padding = torch.arange(T, device=x.device) >= lengths[:, None]
-            x = x.masked_fill(padding[..., None], 0.0)
+            if torch.is_grad_enabled():
+                # the embedding's weight gradient is a product over all positions,
+                # and a zero gradient times what padding may hold need not be zero
+                padding = torch.arange(T, device=x.device) >= lengths[:, None]
+                x = x.masked_fill(padding[..., None], 0.0)
         r = F.linear(x, self.embed.weight.to(x.dtype), self.embed.bias.to(x.dtype))
         pack = self.checkpoint_8bit and torch.is_grad_enabled()
         packed = None
