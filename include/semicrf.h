@@ -313,7 +313,8 @@ int semicrf_unpack(int64_t rows, int64_t D, int dtype, const int8_t* codes,
 /* Gradient of a linear layer's weight from its input's checkpoint:
  * out (M, D) = sum over valid positions of grad_output^T x, grad_output
  * (B, T, M) of type dtype, the checkpoint made of a tensor of type
- * packed_dtype, out of type out_dtype. */
+ * packed_dtype, out of type out_dtype.  Tensor cores, which truncate, sum at
+ * most 2,048 positions; beyond that sums are rounded float32 additions. */
 size_t semicrf_packed_weight_grad_workspace_size(int64_t B, int64_t T, int64_t D, int64_t M,
                                                  int dtype);
 int semicrf_packed_weight_grad(int64_t B, int64_t T, int64_t D, int64_t M, int dtype,

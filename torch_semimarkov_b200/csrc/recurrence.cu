@@ -20,8 +20,7 @@
 // positions of a chunk, a lane H pairs of channels.  Each warp composes its
 // positions, one barrier a chunk makes the compositions known, and each warp
 // goes from the state that entered the chunk over the earlier warps' to its
-// own start.  Products and sums go two channels to an instruction: issue slots
-// are what comes next after DRAM.
+// own start.  Products and sums go two channels to an instruction.
 //
 // One or two more warps keep a ring of chunks of every input on their way to
 // shared memory, so that nothing waits in registers.  Rows on 16-byte
@@ -40,13 +39,16 @@
 // Every order of operations depends on sizes alone.
 //
 // Measured, bfloat16: batch 64 of 10^4 positions with ragged lengths, 512
-// channels, forward 317 us and backward 650 us, where their bytes (3 and 5
-// values an element) take 255 and 425 at the device's copy rate.  The backward
-// is short of issue slots: a sigmoid pair, two walks over a run and two stores
-// an element.  One sequence of 10^6 positions: composing 369 us, walking 518 us,
-// whose own bytes take 315 and 473.  Rows without 16-byte alignment (64 x 5,000
-// x 203): 217 and 418 us, where 208 channels take 124 and 193; their elements
-// are loaded, converted and stored one by one.
+// channels, forward 317 us and backward 645 us, where their bytes (3 and 5
+// values an element) take 255 and 425 at the device's copy rate; float32, half
+// the batch, 292 and 550 us for the same bytes.  The backward's 512 columns are
+// 1.73 waves of CTAs; counted over both (64 x 1,500 x 512) 63% of issue slots and
+// 47% of DRAM are used, and what its 18 warps an SM wait for most is the fixed
+// latency of their own chains of steps.  One sequence of 10^6 positions: composing
+// 355 us, walking 508 us, whose own bytes take 315 and 473.  Rows without 16-byte
+// alignment (64 x 5,000 x 203): 217 and 418 us, 3.6 and 4.2 times their bytes (208
+// channels take 124 and 193); their elements are loaded, converted and stored one
+// by one.
 
 #include <algorithm>
 #include <type_traits>
@@ -705,7 +707,8 @@ struct Cut {
 // Segments: one, or as many as fill the SMs with one CTA or with two, whichever
 // is the least by this measure: a CTA's chunks, 1.6 times as slow where two
 // share an SM, and with segments `compose` times the walk on top (0.7 forward,
-// 0.35 backward).  Measured at 16 bits, us for one / few / many segments:
+// 0.35 backward).  Measured on aligned 16-bit rows and used for all types and
+// alignments, us for one / few / many segments:
 // forward of 128 columns of 4000 positions 99 / - / 136, of 64 columns of
 // 20000 495 / 406 / 315; backward of 64 columns of 40000 - / 733 / 524.
 Cut cut_of(int64_t B, int64_t T, int64_t D, int tile, float compose) {
